@@ -21,16 +21,16 @@
 #include "../../include/gqa_fa_b200.h"
 #include "attn_pair_kernel.cuh"
 #include "attn_dkv_kernel.cuh"
+#include "api_shared.cuh"
 
 namespace gqafa {
 
 __device__ int g_status_word;
 
-namespace {
+static thread_local std::string g_last_error;
 
-thread_local std::string g_last_error;
+void clear_error() { g_last_error.clear(); }
 
-int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int fail(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
@@ -40,6 +40,8 @@ int fail(int code, const char* fmt, ...) {
   g_last_error = buf;
   return code;
 }
+
+namespace {
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -109,6 +111,8 @@ int encode_map(CUtensorMap* m, const TensorDesc& t, int B, int N, int D, int box
   return GQAFA_OK;
 }
 
+}  // namespace
+
 // Make the device of `stream` (or the current device for the legacy stream)
 // current on this thread with its primary context bound. Needed because the
 // caller may run on a thread where no context is current yet (for example the
@@ -123,12 +127,19 @@ int bind_device(cudaStream_t stream) {
   return GQAFA_OK;
 }
 
+namespace {
+
 // Diagnostics buffer (WC_NUM counters) set by gqafa_set_wait_counters; null = off.
 std::atomic<unsigned long long*> g_prof_buffer{nullptr};
 // Test knobs set by gqafa_set_test_waits: the launches' wait bound and the
 // switch that keeps the TMA producers idle.
 std::atomic<long long> g_wait_limit{WAIT_LIMIT_CYCLES};
 std::atomic<int> g_no_loads{0};
+
+}  // namespace
+
+long long wait_limit_setting() { return g_wait_limit.load(std::memory_order_relaxed); }
+int no_loads_setting() { return g_no_loads.load(std::memory_order_relaxed); }
 
 int* status_ptr() {
   static std::mutex mu;
@@ -143,6 +154,8 @@ int* status_ptr() {
   }
   return ptrs[dev];
 }
+
+namespace {
 
 template <class C>
 // maps: R1, R2, C1, C2, Y and (pair kernels) the workspace store map; an

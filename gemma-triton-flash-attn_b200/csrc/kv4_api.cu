@@ -1,0 +1,447 @@
+// Host side of the paged 4-bit KV cache's C ABI (include/gqa_fa_b200.h):
+// argument validation, variant choice and launches of the kernels in
+// kv4_cache_kernels.cuh and kv4_attn_kernel.cuh.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <cmath>
+#include <cstring>
+
+#include "../../include/gqa_fa_b200.h"
+#include "api_shared.cuh"
+#include "kv4_attn_kernel.cuh"
+#include "kv4_cache_kernels.cuh"
+
+namespace gqafa {
+namespace {
+
+int log2_of(int v) {
+  int s = 0;
+  while ((1 << s) < v) ++s;
+  return s;
+}
+
+int check_cache(int heads_kv, int head_dim, int page_size, int dtype) {
+  if (heads_kv <= 0) return fail(GQAFA_ERR_INVALID, "heads_kv must be positive, got %d", heads_kv);
+  if (dtype != GQAFA_DTYPE_FP16 && dtype != GQAFA_DTYPE_BF16)
+    return fail(GQAFA_ERR_INVALID, "dtype code %d is not fp16 (0) or bf16 (1)", dtype);
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256 && head_dim != 512)
+    return fail(GQAFA_ERR_UNSUPPORTED, "head_dim %d is not implemented on sm_100a (supported: 64, 128, 256, 512)",
+                head_dim);
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
+    return fail(GQAFA_ERR_UNSUPPORTED, "page_size %d is not implemented (supported: 16, 32, 64, 128, 256)", page_size);
+  return GQAFA_OK;
+}
+
+int check_pages(const void* pages, long long num_pages, int page_size) {
+  if (pages == nullptr) return fail(GQAFA_ERR_INVALID, "pages: null pointer");
+  if (reinterpret_cast<uintptr_t>(pages) % 16 != 0)
+    return fail(GQAFA_ERR_INVALID, "pages: data pointer must be 16-byte aligned");
+  if (num_pages <= 0 || num_pages * page_size > INT_MAX)
+    return fail(GQAFA_ERR_INVALID, "num_pages %lld out of range (num_pages * page_size must be in 1..2^31-1)", num_pages);
+  return GQAFA_OK;
+}
+
+int check_ints(const char* name, const void* p) {
+  if (p == nullptr) return fail(GQAFA_ERR_INVALID, "%s: null pointer", name);
+  if (reinterpret_cast<uintptr_t>(p) % 4 != 0) return fail(GQAFA_ERR_INVALID, "%s must be 4-byte aligned", name);
+  return GQAFA_OK;
+}
+
+int check_table(const void* table, long long stride, int cols, int page_size) {
+  int rc = check_ints("block_table", table);
+  if (rc) return rc;
+  if (cols <= 0 || static_cast<long long>(cols) * page_size > INT_MAX - 4096)
+    return fail(GQAFA_ERR_INVALID, "block_table: %d columns out of range", cols);
+  if (stride < 0) return fail(GQAFA_ERR_INVALID, "block_table: negative row stride");
+  return GQAFA_OK;
+}
+
+// A [B, H, N, D] tensor with 16-byte rows; strides of size-1 dims are ignored.
+int check_rows(const char* name, const void* ptr, const long long* st, int B, int H, int N, long long* out) {
+  if (ptr == nullptr) return fail(GQAFA_ERR_INVALID, "%s: null pointer", name);
+  if (st == nullptr) return fail(GQAFA_ERR_INVALID, "%s: null strides", name);
+  if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0)
+    return fail(GQAFA_ERR_INVALID, "%s: data pointer must be 16-byte aligned", name);
+  if (st[3] != 1) return fail(GQAFA_ERR_INVALID, "%s: last (head_dim) stride must be 1, got %lld", name, st[3]);
+  const int size[3] = {B, H, N};
+  for (int i = 0; i < 3; ++i) {
+    out[i] = size[i] == 1 ? 0 : st[i];
+    if (out[i] < 0 || out[i] % 8 != 0)
+      return fail(GQAFA_ERR_INVALID, "%s: strides must be multiples of 8 elements (16 bytes), got (%lld, %lld, %lld, %lld)",
+                  name, st[0], st[1], st[2], st[3]);
+  }
+  return GQAFA_OK;
+}
+
+int sm_count() {
+  static std::atomic<int> counts[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  int n = counts[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    counts[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+int launch_status(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(GQAFA_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
+  return GQAFA_OK;
+}
+
+struct AttendShape {
+  int B, Hq, Hkv, N, D, G;
+  int NT, rows, row_tiles, ctas;
+};
+
+// Query rows of a unit (8 * NT), row tiles and CTAs. G * N rows up to 8 and 16
+// take one row tile of that height; more rows take tiles of 32.
+AttendShape attend_shape(int B, int Hq, int Hkv, int N, int D, int max_len, int window, int sms) {
+  AttendShape s{};
+  s.B = B;
+  s.Hq = Hq;
+  s.Hkv = Hkv;
+  s.N = N;
+  s.D = D;
+  s.G = Hq / Hkv;
+  const long long rows = static_cast<long long>(s.G) * N;
+  s.NT = rows <= 8 ? 1 : (rows <= 16 ? 2 : 4);
+  s.rows = 8 * s.NT;
+  s.row_tiles = static_cast<int>((rows + s.rows - 1) / s.rows);
+  const int tile_tokens = 8 * 16 * kv4_warp_blocks(D, s.NT);
+  long long span = max_len;
+  if (window > 0) span = std::min<long long>(span, static_cast<long long>(window) + s.rows / s.G + 1);
+  const long long tiles = (span + 15 + tile_tokens - 1) / tile_tokens + 1;
+  const long long units = static_cast<long long>(B) * s.row_tiles * Hkv;
+  s.ctas = static_cast<int>(std::min<long long>(static_cast<long long>(sms) * (s.NT == 1 ? 2 : 1), units * tiles));
+  return s;
+}
+
+long long attend_workspace(const AttendShape& s) {
+  return 2LL * s.ctas * s.rows * (static_cast<long long>(s.D) * 4 + 8) + 256;
+}
+
+template <class C>
+int launch_attend(Kv4Params p, cudaStream_t st) {
+  static std::atomic<unsigned long long> attr_done_mask{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return fail(GQAFA_ERR_CUDA, "cudaGetDevice failed");
+  const unsigned long long bit = 1ULL << (dev & 63);
+  if (!(attr_done_mask.load() & bit)) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kv4_attn_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+    if (e != cudaSuccess) return fail(GQAFA_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    attr_done_mask.fetch_or(bit);
+  }
+  const long long rows_here = std::min<long long>(C::ROWS, static_cast<long long>(p.G) * p.N);
+  const long long blocks =
+      static_cast<long long>(p.B) * p.row_tiles * p.Hkv * rows_here * (C::D < 128 ? 1 : C::D / 128);
+  if (blocks > INT_MAX) return fail(GQAFA_ERR_INVALID, "grid size %lld out of range", blocks);
+  kv4_attn_kernel<C><<<p.ctas, C::THREADS, C::SMEM_BYTES, st>>>(p);
+  int rc = launch_status("4-bit cache attention");
+  if (rc) return rc;
+  // The join starts while the attention's last CTAs run (programmatic
+  // dependent launch): it reads the lengths and then waits for them.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_combine_kernel<C>, static_cast<const Kv4Params>(p));
+  if (e != cudaSuccess) return fail(GQAFA_ERR_CUDA, "4-bit cache join launch: %s", cudaGetErrorString(e));
+  return GQAFA_OK;
+}
+
+template <int D, bool BF16>
+int attend_rows(int nt, const Kv4Params& p, cudaStream_t st) {
+  if (nt == 1) return launch_attend<Kv4Cfg<D, 1, BF16>>(p, st);
+  if (nt == 2) return launch_attend<Kv4Cfg<D, 2, BF16>>(p, st);
+  return launch_attend<Kv4Cfg<D, 4, BF16>>(p, st);
+}
+
+template <bool BF16>
+int attend_dim(int D, int nt, const Kv4Params& p, cudaStream_t st) {
+  switch (D) {
+    case 64: return attend_rows<64, BF16>(nt, p, st);
+    case 128: return attend_rows<128, BF16>(nt, p, st);
+    case 256: return attend_rows<256, BF16>(nt, p, st);
+    default: return attend_rows<512, BF16>(nt, p, st);
+  }
+}
+
+int check_attend(int batch, int heads_q, int heads_kv, int seqlen_q, int head_dim, int page_size, int dtype) {
+  int rc = check_cache(heads_kv, head_dim, page_size, dtype);
+  if (rc) return rc;
+  if (batch <= 0 || heads_q <= 0 || seqlen_q <= 0)
+    return fail(GQAFA_ERR_INVALID, "sizes must be positive (B=%d H_Q=%d N=%d)", batch, heads_q, seqlen_q);
+  if (heads_q % heads_kv != 0)
+    return fail(GQAFA_ERR_INVALID, "H_Q (%d) must be a multiple of H_KV (%d)", heads_q, heads_kv);
+  if (static_cast<long long>(batch) * heads_q * seqlen_q > INT_MAX / 2)
+    return fail(GQAFA_ERR_INVALID, "B * H_Q * N out of range");
+  return GQAFA_OK;
+}
+
+}  // namespace
+}  // namespace gqafa
+
+using namespace gqafa;
+
+extern "C" long long gqafa_kv4_page_bytes(int heads_kv, int head_dim, int page_size) {
+  clear_error();
+  if (check_cache(heads_kv, head_dim, page_size, GQAFA_DTYPE_BF16)) return -1;
+  return 2LL * heads_kv * (page_size / KV4_TOKENS) * kv4_block_bytes(head_dim);
+}
+
+extern "C" int gqafa_kv4_plan(const int* kv_lens, const int* new_lens, const int* block_table, long long table_stride,
+                              int* free_pages, const int* free_state, int batch, int cols, int num_free,
+                              int page_size, int max_new, int* out_block_table, int* out_kv_lens, int* out_new_lens,
+                              int* out_slot_map, int* out_positions, int* out_accepted, int* out_free_state,
+                              void* stream) {
+  clear_error();
+  int rc;
+  if ((rc = check_cache(1, 64, page_size, GQAFA_DTYPE_BF16))) return rc;
+  if (batch <= 0 || max_new <= 0)
+    return fail(GQAFA_ERR_INVALID, "sizes must be positive (B=%d max_new=%d)", batch, max_new);
+  if ((rc = check_table(block_table, table_stride, cols, page_size))) return rc;
+  if (num_free <= 0 || static_cast<long long>(num_free) * page_size > INT_MAX)
+    return fail(GQAFA_ERR_INVALID, "free_pages: %d entries out of range (entries * page_size must be in 1..2^31-1)",
+                num_free);
+  const void* ints[] = {kv_lens, new_lens, free_pages, free_state, out_block_table, out_kv_lens,
+                        out_new_lens, out_slot_map, out_positions, out_accepted, out_free_state};
+  const char* names[] = {"kv_lens", "new_lens", "free_pages", "free_state", "out_block_table", "out_kv_lens",
+                         "out_new_lens", "out_slot_map", "out_positions", "out_accepted", "out_free_state"};
+  for (int i = 0; i < 11; ++i)
+    if ((rc = check_ints(names[i], ints[i]))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = bind_device(st))) return rc;
+  Kv4PlanParams p{};
+  p.kv_lens = kv_lens;
+  p.new_lens = new_lens;
+  p.table = block_table;
+  p.table_stride = table_stride;
+  p.free_pages = free_pages;
+  p.free_state = free_state;
+  p.B = batch;
+  p.cols = cols;
+  p.F = num_free;
+  p.page = page_size;
+  p.page_shift = log2_of(page_size);
+  p.max_new = max_new;
+  p.out_table = out_block_table;
+  p.out_kv_lens = out_kv_lens;
+  p.out_new_lens = out_new_lens;
+  p.out_slots = out_slot_map;
+  p.out_positions = out_positions;
+  p.out_accepted = out_accepted;
+  p.out_state = out_free_state;
+  kv4_plan_kernel<<<batch, 256, 0, st>>>(p);
+  return launch_status("plan");
+}
+
+extern "C" int gqafa_kv4_append(const void* k, const long long* k_strides, const void* v, const long long* v_strides,
+                                const int* slot_map, long long slot_stride, void* pages, long long num_pages,
+                                int batch, int heads_kv, int seqlen, int head_dim, int page_size, int dtype,
+                                void* stream) {
+  clear_error();
+  int rc;
+  if ((rc = check_cache(heads_kv, head_dim, page_size, dtype))) return rc;
+  if (batch <= 0 || seqlen <= 0) return fail(GQAFA_ERR_INVALID, "sizes must be positive (B=%d N=%d)", batch, seqlen);
+  if ((rc = check_pages(pages, num_pages, page_size))) return rc;
+  if ((rc = check_ints("slot_map", slot_map))) return rc;
+  if (slot_stride < 0) return fail(GQAFA_ERR_INVALID, "slot_map: negative row stride");
+  Kv4AppendParams p{};
+  long long s[3];
+  const void* src[2] = {k, v};
+  const long long* strides[2] = {k_strides, v_strides};
+  for (int i = 0; i < 2; ++i) {
+    if ((rc = check_rows(i ? "v" : "k", src[i], strides[i], batch, heads_kv, seqlen, s))) return rc;
+    p.x[i] = static_cast<const uint16_t*>(src[i]);
+    p.sb[i] = s[0];
+    p.sh[i] = s[1];
+    p.sn[i] = s[2];
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = bind_device(st))) return rc;
+  p.slots = slot_map;
+  p.slots_stride = slot_stride;
+  p.pages = static_cast<uint8_t*>(pages);
+  p.B = batch;
+  p.N = seqlen;
+  p.Hkv = heads_kv;
+  p.page_shift = log2_of(page_size);
+  p.num_slots = num_pages * page_size;
+  p.status = status_ptr();
+  if (!p.status) return fail(GQAFA_ERR_CUDA, "cannot resolve the device status word");
+  const long long octets = static_cast<long long>(batch) * seqlen * heads_kv * (head_dim / KV4_GROUP);
+  const dim3 grid(static_cast<unsigned>(std::min<long long>((octets + 31) / 32, 1 << 20)), 2);
+  const bool bf16 = dtype == GQAFA_DTYPE_BF16;
+#define GQAFA_LAUNCH(DIM)                                   \
+  if (bf16)                                                 \
+    kv4_append_kernel<DIM, true><<<grid, 256, 0, st>>>(p);  \
+  else                                                      \
+    kv4_append_kernel<DIM, false><<<grid, 256, 0, st>>>(p); \
+  break
+  switch (head_dim) {
+    case 64: GQAFA_LAUNCH(64);
+    case 128: GQAFA_LAUNCH(128);
+    case 256: GQAFA_LAUNCH(256);
+    default: GQAFA_LAUNCH(512);
+  }
+#undef GQAFA_LAUNCH
+  return launch_status("append");
+}
+
+extern "C" int gqafa_kv4_read(const void* pages, long long num_pages, const int* block_table, long long table_stride,
+                              int cols, const int* kv_lens, const int* starts, void* k, void* v, int batch,
+                              int heads_kv, int seqlen, int head_dim, int page_size, int dtype, void* stream) {
+  clear_error();
+  int rc;
+  if ((rc = check_cache(heads_kv, head_dim, page_size, dtype))) return rc;
+  if (batch <= 0 || seqlen <= 0) return fail(GQAFA_ERR_INVALID, "sizes must be positive (B=%d n=%d)", batch, seqlen);
+  if ((rc = check_pages(pages, num_pages, page_size))) return rc;
+  if ((rc = check_table(block_table, table_stride, cols, page_size))) return rc;
+  if ((rc = check_ints("kv_lens", kv_lens))) return rc;
+  if (starts && (rc = check_ints("starts", starts))) return rc;
+  void* out[2] = {k, v};
+  for (int i = 0; i < 2; ++i)
+    if (out[i] == nullptr || reinterpret_cast<uintptr_t>(out[i]) % 16 != 0)
+      return fail(GQAFA_ERR_INVALID, "outputs must be 16-byte aligned");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = bind_device(st))) return rc;
+  Kv4ReadParams p{};
+  p.pages = static_cast<const uint8_t*>(pages);
+  p.table = block_table;
+  p.table_stride = table_stride;
+  p.kv_lens = kv_lens;
+  p.starts = starts;
+  p.out[0] = static_cast<uint16_t*>(k);
+  p.out[1] = static_cast<uint16_t*>(v);
+  p.B = batch;
+  p.Hkv = heads_kv;
+  p.n = seqlen;
+  p.cols = cols;
+  p.page_shift = log2_of(page_size);
+  p.num_pages = static_cast<int>(num_pages);
+  p.status = status_ptr();
+  if (!p.status) return fail(GQAFA_ERR_CUDA, "cannot resolve the device status word");
+  const int NG = head_dim / KV4_GROUP;
+  // n tokens from any start touch at most (n + 15 + 15) / 16 blocks
+  const long long items = ((seqlen + 30LL) / 16) * NG;
+  const long long xblocks = (items + 7) / 8, blocks = xblocks * batch * heads_kv;
+  if (blocks > INT_MAX) return fail(GQAFA_ERR_INVALID, "grid size %lld out of range", blocks);
+  p.xblocks = static_cast<int>(xblocks);
+  const dim3 grid(static_cast<unsigned>(blocks), 2);
+  const bool bf16 = dtype == GQAFA_DTYPE_BF16;
+#define GQAFA_LAUNCH(DIM)                                 \
+  if (bf16)                                               \
+    kv4_read_kernel<DIM, true><<<grid, 256, 0, st>>>(p);  \
+  else                                                    \
+    kv4_read_kernel<DIM, false><<<grid, 256, 0, st>>>(p); \
+  break
+  switch (head_dim) {
+    case 64: GQAFA_LAUNCH(64);
+    case 128: GQAFA_LAUNCH(128);
+    case 256: GQAFA_LAUNCH(256);
+    default: GQAFA_LAUNCH(512);
+  }
+#undef GQAFA_LAUNCH
+  return launch_status("read");
+}
+
+extern "C" long long gqafa_kv4_attend_workspace_size(int batch, int heads_q, int heads_kv, int seqlen_q, int head_dim,
+                                                     int max_kv_len, int window) {
+  clear_error();
+  if (check_attend(batch, heads_q, heads_kv, seqlen_q, head_dim, 16, GQAFA_DTYPE_BF16)) return -1;
+  if (max_kv_len < 0 || window < 0) {
+    fail(GQAFA_ERR_INVALID, "max_kv_len and window must be >= 0");
+    return -1;
+  }
+  const int sms = sm_count();
+  if (sms <= 0) {
+    fail(GQAFA_ERR_CUDA, "cannot read the device's multiprocessor count");
+    return -1;
+  }
+  return attend_workspace(attend_shape(batch, heads_q, heads_kv, seqlen_q, head_dim, max_kv_len, window, sms));
+}
+
+extern "C" int gqafa_kv4_attend(const void* q, const long long* q_strides, const void* pages, long long num_pages,
+                                const int* block_table, long long table_stride, int cols, const int* kv_lens,
+                                const int* q_lens, void* o, const long long* o_strides, float* lse, int batch,
+                                int heads_q, int heads_kv, int seqlen_q, int head_dim, int page_size, int max_kv_len,
+                                float softmax_scale, int causal, int window, int dtype, void* workspace,
+                                long long workspace_bytes, void* stream) {
+  clear_error();
+  int rc;
+  if ((rc = check_attend(batch, heads_q, heads_kv, seqlen_q, head_dim, page_size, dtype))) return rc;
+  if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale))
+    return fail(GQAFA_ERR_INVALID, "softmax_scale must be positive and finite");
+  if (window < 0) return fail(GQAFA_ERR_INVALID, "window must be >= 0");
+  if ((rc = check_pages(pages, num_pages, page_size))) return rc;
+  if ((rc = check_table(block_table, table_stride, cols, page_size))) return rc;
+  if ((rc = check_ints("kv_lens", kv_lens))) return rc;
+  if (q_lens && (rc = check_ints("q_lens", q_lens))) return rc;
+  if (lse && reinterpret_cast<uintptr_t>(lse) % 4 != 0) return fail(GQAFA_ERR_INVALID, "lse must be 4-byte aligned");
+  long long qs[3], os[3];
+  if ((rc = check_rows("q", q, q_strides, batch, heads_q, seqlen_q, qs))) return rc;
+  if ((rc = check_rows("o", o, o_strides, batch, heads_q, seqlen_q, os))) return rc;
+  const long long capacity = static_cast<long long>(cols) * page_size;
+  if (max_kv_len < 0) return fail(GQAFA_ERR_INVALID, "max_kv_len must be >= 0");
+  if (max_kv_len == 0 || max_kv_len > capacity) max_kv_len = static_cast<int>(capacity);
+  const int win = causal ? window : 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = bind_device(st))) return rc;
+  const int sms = sm_count();
+  if (sms <= 0) return fail(GQAFA_ERR_CUDA, "cannot read the device's multiprocessor count");
+  const AttendShape s = attend_shape(batch, heads_q, heads_kv, seqlen_q, head_dim, max_kv_len, win, sms);
+  const long long need = attend_workspace(s);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(GQAFA_ERR_INVALID, "workspace of %lld bytes needed, got %lld", need, workspace_bytes);
+  if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
+    return fail(GQAFA_ERR_INVALID, "workspace must be 256-byte aligned");
+  Kv4Params p{};
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_sb = qs[0];
+  p.q_sh = qs[1];
+  p.q_sn = qs[2];
+  p.o = static_cast<uint16_t*>(o);
+  p.o_sb = os[0];
+  p.o_sh = os[1];
+  p.o_sn = os[2];
+  p.lse = lse;
+  p.pages = static_cast<const uint8_t*>(pages);
+  p.table = block_table;
+  p.table_stride = table_stride;
+  p.kv_lens = kv_lens;
+  p.q_lens = q_lens;
+  p.B = batch;
+  p.Hq = heads_q;
+  p.Hkv = heads_kv;
+  p.G = s.G;
+  p.N = seqlen_q;
+  p.cols = cols;
+  p.page_shift = log2_of(page_size);
+  p.num_pages = static_cast<int>(num_pages);
+  p.causal = causal ? 1 : 0;
+  p.window = win;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.row_tiles = s.row_tiles;
+  p.ctas = s.ctas;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) +
+                                        2LL * s.ctas * s.rows * static_cast<long long>(s.D) * 4);
+  p.status = status_ptr();
+  if (!p.status) return fail(GQAFA_ERR_CUDA, "cannot resolve the device status word");
+  p.wait_limit = wait_limit_setting();
+  p.no_loads = no_loads_setting();
+  return dtype == GQAFA_DTYPE_BF16 ? attend_dim<true>(head_dim, s.NT, p, st)
+                                   : attend_dim<false>(head_dim, s.NT, p, st);
+}

@@ -1,0 +1,841 @@
+// Attention of a few new tokens over the paged 4-bit KV cache (kv4_layout.cuh):
+//
+//   O[n] = sum_j softmax_j(scale * q_n . k_j) v_j over the keys j that the
+//   causal mask and the window leave to token n, k and v read from the codes.
+//
+// Mathematics. With k = s (c - z) per group of 64 dims, a group's part of a
+// score is s * (q . (16 + c) - (16 + z) * sum(q)): the 16-bit number 16 + c is
+// one AND-OR of a shifted code word (the code becomes the top four mantissa
+// bits), so the codes go into the MMAs without a conversion, and scale and
+// zero point are applied once per group to the fp32 result. On the value side
+// P' = round16(s * P) is the B operand and 16 + c the A operand; the term
+// sum_j (16 + z_j) P'_j is one more MMA with the same rounded P', so the
+// offset cancels exactly and only P' itself is rounded.
+//
+// Shape. A decode step has G = H_Q / H_KV query rows per KV head, far below
+// the 128 rows of a tcgen05 tile, and reads each cached byte once: it is bound
+// by HBM. The products therefore run transposed on m16n8k16 MMAs with the
+// CACHE as the A operand (16 tokens, or 16 dims, by 8 query rows): padding
+// costs at most 8 rows, and the codes go from shared memory to registers to
+// the tensor cores without a dequantised copy in between.
+//
+// One CTA: eight compute warps and one producer warp. The producer walks the
+// block table and brings whole blocks (codes and scales together) into a ring
+// of stages with bulk copies. Work is cut into tiles of TB blocks. Scores: warp
+// w takes blocks w, w + 8, ... over all of head_dim, with its own running
+// maximum; P goes to shared memory (fp32), one barrier per tile. Values: warp
+// (dim group, slice) takes 64 dims of every NG-th block, so the output
+// accumulator is 16 registers per 8 query rows; it rescales P by
+// exp2(m_warp - M), M the maximum over the eight warps.
+//
+// Split. The tiles of all (request, row tile, KV head) units form one list,
+// cut into equal contiguous shares, one per CTA: ragged lengths and a single
+// long request both fill the GPU. A unit inside one share is written straight
+// to the output; parts of a cut unit go to a workspace (fp32, with maximum and
+// sum) and kv4_combine_kernel joins them in list order, so results do not
+// depend on timing.
+#pragma once
+#include "kv4_layout.cuh"
+#include "ptx_sm100.cuh"
+
+namespace gqafa {
+
+struct Kv4Params {
+  const uint16_t* q;
+  long long q_sb, q_sh, q_sn;
+  uint16_t* o;
+  long long o_sb, o_sh, o_sn;
+  float* lse;  // [B, Hq, N] or null
+  const uint8_t* pages;
+  const int* table;  // [B][cols]
+  long long table_stride;
+  const int* kv_lens;
+  const int* q_lens;  // [B] or null (N)
+  int B, Hq, Hkv, G, N;
+  int cols, page_shift, num_pages;  // page_shift: log2 of the page's tokens
+  int causal, window;
+  float scale_log2;
+  int row_tiles;  // row tiles (8 * NT rows each) of G * N rows
+  int ctas;       // CTAs of the attention launch (the combine launch needs it)
+  float* part_o;  // [2 * ctas][8 * NT][D]
+  float2* part_ml;  // [2 * ctas][8 * NT]: maximum (log2 units), sum
+  int* status;
+  long long wait_limit;
+  int no_loads;
+};
+
+// Blocks per warp and tile: enough work between barriers at small head_dim,
+// within the shared memory that P takes (it grows with the rows).
+__host__ __device__ constexpr int kv4_warp_blocks(int D, int NT) {
+  return D >= 256 ? 1 : (D == 128 || NT > 1 ? 2 : 4);
+}
+
+template <int D_, int NT_, bool BF16_>
+struct Kv4Cfg {
+  static constexpr int D = D_, NT = NT_;
+  static constexpr bool BF16 = BF16_;
+  static constexpr int ROWS = 8 * NT;         // query rows of a unit
+  static constexpr int NG = D / KV4_GROUP;    // groups of a token
+  static constexpr int KS = 8 / NG;           // value-side slices of a tile's blocks
+  static constexpr int KB = kv4_warp_blocks(D, NT);
+  static constexpr int TB = 8 * KB;           // blocks per tile
+  static constexpr int SB = TB / 2;           // blocks per stage
+  static constexpr int BLOCK_BYTES = kv4_block_bytes(D);
+  static constexpr int STAGE_BYTES = SB * BLOCK_BYTES;
+  static constexpr int Q_PITCH = D * 2 + 16;  // bytes; +16: fragment loads hit all banks
+  static constexpr int Q_BYTES = ROWS * Q_PITCH;
+  static constexpr int SUMQ_BYTES = NG * ROWS * 4;
+  static constexpr int P_PITCH = 20;          // floats of a row's 16 probabilities
+  static constexpr int P_BYTES = TB * ROWS * P_PITCH * 4;  // one of two buffers
+  static constexpr int M_BYTES = 8 * ROWS * 4;             // one of two buffers
+  static constexpr int MISC_BYTES = 2 * P_BYTES + 2 * M_BYTES + Q_BYTES + SUMQ_BYTES + ROWS * 8 + 256;
+  static constexpr int CTAS_PER_SM = NT == 1 ? 2 : 1;
+  static constexpr int SMEM_BUDGET = CTAS_PER_SM == 2 ? 115000 : 232448;
+  static constexpr int NST_FIT = (SMEM_BUDGET - MISC_BYTES) / STAGE_BYTES;
+  static constexpr int NST = NST_FIT < 12 ? NST_FIT : 12;
+  static constexpr int SMEM_BYTES = NST * STAGE_BYTES + MISC_BYTES;
+  static constexpr int THREADS = 288;
+  static_assert(NST >= 4, "two stages of keys and two of values");
+  // the slices' sums are joined through the P buffers
+  static_assert(KS == 1 || (KS / 2) * ROWS * D * 4 <= 2 * P_BYTES, "slice exchange");
+};
+
+// One unit's keys: tiles of blocks [b0, b0 + nblk) of request b.
+struct Kv4Unit {
+  int b, rt, len, qlen;
+  int b0, nblk, tiles;
+};
+
+template <class C>
+__device__ __forceinline__ Kv4Unit kv4_unit(const Kv4Params& p, int entry) {
+  Kv4Unit u;
+  u.b = entry / p.row_tiles;
+  u.rt = entry - u.b * p.row_tiles;
+  const int capacity = p.cols << p.page_shift;
+  u.len = min(max(p.kv_lens[u.b], 0), capacity);
+  u.qlen = p.q_lens ? min(max(p.q_lens[u.b], 0), p.N) : p.N;
+  u.b0 = u.nblk = u.tiles = 0;
+  const int r0 = u.rt * C::ROWS, rows = p.G * u.qlen;
+  if (r0 >= rows) return u;
+  const int n0 = r0 / p.G, n1 = (min(r0 + C::ROWS, rows) - 1) / p.G;
+  const int off = u.len - u.qlen;
+  const int hi = p.causal ? min(u.len, off + n1 + 1) : u.len;
+  const int lo = (p.causal && p.window > 0) ? max(0, off + n0 - p.window + 1) : 0;
+  if (hi <= lo) return u;
+  u.b0 = lo >> 4;
+  u.nblk = ((hi + 15) >> 4) - u.b0;
+  u.tiles = (u.nblk + C::TB - 1) / C::TB;
+  return u;
+}
+
+// Position of a CTA's share in the list of tiles: entries in order, the KV
+// heads of an entry one after the other.
+struct Kv4Share {
+  int entry;      // entry that holds the share's first tile
+  int base;       // index of that entry's first tile
+  int total;      // tiles in all
+};
+
+// Block-wide (NTHR threads): total number of tiles, and the entry that holds
+// tile `per * index` with per = ceil(total / ctas). Every thread gets the
+// result. `scratch`: 40 ints of shared memory.
+template <class C, int NTHR>
+__device__ __forceinline__ Kv4Share kv4_find(const Kv4Params& p, int index, int* scratch) {
+  const int entries = p.B * p.row_tiles;
+  const int each = (entries + NTHR - 1) / NTHR;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int e0 = min(entries, static_cast<int>(threadIdx.x) * each), e1 = min(entries, e0 + each);
+  int sum = 0;
+  for (int e = e0; e < e1; ++e) sum += kv4_unit<C>(p, e).tiles * p.Hkv;
+  int s = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += u;
+  }
+  if (lane == 31) scratch[warp] = s;
+  if (threadIdx.x == 0) {
+    scratch[32] = 0;
+    scratch[33] = 0;
+  }
+  __syncthreads();
+  int before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < NTHR / 32; ++w) {
+    const int v = scratch[w];
+    if (w < warp) before += v;
+    total += v;
+  }
+  const int first = before + s - sum;
+  const int per = max(1, (total + p.ctas - 1) / p.ctas);
+  const long long at = static_cast<long long>(per) * index;
+  if (at >= first && at < first + sum) {
+    int base = first;
+    for (int e = e0; e < e1; ++e) {
+      const int t = kv4_unit<C>(p, e).tiles * p.Hkv;
+      if (at < base + t) {
+        scratch[32] = e;
+        scratch[33] = base;
+        break;
+      }
+      base += t;
+    }
+  }
+  __syncthreads();
+  Kv4Share r;
+  r.entry = scratch[32];
+  r.base = scratch[33];
+  r.total = total;
+  return r;
+}
+
+// ------------------------------------------------------------------ fragments
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  if constexpr (BF16) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+}
+
+// 16 + code for nibble I of both 16-bit halves of w: in [16, 32) the code is
+// the top four mantissa bits (bf16 bits 3..6, fp16 bits 6..9).
+template <bool BF16, int I>
+__device__ __forceinline__ uint32_t code16(uint32_t w) {
+  constexpr int SH = (BF16 ? 3 : 6) - 4 * I;
+  const uint32_t x = SH >= 0 ? (w << (SH >= 0 ? SH : 0)) : (w >> (SH < 0 ? -SH : 0));
+  return BF16 ? ((x & 0x00780078u) | 0x41804180u) : ((x & 0x03C003C0u) | 0x4C004C00u);
+}
+// -(16 + zero point) of two packed meta words, as 16-bit numbers.
+template <bool BF16>
+__device__ __forceinline__ uint32_t minus_zero16(uint32_t w) {
+  const uint32_t z = w & 0x000F000Fu;
+  return BF16 ? ((z << 3) | 0xC180C180u) : ((z << 6) | 0xCC00CC00u);
+}
+__device__ __forceinline__ float scale_lo(uint32_t w) { return __uint_as_float((w << 16) & 0xFFF00000u); }
+__device__ __forceinline__ float scale_hi(uint32_t w) { return __uint_as_float(w & 0xFFF00000u); }
+// 16 + zero point in fp32.
+__device__ __forceinline__ float zero_lo(uint32_t w) { return __uint_as_float(0x41800000u | ((w & 0xFu) << 19)); }
+__device__ __forceinline__ float zero_hi(uint32_t w) { return __uint_as_float(0x41800000u | ((w & 0xF0000u) << 3)); }
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+      "r"(bytes), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+__device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
+
+template <class C>
+__global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(const Kv4Params p) {
+  constexpr int D = C::D, NT = C::NT, NG = C::NG, KS = C::KS, KB = C::KB, TB = C::TB, SB = C::SB, ROWS = C::ROWS;
+  constexpr int NST = C::NST, BB = C::BLOCK_BYTES, PP = C::P_PITCH;
+  constexpr bool BF16 = C::BF16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* sRing = smem;
+  float* sP = reinterpret_cast<float*>(smem + NST * C::STAGE_BYTES);  // [2][TB][ROWS][PP]
+  float* sM = sP + 2 * C::P_BYTES / 4;                                 // [2][8 warps][ROWS]
+  uint8_t* sQ = reinterpret_cast<uint8_t*>(sM + 2 * 8 * ROWS);         // [ROWS] rows of Q_PITCH bytes
+  float* sSum = reinterpret_cast<float*>(sQ + C::Q_BYTES);             // [NG][ROWS]
+  int2* sMask = reinterpret_cast<int2*>(sSum + NG * ROWS);             // [ROWS]: first key, number of keys
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sMask + ROWS);
+  __shared__ int scratch[40];
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t bar0 = smem_u32(bars);
+  auto FULL = [&](int s) { return bar0 + 8u * s; };
+  auto EMPTY = [&](int s) { return bar0 + 8u * (NST + s); };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NST; ++s) {
+      mbar_init(FULL(s), 1);
+      mbar_init(EMPTY(s), 8);
+    }
+    abort_word = 0;
+    fence_mbar_init();
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const Kv4Share share = kv4_find<C, C::THREADS>(p, blockIdx.x, scratch);  // also orders the barrier setup
+  const int per = max(1, (share.total + p.ctas - 1) / p.ctas);
+  const long long begin = static_cast<long long>(per) * blockIdx.x;
+  if (begin >= share.total) return;
+  const int first_tile = static_cast<int>(begin);
+  const int last_tile = min(share.total, first_tile + per);
+
+  // Walk the pieces of the share: f(unit, entry's first tile, head, tile
+  // range inside the unit). Producer and compute warps walk the same way.
+  auto pieces = [&](auto&& f) {
+    int entry = share.entry, base = share.base, at = first_tile;
+    while (at < last_tile) {
+      const Kv4Unit u = kv4_unit<C>(p, entry);
+      const int end = base + u.tiles * p.Hkv;
+      while (at < end && at < last_tile) {
+        const int h = (at - base) / u.tiles;
+        const int t0 = (at - base) - h * u.tiles;
+        const int t1 = min(u.tiles, t0 + (last_tile - at));
+        f(u, h, t0, t1);
+        at += t1 - t0;
+      }
+      base = end;
+      ++entry;
+    }
+  };
+
+  if (warp == 8) {
+    // ======================= producer =======================
+    if (p.no_loads) return;
+    uint32_t cnt = 0;
+    bool ok = true;
+    const int bpp_shift = p.page_shift - 4, bpp_mask = (1 << bpp_shift) - 1;
+    pieces([&](const Kv4Unit& u, int h, int t0, int t1) {
+      const int* row = p.table + u.b * p.table_stride;
+      // lane's page of the tile's block `lane`; the next tile's is fetched ahead
+      auto page_at = [&](int tile) -> int {
+        const int a = u.b0 + tile * TB + lane;
+        return (tile < t1 && lane < TB && tile * TB + lane < u.nblk) ? __ldg(row + (a >> bpp_shift)) : 0;
+      };
+      int next = page_at(t0);
+      for (int tile = t0; tile < t1; ++tile) {
+        int page = next;
+        next = page_at(tile + 1);
+        if (page < 0 || page >= p.num_pages) {
+          atomicCAS(p.status, 0, ST_KV4_PAGE);
+          page = 0;  // stays in bounds; the status word tells
+        }
+        const int nv = min(TB, u.nblk - tile * TB);  // blocks of this tile
+        const int a = u.b0 + tile * TB + lane;
+        const int off = a & bpp_mask;
+#pragma unroll
+        for (int st4 = 0; st4 < 4; ++st4) {  // keys: two stages, values: two stages
+          const int kind = st4 >> 1, half = st4 & 1;
+          const int slot = cnt % NST;
+          if (ok) ok = mbar_wait(EMPTY(slot), ((cnt / NST) & 1u) ^ 1u, abort_flag, p.status, ST_TIMEOUT_RING_EMPTY,
+                                 p.wait_limit);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) continue;
+          const int cn = min(max(nv - half * SB, 0), SB);  // blocks of this stage
+          if (lane == 0) {
+            if (cn > 0)
+              mbar_arrive_expect_tx(FULL(slot), cn * BB);
+            else
+              mbar_arrive(FULL(slot));
+          }
+          __syncwarp();
+          const int j = lane - half * SB;
+          // one copy for the blocks of a page that follow each other
+          if (j >= 0 && j < cn && (j == 0 || off == 0)) {
+            const int run = min(bpp_mask + 1 - off, cn - j);
+            const uint8_t* src = p.pages +
+                                 ((((static_cast<long long>(page) * 2 + kind) * p.Hkv + h) << bpp_shift) + off) * BB;
+            bulk_load(smem_u32(sRing + slot * C::STAGE_BYTES + j * BB), src, run * BB, FULL(slot));
+          }
+          ++cnt;
+        }
+      }
+    });
+    if (!ok) {
+      // aborted: the copies in flight land before the CTA's memory goes
+      for (uint32_t c = cnt > NST ? cnt - NST : 0; c < cnt; ++c) {
+        const long long t0 = clock64();
+        while (!mbar_try_wait(FULL(c % NST), (c / NST) & 1u) && clock64() - t0 < p.wait_limit) {
+        }
+      }
+    }
+    return;
+  }
+
+  // ======================= compute warps =======================
+  const int gid = lane >> 2, tig = lane & 3;
+  const int dg = warp % NG, ks = warp / NG;  // value side: dim group, slice of the blocks
+  uint32_t cnt = 0;
+  int buf = 0;
+  auto wait_full = [&](int slot, uint32_t c) {
+    mbar_wait(FULL(slot), (c / NST) & 1u, abort_flag, p.status, ST_TIMEOUT_RING_FULL, p.wait_limit);
+    __syncwarp();
+  };
+  auto release = [&](int slot) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(EMPTY(slot));
+  };
+
+  pieces([&](const Kv4Unit& u, int h, int t0, int t1) {
+    // ---- queries of the unit, their sums per group, the rows' key ranges
+    compute_barrier();  // the previous piece's readers are done
+    const int r0 = u.rt * ROWS, rows = p.G * u.qlen, off = u.len - u.qlen;
+    constexpr int CH = D / 8, RSTEP = 256 / CH;
+#pragma unroll 2
+    for (int i = threadIdx.x / CH; i < ROWS; i += RSTEP) {
+      const int c = threadIdx.x % CH, r = r0 + i;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < rows) {
+        const int n = r / p.G, hq = h * p.G + r - n * p.G;
+        v = *reinterpret_cast<const uint4*>(p.q + u.b * p.q_sb + hq * p.q_sh + n * p.q_sn + c * 8);
+      }
+      *reinterpret_cast<uint4*>(sQ + i * C::Q_PITCH + c * 16) = v;
+      float s = unpack_lo<BF16>(v.x) + unpack_hi<BF16>(v.x) + unpack_lo<BF16>(v.y) + unpack_hi<BF16>(v.y) +
+                unpack_lo<BF16>(v.z) + unpack_hi<BF16>(v.z) + unpack_lo<BF16>(v.w) + unpack_hi<BF16>(v.w);
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if ((c & 7) == 0) sSum[(c >> 3) * ROWS + i] = s;
+    }
+    if (threadIdx.x < ROWS) {
+      const int r = r0 + threadIdx.x;
+      int lo = 0, hi = 0;
+      if (r < rows) {
+        const int pos = off + r / p.G;
+        hi = p.causal ? min(u.len, pos + 1) : u.len;
+        lo = (p.causal && p.window > 0) ? max(0, pos - p.window + 1) : 0;
+      }
+      sMask[threadIdx.x] = make_int2(lo, max(0, hi - lo));
+    }
+    compute_barrier();
+    // keys that every row of the unit sees: [all_lo, all_hi) (what its padding rows see is not used)
+    const int nlast = (min(r0 + ROWS, rows) - 1) / p.G;
+    const int all_hi = p.causal ? min(u.len, off + r0 / p.G + 1) : u.len;
+    const int all_lo = (p.causal && p.window > 0) ? max(0, off + nlast - p.window + 1) : 0;
+
+    float acc[NT][4][4], wz[NT][4];
+    float m_run[NT][2], l_run[NT][2];  // score side: this warp's blocks, rows 2 tig, 2 tig + 1
+    float m_all[NT];                   // value side: row gid, over all warps
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        wz[nt][j] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[nt][j][e] = 0.f;
+      }
+      m_run[nt][0] = m_run[nt][1] = -INFINITY;
+      l_run[nt][0] = l_run[nt][1] = 0.f;
+      m_all[nt] = -INFINITY;
+    }
+
+    for (int tile = t0; tile < t1; ++tile) {
+      const int nv = min(TB, u.nblk - tile * TB);
+      const int key_tile = (u.b0 + tile * TB) * 16;
+      // ---------------- scores ----------------
+      float s[KB][NT][4];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int slot = cnt % NST;
+        wait_full(slot, cnt);
+        ++cnt;
+        const uint32_t stage = smem_u32(sRing + slot * C::STAGE_BYTES);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          const int blk = warp + 8 * kb;
+          if (blk / SB != half || blk >= nv) continue;
+          const uint32_t base = stage + (blk - half * SB) * BB;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[kb][nt][e] = 0.f;
+#pragma unroll(NG > 2 ? 2 : NG)
+          for (int g = 0; g < NG; ++g) {
+            const uint4 w = lds128(base + g * KV4_CODE_BYTES + lane * 16);
+            const uint32_t meta = lds32(base + NG * KV4_CODE_BYTES + g * KV4_META_BYTES + gid * 4);
+            const float s0 = scale_lo(meta), s1 = scale_hi(meta), z0 = zero_lo(meta), z1 = zero_hi(meta);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint32_t qa = smem_u32(sQ + (nt * 8 + gid) * C::Q_PITCH + g * 128 + tig * 32);
+              const uint4 q0 = lds128(qa), q1 = lds128(qa + 16);
+              float t[4] = {0.f, 0.f, 0.f, 0.f};
+              mma16816<BF16>(t, code16<BF16, 0>(w.x), code16<BF16, 0>(w.z), code16<BF16, 1>(w.x),
+                             code16<BF16, 1>(w.z), q0.x, q0.y);
+              mma16816<BF16>(t, code16<BF16, 2>(w.x), code16<BF16, 2>(w.z), code16<BF16, 3>(w.x),
+                             code16<BF16, 3>(w.z), q0.z, q0.w);
+              mma16816<BF16>(t, code16<BF16, 0>(w.y), code16<BF16, 0>(w.w), code16<BF16, 1>(w.y),
+                             code16<BF16, 1>(w.w), q1.x, q1.y);
+              mma16816<BF16>(t, code16<BF16, 2>(w.y), code16<BF16, 2>(w.w), code16<BF16, 3>(w.y),
+                             code16<BF16, 3>(w.w), q1.z, q1.w);
+              const float2 sq = *reinterpret_cast<const float2*>(sSum + g * ROWS + nt * 8 + 2 * tig);
+              s[kb][nt][0] = fmaf(s0, fmaf(-z0, sq.x, t[0]), s[kb][nt][0]);
+              s[kb][nt][1] = fmaf(s0, fmaf(-z0, sq.y, t[1]), s[kb][nt][1]);
+              s[kb][nt][2] = fmaf(s1, fmaf(-z1, sq.x, t[2]), s[kb][nt][2]);
+              s[kb][nt][3] = fmaf(s1, fmaf(-z1, sq.y, t[3]), s[kb][nt][3]);
+            }
+          }
+        }
+        release(slot);
+      }
+
+      // ---------------- softmax over this warp's blocks ----------------
+      float* P = sP + buf * (C::P_BYTES / 4);
+      float* M = sM + buf * 8 * ROWS;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int4 mk = *reinterpret_cast<const int4*>(sMask + nt * 8 + 2 * tig);  // two rows' (first, count)
+        float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          const int blk = warp + 8 * kb;
+          if (blk >= nv) continue;
+          const int key = key_tile + blk * 16 + gid;
+          const bool edge = (key_tile + blk * 16 < all_lo) || (key_tile + blk * 16 + 16 > all_hi);
+          float* v = s[kb][nt];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] *= p.scale_log2;
+          if (edge) {
+            if (static_cast<unsigned>(key - mk.x) >= static_cast<unsigned>(mk.y)) v[0] = -INFINITY;
+            if (static_cast<unsigned>(key - mk.z) >= static_cast<unsigned>(mk.w)) v[1] = -INFINITY;
+            if (static_cast<unsigned>(key + 8 - mk.x) >= static_cast<unsigned>(mk.y)) v[2] = -INFINITY;
+            if (static_cast<unsigned>(key + 8 - mk.z) >= static_cast<unsigned>(mk.w)) v[3] = -INFINITY;
+          }
+          mx0 = fmaxf(mx0, fmaxf(v[0], v[2]));
+          mx1 = fmaxf(mx1, fmaxf(v[1], v[3]));
+        }
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o));
+        }
+        const float n0 = fmaxf(m_run[nt][0], mx0), n1 = fmaxf(m_run[nt][1], mx1);
+        const float f0 = finite_or_zero(n0), f1 = finite_or_zero(n1);
+        float l0 = 0.f, l1 = 0.f;
+        const int perm = (gid >> 1) * 4 + (gid & 1);  // order (2t, 2t+1, 2t+8, 2t+9) of the value side
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          const int blk = warp + 8 * kb;
+          if (blk >= nv) continue;
+          float* v = s[kb][nt];
+          v[0] = ex2(v[0] - f0);
+          v[1] = ex2(v[1] - f1);
+          v[2] = ex2(v[2] - f0);
+          v[3] = ex2(v[3] - f1);
+          l0 += v[0] + v[2];
+          l1 += v[1] + v[3];
+          float* d = P + (blk * ROWS + nt * 8 + 2 * tig) * PP + perm;
+          d[0] = v[0];
+          d[2] = v[2];
+          d[PP] = v[1];
+          d[PP + 2] = v[3];
+        }
+        l_run[nt][0] = l_run[nt][0] * ex2(m_run[nt][0] - f0) + l0;
+        l_run[nt][1] = l_run[nt][1] * ex2(m_run[nt][1] - f1) + l1;
+        m_run[nt][0] = n0;
+        m_run[nt][1] = n1;
+        if (gid == 0) *reinterpret_cast<float2*>(M + warp * ROWS + nt * 8 + 2 * tig) = make_float2(n0, n1);
+      }
+      compute_barrier();
+
+      // ---------------- values ----------------
+      // Reference maximum of every row over the eight warps; the accumulators
+      // follow it when it grows.
+      float fm[NT], up[NT];
+      bool grew = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float m = m_all[nt];
+#pragma unroll
+        for (int w = 0; w < 8; ++w) m = fmaxf(m, M[w * ROWS + nt * 8 + gid]);
+        fm[nt] = finite_or_zero(m);
+        grew |= m > m_all[nt];
+        up[nt] = ex2(m_all[nt] - fm[nt]);
+        m_all[nt] = m;
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float a = up[nt];
+          const float a0 = __shfl_sync(0xffffffffu, a, 8 * tig), a1 = __shfl_sync(0xffffffffu, a, 8 * tig + 4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            acc[nt][j][0] *= a0;
+            acc[nt][j][1] *= a1;
+            acc[nt][j][2] *= a0;
+            acc[nt][j][3] *= a1;
+          }
+          wz[nt][0] *= a0;
+          wz[nt][1] *= a1;
+          wz[nt][2] *= a0;
+          wz[nt][3] *= a1;
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int slot = cnt % NST;
+        wait_full(slot, cnt);
+        ++cnt;
+        const uint32_t stage = smem_u32(sRing + slot * C::STAGE_BYTES);
+#pragma unroll(SB / KS > 4 ? 4 : SB / KS)
+        for (int i = 0; i < SB / KS; ++i) {
+          const int sblk = i * KS + ks, blk = half * SB + sblk;
+          if (blk >= nv) break;
+          const uint32_t base = stage + sblk * BB;
+          const uint2 mv = lds64(base + NG * KV4_CODE_BYTES + dg * KV4_META_BYTES + tig * 8);
+          const uint4 c = lds128(base + dg * KV4_CODE_BYTES + (tig * 8 + (gid ^ (2 * tig))) * 16);
+          const uint32_t m0 = __byte_perm(c.x, c.y, 0x5410), m1 = __byte_perm(c.x, c.y, 0x7632);
+          const uint32_t m2 = __byte_perm(c.z, c.w, 0x5410), m3 = __byte_perm(c.z, c.w, 0x7632);
+          const uint32_t nz0 = minus_zero16<BF16>(mv.x), nz1 = minus_zero16<BF16>(mv.y);
+          const float s0 = scale_lo(mv.x), s1 = scale_hi(mv.x), s2 = scale_lo(mv.y), s3 = scale_hi(mv.y);
+          const bool edge = (key_tile + blk * 16 < all_lo) || (key_tile + blk * 16 + 16 > all_hi);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint4 pr = lds128(smem_u32(P + (blk * ROWS + nt * 8 + gid) * PP + tig * 4));
+            const float f = ex2(M[(blk & 7) * ROWS + nt * 8 + gid] - fm[nt]);
+            float p0 = __uint_as_float(pr.x) * f, p1 = __uint_as_float(pr.y) * f;
+            float p2 = __uint_as_float(pr.z) * f, p3 = __uint_as_float(pr.w) * f;
+            if (edge) {
+              // a masked token's scale may be anything (a slot never written): its product must be 0
+              p0 = p0 == 0.f ? 0.f : p0 * s0;
+              p1 = p1 == 0.f ? 0.f : p1 * s1;
+              p2 = p2 == 0.f ? 0.f : p2 * s2;
+              p3 = p3 == 0.f ? 0.f : p3 * s3;
+            } else {
+              p0 *= s0;
+              p1 *= s1;
+              p2 *= s2;
+              p3 *= s3;
+            }
+            const uint32_t b0 = pack2<BF16>(p0, p1), b1 = pack2<BF16>(p2, p3);
+            mma16816<BF16>(acc[nt][0], code16<BF16, 0>(m0), code16<BF16, 1>(m0), code16<BF16, 0>(m2),
+                           code16<BF16, 1>(m2), b0, b1);
+            mma16816<BF16>(acc[nt][1], code16<BF16, 2>(m0), code16<BF16, 3>(m0), code16<BF16, 2>(m2),
+                           code16<BF16, 3>(m2), b0, b1);
+            mma16816<BF16>(acc[nt][2], code16<BF16, 0>(m1), code16<BF16, 1>(m1), code16<BF16, 0>(m3),
+                           code16<BF16, 1>(m3), b0, b1);
+            mma16816<BF16>(acc[nt][3], code16<BF16, 2>(m1), code16<BF16, 3>(m1), code16<BF16, 2>(m3),
+                           code16<BF16, 3>(m3), b0, b1);
+            mma16816<BF16>(wz[nt], nz0, nz0, nz1, nz1, b0, b1);
+          }
+        }
+        release(slot);
+      }
+      buf ^= 1;
+    }
+
+    // ---------------- epilogue of the piece ----------------
+    // sums of the eight warps' l, relative to the common maximum
+    compute_barrier();  // all value-side reads of P and M are done
+    float* xM = sM;             // [8][ROWS] maxima
+    float* xL = sM + 8 * ROWS;  // [8][ROWS] sums
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float l0 = l_run[nt][0], l1 = l_run[nt][1];
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+      }
+      if (gid == 0) {
+        *reinterpret_cast<float2*>(xM + warp * ROWS + nt * 8 + 2 * tig) = make_float2(m_run[nt][0], m_run[nt][1]);
+        *reinterpret_cast<float2*>(xL + warp * ROWS + nt * 8 + 2 * tig) = make_float2(l0, l1);
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[nt][j][e] += wz[nt][e];
+    // value-side slices: halve their number until one is left
+    if constexpr (KS > 1) {
+#pragma unroll
+      for (int live = KS / 2; live >= 1; live >>= 1) {
+        float* X = sP;
+        const int lane_at = ((dg * live + (ks % live)) * 32 + lane) * 4;
+        if (ks >= live && ks < 2 * live) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<float4*>(X + (nt * 4 + j) * (NG * live * 128) + lane_at) =
+                  make_float4(acc[nt][j][0], acc[nt][j][1], acc[nt][j][2], acc[nt][j][3]);
+        }
+        compute_barrier();
+        if (ks < live) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float4 v = *reinterpret_cast<const float4*>(X + (nt * 4 + j) * (NG * live * 128) + lane_at);
+              acc[nt][j][0] += v.x;
+              acc[nt][j][1] += v.y;
+              acc[nt][j][2] += v.z;
+              acc[nt][j][3] += v.w;
+            }
+        }
+        compute_barrier();
+      }
+    } else {
+      compute_barrier();
+    }
+    const bool whole = t0 == 0 && t1 == u.tiles;
+    const int part = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);  // a unit's later parts start a share
+    if (ks == 0) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {  // rows 2 tig, 2 tig + 1
+          const int i = nt * 8 + 2 * tig + e, r = r0 + i;
+          float m = -INFINITY, l = 0.f;
+#pragma unroll
+          for (int w = 0; w < 8; ++w) m = fmaxf(m, xM[w * ROWS + i]);
+#pragma unroll
+          for (int w = 0; w < 8; ++w) l += xL[w * ROWS + i] * ex2(xM[w * ROWS + i] - finite_or_zero(m));
+          // dims 64 dg + 8 gid + (0..7): MMA rows gid and gid + 8 of tile j are dims 2j and 2j + 1
+          if (whole) {
+            if (r < rows) {
+              const float inv = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
+              const int n = r / p.G, hq = h * p.G + r - n * p.G;
+              uint4 v;
+              v.x = pack2<BF16>(acc[nt][0][e] * inv, acc[nt][0][2 + e] * inv);
+              v.y = pack2<BF16>(acc[nt][1][e] * inv, acc[nt][1][2 + e] * inv);
+              v.z = pack2<BF16>(acc[nt][2][e] * inv, acc[nt][2][2 + e] * inv);
+              v.w = pack2<BF16>(acc[nt][3][e] * inv, acc[nt][3][2 + e] * inv);
+              *reinterpret_cast<uint4*>(p.o + u.b * p.o_sb + hq * p.o_sh + n * p.o_sn + dg * 64 + gid * 8) = v;
+              if (p.lse && dg == 0 && gid == 0)
+                p.lse[(static_cast<long long>(u.b) * p.Hq + hq) * p.N + n] =
+                    l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+            }
+          } else {
+            float* d = p.part_o + (static_cast<long long>(part) * ROWS + i) * D + dg * 64 + gid * 8;
+            *reinterpret_cast<float4*>(d) =
+                make_float4(acc[nt][0][e], acc[nt][0][2 + e], acc[nt][1][e], acc[nt][1][2 + e]);
+            *reinterpret_cast<float4*>(d + 4) =
+                make_float4(acc[nt][2][e], acc[nt][2][2 + e], acc[nt][3][e], acc[nt][3][2 + e]);
+            if (dg == 0 && gid == 0) p.part_ml[static_cast<long long>(part) * ROWS + i] = make_float2(m, l);
+          }
+        }
+      }
+    }
+  });
+}
+
+// Joins the parts of units that several CTAs worked on, and writes zeros for
+// rows that no unit covers. One CTA per (unit, row, 128 dims): warp w adds parts w,
+// w + 8, ...; then the eight partial sums are added in order. For a unit that
+// one CTA did alone there is nothing to do.
+template <class C>
+__global__ void __launch_bounds__(256) kv4_combine_kernel(const Kv4Params p) {
+  constexpr int D = C::D, ROWS = C::ROWS, DC = D < 128 ? D : 128;
+  __shared__ int scratch[40];
+  __shared__ float4 sum[8][32];
+  __shared__ float2 ml[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int idx = blockIdx.x;
+  const int dc = idx % (D / DC);
+  idx /= (D / DC);
+  const int rows_here = min(ROWS, p.G * p.N);
+  const int i = idx % rows_here;
+  idx /= rows_here;
+  const int h = idx % p.Hkv, entry = idx / p.Hkv;
+  const Kv4Unit u = kv4_unit<C>(p, entry);
+  const int r = u.rt * ROWS + i;
+  if (r >= p.G * p.N) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
+  const int n = r / p.G, hq = h * p.G + r - n * p.G;
+  uint16_t* o = p.o + u.b * p.o_sb + hq * p.o_sh + n * p.o_sn + dc * DC + lane * 4;
+  float* lse = (p.lse && dc == 0) ? p.lse + (static_cast<long long>(u.b) * p.Hq + hq) * p.N + n : nullptr;
+  const bool unseen = u.tiles == 0 || n >= u.qlen;
+  // first tile of the unit: tiles of all entries before it, then of its heads
+  const int entries = p.B * p.row_tiles;
+  int before = 0, total = 0;
+  for (int e = threadIdx.x; e < entries; e += 256) {
+    const int t = kv4_unit<C>(p, e).tiles * p.Hkv;
+    total += t;
+    if (e < entry) before += t;
+  }
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, s);
+    total += __shfl_xor_sync(0xffffffffu, total, s);
+  }
+  if (lane == 0) {
+    scratch[warp] = before;
+    scratch[8 + warp] = total;
+  }
+  __syncthreads();
+  before = total = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    before += scratch[w];
+    total += scratch[8 + w];
+  }
+  // only the lengths, which the attention launch does not write, are read before it ends
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (unseen) {
+    if (warp == 0) {
+      if (lane * 4 < DC) *reinterpret_cast<uint2*>(o) = make_uint2(0, 0);
+      if (lse && lane == 0) *lse = -INFINITY;
+    }
+    return;
+  }
+  const int per = max(1, (total + p.ctas - 1) / p.ctas);
+  const int first = before + h * u.tiles, last = first + u.tiles - 1;
+  const int c0 = first / per, c1 = last / per;
+  if (c0 == c1) return;  // written by its one CTA
+  // part of CTA c: its share's first piece unless the unit starts there
+  auto part_of = [&](int c) { return 2 * c + (c == c0 ? 1 : 0); };
+  float m = -INFINITY;
+  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, p.part_ml[static_cast<long long>(part_of(c)) * ROWS + i].x);
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+  const float fm = finite_or_zero(m);
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 4
+  for (int c = c0 + warp; c <= c1; c += 8) {
+    const long long at = static_cast<long long>(part_of(c)) * ROWS + i;
+    const float2 q = p.part_ml[at];
+    const float f = ex2(q.x - fm);
+    l += q.y * f;
+    if (lane * 4 < DC) {
+      const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * D + dc * DC + lane * 4);
+      a.x = fmaf(v.x, f, a.x);
+      a.y = fmaf(v.y, f, a.y);
+      a.z = fmaf(v.z, f, a.z);
+      a.w = fmaf(v.w, f, a.w);
+    }
+  }
+  sum[warp][lane] = a;
+  if (lane == 0) ml[warp] = make_float2(l, 0.f);
+  __syncthreads();
+  if (warp != 0) return;
+  a = make_float4(0.f, 0.f, 0.f, 0.f);
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const float4 v = sum[w][lane];
+    a.x += v.x;
+    a.y += v.y;
+    a.z += v.z;
+    a.w += v.w;
+    l += ml[w].x;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (lane * 4 < DC)
+    *reinterpret_cast<uint2*>(o) = make_uint2(pack2<C::BF16>(a.x * inv, a.y * inv), pack2<C::BF16>(a.z * inv, a.w * inv));
+  if (lse && lane == 0) *lse = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+}
+
+}  // namespace gqafa

@@ -1,0 +1,384 @@
+// The paged 4-bit KV cache's own kernels: the plan of a step (block tables,
+// slots and positions from the requests' lengths), the quantised write of new
+// tokens and the read back of cached ones. Formats: kv4_layout.cuh.
+#pragma once
+#include "kv4_layout.cuh"
+#include "ptx_sm100.cuh"
+
+namespace gqafa {
+
+// ------------------------------------------------------------------ plan
+struct Kv4PlanParams {
+  const int* kv_lens;   // [B] tokens already cached
+  const int* new_lens;  // [B] tokens of this step; -1: the request is finished
+  const int* table;     // [B][cols]
+  long long table_stride;
+  int* free_pages;        // ring of F page ids
+  const int* free_state;  // {head, count}
+  int B, cols, F, page, page_shift, max_new;
+  int* out_table;  // [B][cols]
+  int* out_kv_lens;
+  int* out_new_lens;
+  int* out_slots;      // [B][max_new]
+  int* out_positions;  // [B][max_new]
+  int* out_accepted;   // [B]
+  int* out_state;      // {head, count}
+};
+
+struct Kv4Request {
+  int len, add, used, need, back;
+  bool gone, fits;
+};
+
+__device__ __forceinline__ Kv4Request kv4_request(const Kv4PlanParams& p, int b) {
+  Kv4Request r;
+  const int capacity = p.cols << p.page_shift;
+  r.len = min(max(p.kv_lens[b], 0), capacity);
+  r.add = p.new_lens[b];
+  r.gone = r.add < 0;
+  r.used = (r.len + p.page - 1) >> p.page_shift;
+  r.fits = r.add <= p.max_new && r.add <= capacity - r.len;
+  r.need = (r.gone || !r.fits) ? 0 : ((r.len + r.add + p.page - 1) >> p.page_shift) - r.used;
+  r.back = r.gone ? r.used : 0;
+  return r;
+}
+
+// One CTA per request. Each CTA scans the page counts of all requests (a few
+// hundred integers from L2) instead of waiting for another CTA's prefix, so
+// the plan is a single launch without communication. Requests take free pages
+// in request order; one whose running total passes the free count is refused.
+__global__ void __launch_bounds__(256) kv4_plan_kernel(const Kv4PlanParams p) {
+  __shared__ long long warp_sum[8];
+  __shared__ long long mine;  // (pages needed, pages given back) before this request
+  const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int head = p.free_state[0] % p.F;
+  if (head < 0) head += p.F;
+  const int count = min(max(p.free_state[1], 0), p.F);
+
+  // Two running sums in one 64-bit word: needed pages in the high half, pages
+  // given back in the low half (both below 2^31: at most every page once).
+  long long carry = 0, given_total = 0;
+  for (int base = 0; base < p.B; base += 256) {
+    const int i = base + threadIdx.x;
+    long long v = 0;
+    if (i < p.B) {
+      const Kv4Request r = kv4_request(p, i);
+      v = (static_cast<long long>(r.need) << 32) | static_cast<unsigned>(r.back);
+    }
+    long long s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    if (lane == 31) warp_sum[warp] = s;
+    __syncthreads();
+    long long before = carry;
+    for (int w = 0; w < warp; ++w) before += warp_sum[w];
+    const long long upto = before + s;
+    if (i == b) mine = upto - v;
+    // pages that requests up to this one really take (only CTA 0 reports it)
+    if (i < p.B && (upto >> 32) <= count) given_total = max(given_total, upto >> 32);
+    for (int w = 0; w < 8; ++w) carry += warp_sum[w];
+    __syncthreads();
+  }
+
+  const Kv4Request r = kv4_request(p, b);
+  const int first = static_cast<int>(mine >> 32), back0 = static_cast<int>(mine & 0x7fffffff);
+  const bool ok = r.gone || (r.fits && (r.need == 0 || first + r.need <= count));
+  const int add = (ok && !r.gone) ? r.add : 0;
+  const int need = ok ? r.need : 0;
+  if (threadIdx.x == 0) {
+    p.out_kv_lens[b] = r.gone ? 0 : r.len + add;
+    p.out_new_lens[b] = add;
+    p.out_accepted[b] = ok ? 1 : 0;
+  }
+  if (b == 0) {
+    // the requests that get pages are a prefix of those that need some
+    __shared__ long long best[8];
+    long long g = given_total;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+    if (lane == 0) best[warp] = g;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < 8; ++w) g = max(g, best[w]);
+      const int returned = min(static_cast<int>(carry & 0x7fffffff), p.F - count);
+      p.out_state[0] = static_cast<int>((head + g) % p.F);
+      p.out_state[1] = count - static_cast<int>(g) + returned;
+    }
+  }
+
+  const int* row = p.table + b * p.table_stride;
+  auto page_of = [&](int col) -> int {
+    if (col < r.used) return row[col];
+    const long long at = static_cast<long long>(head) + first + (col - r.used);
+    return p.free_pages[at % p.F];
+  };
+  for (int col = threadIdx.x; col < p.cols; col += 256) {
+    int v = -1;
+    if (!r.gone && col < r.used + need) v = page_of(col);
+    p.out_table[static_cast<long long>(b) * p.cols + col] = v;
+    if (r.gone && col < r.used) {
+      // behind the live part of the ring, which no CTA of this launch reads
+      const long long at = static_cast<long long>(back0) + col;
+      if (count + at < p.F) p.free_pages[(head + count + at) % p.F] = row[col];
+    }
+  }
+  for (int i = threadIdx.x; i < p.max_new; i += 256) {
+    const long long at = static_cast<long long>(b) * p.max_new + i;
+    int slot = -1, pos = -1;
+    if (i < add) {
+      pos = r.len + i;
+      const int page = page_of(pos >> p.page_shift);
+      if (page >= 0 && page < p.F) slot = (page << p.page_shift) + (pos & (p.page - 1));
+    }
+    p.out_slots[at] = slot;
+    p.out_positions[at] = pos;
+  }
+}
+
+// ------------------------------------------------------------------ append
+struct Kv4AppendParams {
+  const uint16_t* x[2];  // keys, values [B, Hkv, N, D]
+  long long sb[2], sh[2], sn[2];
+  const int* slots;  // [B][N]
+  long long slots_stride;
+  uint8_t* pages;
+  int B, N, Hkv, page_shift;  // page_shift: log2 of the page's tokens
+  long long num_slots;
+  int* status;
+};
+
+template <bool BF16>
+__device__ __forceinline__ constexpr float kv4_max_finite() {
+  return BF16 ? 3.3895313892515355e38f : 65504.f;
+}
+
+// Quantise the eight values of this lane's word of a group whose other words
+// are held by the octet's seven other lanes. Returns the codes (value i of the
+// word in nibble i) and the group's meta word.
+template <bool BF16>
+__device__ __forceinline__ uint32_t kv4_quantise(const uint4 raw, uint32_t& meta) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = unpack_lo<BF16>(w[i]);
+    x[2 * i + 1] = unpack_hi<BF16>(w[i]);
+  }
+  const float most = kv4_max_finite<BF16>();
+  float hi = 0.f, lo = 0.f;
+  bool odd = false;  // an infinity or a NaN
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    hi = fmaxf(hi, x[i]);
+    lo = fminf(lo, x[i]);
+    odd |= !(fabsf(x[i]) <= most);
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+  }
+  const uint32_t odd_lanes = __ballot_sync(0xffffffffu, odd);
+  if ((odd_lanes >> (threadIdx.x & 24)) & 0xffu) {
+    meta = KV4_META_NAN;
+    return 0;
+  }
+  // up to 4 significant bits: clear the 20 low mantissa bits, rounding up
+  const float step = __fdiv_rn(hi * 0.5f - lo * 0.5f, 7.5f);
+  const float s = fmaxf(__uint_as_float((__float_as_uint(step) + 0xFFFFFu) & ~0xFFFFFu),
+                        BF16 ? 1.1754943508222875e-38f : 4.76837158203125e-7f);
+  const float inv = __frcp_rn(s);
+  // floor(x/s + 1/2) by x * (1/s): ties must go up. x/s is a tie or at least
+  // 2^-14 away from one (x has at most 11 bits, s 4), and the product is off
+  // by less than 2^-19, so a bias of 2^-17 decides every case rightly. Adding
+  // 1.5 * 2^23 then rounds to the nearest integer in the low mantissa bits.
+  constexpr float EPS = 7.62939453125e-6f, MAGIC = 12582912.f;
+  const float zr = fmaf(-lo, inv, EPS) + MAGIC;
+  const uint32_t z = __float_as_uint(zr) & 15u;
+  const float zb = static_cast<float>(z) + EPS;
+  meta = (__float_as_uint(s) >> 16) | z;
+  const bool far = fmaxf(hi, -lo) > most - s;  // a code may pass the largest number
+  uint32_t codes = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float y = fminf(fmaf(x[i], inv, zb) + MAGIC, MAGIC + 15.f);
+    if (far) {
+      const float v = s * (y - MAGIC - static_cast<float>(z));
+      y += (v > most) ? -1.f : (v < -most) ? 1.f : 0.f;
+    }
+    codes |= (__float_as_uint(y) & 15u) << (4 * i);
+  }
+  return codes;
+}
+
+// Value order -> key word order (nibble i: dim 2i, nibble 4+i: dim 2i+1).
+__device__ __forceinline__ uint32_t kv4_key_nibbles(uint32_t c) {
+  // two 4-step perfect-unshuffle moves of nibbles inside the word
+  uint32_t t = (c ^ (c >> 4)) & 0x00F000F0u;
+  c ^= t ^ (t << 4);
+  t = (c ^ (c >> 8)) & 0x0000FF00u;
+  c ^= t ^ (t << 8);
+  return c;
+}
+// Inverse of kv4_key_nibbles.
+__device__ __forceinline__ uint32_t kv4_key_values(uint32_t c) {
+  uint32_t t = (c ^ (c >> 8)) & 0x0000FF00u;
+  c ^= t ^ (t << 8);
+  t = (c ^ (c >> 4)) & 0x00F000F0u;
+  c ^= t ^ (t << 4);
+  return c;
+}
+
+// Eight lanes (an octet) hold one group, 16 bytes of input each: the group's
+// extremes are a shuffle reduction, and nothing else is shared. blockIdx.y: 0
+// keys, 1 values.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p) {
+  constexpr int NG = D / KV4_GROUP;
+  const int kind = blockIdx.y;
+  const int j = threadIdx.x & 7;
+  const long long octets = static_cast<long long>(p.B) * p.N * p.Hkv * NG;
+  const long long stride = static_cast<long long>(gridDim.x) * 32;
+  const int blocks_shift = p.page_shift - 4;
+  // every lane of a warp runs the same number of rounds: the shuffles need all
+  for (long long first = (static_cast<long long>(blockIdx.x) * 256 + (threadIdx.x & ~31)) >> 3; first < octets;
+       first += stride) {
+    const long long o = first + ((threadIdx.x & 31) >> 3);
+    const bool live = o < octets;
+    const int g = static_cast<int>(o % NG);
+    long long rest = o / NG;
+    const int h = static_cast<int>(rest % p.Hkv);
+    rest /= p.Hkv;
+    const int n = static_cast<int>(rest % p.N);
+    const int b = static_cast<int>(rest / p.N);
+    long long slot = -1;
+    if (live) slot = p.slots[b * p.slots_stride + n];
+    if (slot >= p.num_slots || slot < -1) {
+      if (j == 0) atomicCAS(p.status, 0, ST_KV4_SLOT);
+      slot = -1;
+    }
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (slot >= 0)
+      raw = *reinterpret_cast<const uint4*>(p.x[kind] + b * p.sb[kind] + h * p.sh[kind] + n * p.sn[kind] +
+                                            g * KV4_GROUP + j * 8);
+    uint32_t meta;
+    uint32_t codes = kv4_quantise<BF16>(raw, meta);
+    if (slot < 0) continue;
+    const int r = static_cast<int>(slot & 15);
+    const long long page = slot >> p.page_shift;
+    const int blk = static_cast<int>(slot >> 4) & ((1 << blocks_shift) - 1);
+    uint8_t* dst = p.pages + ((((page * 2 + kind) * p.Hkv + h) << blocks_shift) + blk) * kv4_block_bytes(D);
+    if (kind == 0) codes = kv4_key_nibbles(codes);
+    *reinterpret_cast<uint32_t*>(dst + g * KV4_CODE_BYTES + (kind == 0 ? kv4_key_word(r, j) : kv4_value_word(r, j))) =
+        codes;
+    if (j == 0)
+      reinterpret_cast<uint16_t*>(dst + NG * KV4_CODE_BYTES + g * KV4_META_BYTES)[kind == 0 ? kv4_key_meta(r)
+                                                                                           : kv4_value_meta(r)] =
+          static_cast<uint16_t>(meta);
+  }
+}
+
+// ------------------------------------------------------------------ read
+struct Kv4ReadParams {
+  const uint8_t* pages;
+  const int* table;  // [B][cols]
+  long long table_stride;
+  const int* kv_lens;
+  const int* starts;  // [B] or null (0)
+  uint16_t* out[2];   // keys, values [B, Hkv, n, D] contiguous
+  int B, Hkv, n, cols, page_shift, num_pages;
+  int xblocks;  // CTAs per request and head
+  int* status;
+};
+
+// Eight values of a word as 16 bytes of 16-bit values, exactly s * (c - z).
+template <bool BF16>
+__device__ __forceinline__ uint4 kv4_values(uint32_t codes, uint32_t meta) {
+  const float s = __uint_as_float((meta & 0xFFF0u) << 16);
+  const float zs = -(static_cast<float>(meta & 15u)) * s;  // at most 8 bits: exact
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float lo = fmaf(static_cast<float>((codes >> (8 * i)) & 15u), s, zs);
+    const float hi = fmaf(static_cast<float>((codes >> (8 * i + 4)) & 15u), s, zs);
+    w[i] = pack2<BF16>(lo, hi);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A warp reads one group's codes of one block (16 bytes a lane, as stored) and
+// writes 16 tokens x 64 values: 128 contiguous bytes per token. blockIdx.x:
+// request, head and eight (block, group) pairs; blockIdx.y: keys / values. Rows
+// behind a request's last token become zeros.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
+  constexpr int NG = D / KV4_GROUP;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int kind = blockIdx.y;
+  const int bh = blockIdx.x / p.xblocks;
+  const int h = bh % p.Hkv, b = bh / p.Hkv;
+  const int capacity = p.cols << p.page_shift;
+  int len = p.kv_lens[b];
+  if (len > capacity) {
+    if (threadIdx.x == 0) atomicCAS(p.status, 0, ST_KV4_LENGTH);
+    len = capacity;
+  }
+  const int start = p.starts ? max(p.starts[b], 0) : 0;
+  const int item = (blockIdx.x - bh * p.xblocks) * 8 + warp;
+  const int g = item % NG;
+  const long long pos0 = (static_cast<long long>(start) / 16 + item / NG) * 16;  // first token of the block
+  if (pos0 >= static_cast<long long>(start) + p.n) return;
+  uint4 codes = make_uint4(0, 0, 0, 0);
+  uint32_t meta[4] = {0, 0, 0, 0};
+  if (pos0 < len) {
+    const int blk = static_cast<int>(pos0 >> 4);
+    const int blocks_shift = p.page_shift - 4;
+    int page = p.table[b * p.table_stride + (blk >> blocks_shift)];
+    if (page < 0 || page >= p.num_pages) {
+      if (lane == 0) atomicCAS(p.status, 0, ST_KV4_PAGE);
+      len = 0;
+    } else {
+      const uint8_t* src = p.pages + ((((static_cast<long long>(page) * 2 + kind) * p.Hkv + h) << blocks_shift) +
+                                      (blk & ((1 << blocks_shift) - 1))) *
+                                         kv4_block_bytes(D);
+      codes = __ldg(reinterpret_cast<const uint4*>(src + g * KV4_CODE_BYTES + lane * 16));
+      const uint8_t* m = src + NG * KV4_CODE_BYTES + g * KV4_META_BYTES;
+      if (kind == 0) {
+        const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(m + (lane >> 2) * 4));
+        meta[0] = w & 0xFFFFu;
+        meta[1] = w >> 16;
+      } else {
+        const uint2 w = __ldg(reinterpret_cast<const uint2*>(m + (lane >> 3) * 8));
+        meta[0] = w.x & 0xFFFFu;
+        meta[1] = w.x >> 16;
+        meta[2] = w.y & 0xFFFFu;
+        meta[3] = w.y >> 16;
+      }
+    }
+  }
+  uint16_t* out = p.out[kind] + (static_cast<long long>(b) * p.Hkv + h) * p.n * D + g * KV4_GROUP;
+  auto store = [&](int r, int j, uint32_t c, uint32_t m) {
+    const long long i = pos0 + r - start;
+    if (i < 0 || i >= p.n) return;
+    const uint4 v = (pos0 + r < len) ? kv4_values<BF16>(c, m) : make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(out + i * D + j * 8) = v;
+  };
+  if (kind == 0) {
+    const int r = lane >> 2, t = lane & 3;
+    store(r, 2 * t, kv4_key_values(codes.x), meta[0]);
+    store(r, 2 * t + 1, kv4_key_values(codes.y), meta[0]);
+    store(r + 8, 2 * t, kv4_key_values(codes.z), meta[1]);
+    store(r + 8, 2 * t + 1, kv4_key_values(codes.w), meta[1]);
+  } else {
+    const int t = lane >> 3, j = (lane & 7) ^ (2 * t);
+    store(2 * t, j, codes.x, meta[0]);
+    store(2 * t + 1, j, codes.y, meta[1]);
+    store(2 * t + 8, j, codes.z, meta[2]);
+    store(2 * t + 9, j, codes.w, meta[3]);
+  }
+}
+
+}  // namespace gqafa

@@ -15,6 +15,15 @@ from .attention import (
     flash_attn_gqa_forward_with_lse,
     flash_attn_gqa_backward,
 )
+from .kv4 import (
+    KV4Cache,
+    KV4Plan,
+    kv4_alloc,
+    kv4_plan,
+    kv4_append,
+    kv4_read,
+    attention_flash_gqa_kv4,
+)
 from .hf_integration import (
     register_triton_attention,
     triton_gqa_attention,
@@ -31,6 +40,13 @@ __all__ = [
     "attention_gqa_ref",
     "attention_swa_ref",
     "attention",
+    "KV4Cache",
+    "KV4Plan",
+    "kv4_alloc",
+    "kv4_plan",
+    "kv4_append",
+    "kv4_read",
+    "attention_flash_gqa_kv4",
     "register_triton_attention",
     "triton_gqa_attention",
     "patch_transformers_5_5_4_flash_attn_key",

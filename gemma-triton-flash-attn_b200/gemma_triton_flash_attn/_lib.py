@@ -3,9 +3,9 @@
 Two in-tree libraries (``make`` in the package directory, or
 ``__graft_entry__.build()``): ``libgqa_fa_b200.so``, the kernels behind the C
 ABI, bound here with ctypes for every entry point; and ``libgqa_fa_ops.so``,
-torch operators ``torch.ops.gqafa.fwd`` / ``torch.ops.gqafa.bwd`` over the
-same ABI, which the autograd function's hot path calls (no per-call Python
-argument marshalling). There is no CPU or Triton fallback: if a library is
+torch operators ``torch.ops.gqafa.fwd`` / ``torch.ops.gqafa.bwd`` and the
+``kv4_*`` ones of the paged 4-bit cache over the same ABI, which the hot paths
+call (no per-call Python argument marshalling). There is no CPU or Triton fallback: if a library is
 missing, loading it raises.
 """
 from __future__ import annotations
@@ -45,6 +45,12 @@ EXPORTED_SYMBOLS = (
     "gqafa_version",
     "gqafa_set_wait_counters",
     "gqafa_set_test_waits",
+    "gqafa_kv4_page_bytes",
+    "gqafa_kv4_plan",
+    "gqafa_kv4_append",
+    "gqafa_kv4_read",
+    "gqafa_kv4_attend_workspace_size",
+    "gqafa_kv4_attend",
 )
 
 OPS_PATH = os.path.join(os.path.dirname(LIB_PATH), "libgqa_fa_ops.so")
@@ -105,6 +111,20 @@ def load():
         lib.gqafa_bwd_partial.restype = _I
         lib.gqafa_bwd_workspace_size.argtypes = [_I] * 7
         lib.gqafa_bwd_workspace_size.restype = _L
+        lib.gqafa_kv4_page_bytes.argtypes = [_I] * 3
+        lib.gqafa_kv4_page_bytes.restype = _L
+        lib.gqafa_kv4_plan.argtypes = [_P, _P, _P, _L, _P, _P] + [_I] * 5 + [_P] * 8
+        lib.gqafa_kv4_plan.restype = _I
+        lib.gqafa_kv4_append.argtypes = [_P, _S, _P, _S, _P, _L, _P, _L] + [_I] * 6 + [_P]
+        lib.gqafa_kv4_append.restype = _I
+        lib.gqafa_kv4_read.argtypes = [_P, _L, _P, _L, _I, _P, _P, _P, _P] + [_I] * 6 + [_P]
+        lib.gqafa_kv4_read.restype = _I
+        lib.gqafa_kv4_attend_workspace_size.argtypes = [_I] * 7
+        lib.gqafa_kv4_attend_workspace_size.restype = _L
+        lib.gqafa_kv4_attend.argtypes = (
+            [_P, _S, _P, _L, _P, _L, _I, _P, _P, _P, _S, _P] + [_I] * 7 + [_F] + [_I] * 3 + [_P, _L, _P]
+        )
+        lib.gqafa_kv4_attend.restype = _I
         lib.gqafa_supported.argtypes = [_I, _I]
         lib.gqafa_supported.restype = _I
         lib.gqafa_last_error.argtypes = []

@@ -190,6 +190,81 @@ GQAFA_API int gqafa_bwd_stage_rows(int stage, const void* q, const long long* q_
                                    int heads_kv, int seqlen, int head_dim, float softmax_scale, int causal,
                                    int window, int dtype, void* stream, int row_begin, int row_end);
 
+/* ---------------------------------------------------------------------------
+ * Serving from a paged KV cache held in 4 bits (no counterpart in the
+ * reference). The cache is one uint8 array of num_pages pages of
+ * gqafa_kv4_page_bytes bytes, 16-byte aligned; page_size (tokens of a page) is
+ * 16, 32, 64, 128 or 256. Values are held as s * (c - z) in groups of 64 along
+ * head_dim: a 4-bit code c each, and a scale s of 4 significant bits and a zero
+ * point z in 0..15 per group (4.25 bits a value; layout in csrc/kv4_layout.cuh).
+ * s * (c - z) is exact in fp16 and bf16.
+ *
+ * Integer arrays are int32 device memory. A request's token t lies in page
+ * block_table[b][t / page_size]; a slot is page * page_size + t % page_size.
+ * Lengths, tables and slots are read on the device, so a captured graph can be
+ * replayed with new ones. Entries that are out of range never leave the given
+ * arrays: a slot outside the cache is skipped, a page outside the pool is
+ * replaced by page 0, a length beyond the block table is clamped to it; the
+ * first such entry is recorded in the status word (gqafa_device_status: 16
+ * page, 17 slot, 18 length), and the results of that request are undefined.
+ * Nothing is allocated and nothing synchronises.
+ * ------------------------------------------------------------------------- */
+
+/* Bytes of one page (keys and values of all heads), -1 for invalid sizes. */
+GQAFA_API long long gqafa_kv4_page_bytes(int heads_kv, int head_dim, int page_size);
+
+/* The plan of a step. Request b has kv_lens[b] cached tokens and gets
+ * new_lens[b] more (0..max_new), or is finished (negative: its pages go back).
+ * free_pages is a ring of num_free page ids (each in 0..num_free-1) whose live
+ * part starts at free_state[0] and holds free_state[1] ids. Requests take free
+ * pages in request order. A request is refused (accepted 0, nothing added)
+ * when its length would pass the block table or max_new, or when the pages
+ * wanted by it and the requests before it pass the free count. Pages given
+ * back are written behind the live part of the ring, for later steps.
+ * Outputs: block table [batch][cols] (-1 where unused), lengths after the
+ * step, tokens added, slot and position of every new token [batch][max_new]
+ * (-1 behind the last one), accepted, and the ring's new state. Inputs other
+ * than the dead part of the ring are not written; outputs may not overlap
+ * them. */
+GQAFA_API int gqafa_kv4_plan(const int* kv_lens, const int* new_lens, const int* block_table, long long table_stride,
+                             int* free_pages, const int* free_state, int batch, int cols, int num_free, int page_size,
+                             int max_new, int* out_block_table, int* out_kv_lens, int* out_new_lens, int* out_slot_map,
+                             int* out_positions, int* out_accepted, int* out_free_state, void* stream);
+
+/* Quantise k and v [batch, heads_kv, seqlen, head_dim] into the slots of
+ * slot_map [batch][seqlen] (-1: skip the token). Slots must be distinct. A
+ * group of 64 values with an infinity or a NaN reads back as NaN. */
+GQAFA_API int gqafa_kv4_append(const void* k, const long long* k_strides, const void* v, const long long* v_strides,
+                               const int* slot_map, long long slot_stride, void* pages, long long num_pages, int batch,
+                               int heads_kv, int seqlen, int head_dim, int page_size, int dtype, void* stream);
+
+/* Cached keys and values as contiguous [batch, heads_kv, seqlen, head_dim]
+ * tensors: row i of request b is position starts[b] + i (starts NULL: 0), zeros
+ * from kv_lens[b] on. */
+GQAFA_API int gqafa_kv4_read(const void* pages, long long num_pages, const int* block_table, long long table_stride,
+                             int cols, const int* kv_lens, const int* starts, void* k, void* v, int batch,
+                             int heads_kv, int seqlen, int head_dim, int page_size, int dtype, void* stream);
+
+/* Attention of q [batch, heads_q, seqlen_q, head_dim] over the cache. Request
+ * b has kv_lens[b] keys; its first q_lens[b] query rows (q_lens NULL: all) are
+ * the last of those positions: row r sits at kv_lens[b] - q_lens[b] + r. With
+ * causal != 0 a row sees the keys up to its own position, and with window > 0
+ * the last `window` of them; without causal every row sees all keys. Rows from
+ * q_lens[b] on, and rows that see no key, get zeros (lse -inf). lse may be
+ * NULL, else fp32 [batch, heads_q, seqlen_q]. max_kv_len is an upper bound of
+ * kv_lens that the host knows (0: the block table's capacity); it sizes the
+ * launch and the workspace, longer lengths are still attended whole.
+ * workspace: gqafa_kv4_attend_workspace_size bytes, 256-byte aligned, any
+ * contents, not shared by calls that overlap on the GPU. */
+GQAFA_API long long gqafa_kv4_attend_workspace_size(int batch, int heads_q, int heads_kv, int seqlen_q, int head_dim,
+                                                    int max_kv_len, int window);
+GQAFA_API int gqafa_kv4_attend(const void* q, const long long* q_strides, const void* pages, long long num_pages,
+                               const int* block_table, long long table_stride, int cols, const int* kv_lens,
+                               const int* q_lens, void* o, const long long* o_strides, float* lse, int batch,
+                               int heads_q, int heads_kv, int seqlen_q, int head_dim, int page_size, int max_kv_len,
+                               float softmax_scale, int causal, int window, int dtype, void* workspace,
+                               long long workspace_bytes, void* stream);
+
 /* 1 if (head_dim, dtype) has a compiled kernel set, else 0. */
 GQAFA_API int gqafa_supported(int head_dim, int dtype);
 
