@@ -120,7 +120,14 @@ int encode_map(CUtensorMap* m, const TensorDesc& t, int B, int N, int D, int box
 // encoding) need one.
 int bind_device(cudaStream_t stream) {
   int dev = 0;
-  cudaError_t e = (stream != nullptr) ? cudaStreamGetDevice(stream, &dev) : cudaGetDevice(&dev);
+  // A stream under capture may not be asked for its device (the query would
+  // end the capture): the current device is then the caller's word.
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  cudaError_t e = cudaSuccess;
+  if (stream != nullptr) e = cudaStreamIsCapturing(stream, &capture);
+  if (e == cudaSuccess)
+    e = (stream != nullptr && capture == cudaStreamCaptureStatusNone) ? cudaStreamGetDevice(stream, &dev)
+                                                                      : cudaGetDevice(&dev);
   if (e != cudaSuccess) return fail(GQAFA_ERR_CUDA, "cannot resolve the stream's device: %s", cudaGetErrorString(e));
   e = cudaSetDevice(dev);
   if (e != cudaSuccess) return fail(GQAFA_ERR_CUDA, "cudaSetDevice(%d): %s", dev, cudaGetErrorString(e));

@@ -408,6 +408,7 @@ extern "C" int gqafa_kv4_attend(const void* q, const long long* q_strides, const
   if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
     return fail(GQAFA_ERR_INVALID, "workspace must be 256-byte aligned");
   Kv4Params p{};
+  p.tops = kv4_tops(dtype == GQAFA_DTYPE_BF16);
   p.q = static_cast<const uint16_t*>(q);
   p.q_sb = qs[0];
   p.q_sh = qs[1];

@@ -3,14 +3,18 @@
 //   O[n] = sum_j softmax_j(scale * q_n . k_j) v_j over the keys j that the
 //   causal mask and the window leave to token n, k and v read from the codes.
 //
-// Mathematics. With k = s (c - z) per group of 64 dims, a group's part of a
-// score is s * (q . (16 + c) - (16 + z) * sum(q)): the 16-bit number 16 + c is
-// one AND-OR of a shifted code word (the code becomes the top four mantissa
-// bits), so the codes go into the MMAs without a conversion, and scale and
-// zero point are applied once per group to the fp32 result. On the value side
-// P' = round16(s * P) is the B operand and 16 + c the A operand; the term
-// sum_j (16 + z_j) P'_j is one more MMA with the same rounded P', so the
-// offset cancels exactly and only P' itself is rounded.
+// Mathematics. A code c goes into the MMAs as the 16-bit number F + c: with the
+// code in the low mantissa bits of a power of two F this is one AND-OR of a
+// (shifted) code word, no conversion. bf16: F = 128 for every nibble. fp16:
+// F = 256 and 16 for even and odd nibbles, so that one shift serves two. The
+// offsets leave the results through linear terms:
+//   scores: a group's part is s * (q . (F + c) - q . F - z * sum(q)), scale
+//     and zero point applied once per group to the fp32 MMA result;
+//   values: P' = round16(s * P) is the B operand, and one more MMA subtracts
+//     sum_j (F + z_j) P'_j with the same rounded P', so the offset cancels
+//     exactly and only P' itself is rounded. The two accumulators are joined
+//     after every tile: F * sum(P') would otherwise outgrow the result over a
+//     long cache and cost it its low bits.
 //
 // Shape. A decode step has G = H_Q / H_KV query rows per KV head, far below
 // the 128 rows of a tcgen05 tile, and reads each cached byte once: it is bound
@@ -22,11 +26,12 @@
 // One CTA: eight compute warps and one producer warp. The producer walks the
 // block table and brings whole blocks (codes and scales together) into a ring
 // of stages with bulk copies. Work is cut into tiles of TB blocks. Scores: warp
-// w takes blocks w, w + 8, ... over all of head_dim, with its own running
-// maximum; P goes to shared memory (fp32), one barrier per tile. Values: warp
-// (dim group, slice) takes 64 dims of every NG-th block, so the output
-// accumulator is 16 registers per 8 query rows; it rescales P by
-// exp2(m_warp - M), M the maximum over the eight warps.
+// w takes blocks w, w + 8, ... over all of head_dim; P goes to shared memory
+// (fp32), one barrier per tile. Values: warp (dim group, slice) takes 64 dims
+// of every KS-th block, so the output accumulator is 16 registers per 8 query
+// rows. All warps share one reference maximum per row; a warp that meets a
+// larger score publishes its own for this tile, and only then are P and the
+// accumulators rescaled.
 //
 // Split. The tiles of all (request, row tile, KV head) units form one list,
 // cut into equal contiguous shares, one per CTA: ragged lengths and a single
@@ -35,12 +40,24 @@
 // sum) and kv4_combine_kernel joins them in list order, so results do not
 // depend on timing.
 #pragma once
+#include <type_traits>
+
 #include "kv4_layout.cuh"
 #include "ptx_sm100.cuh"
 
 namespace gqafa {
 
+// The powers of two that codes are set into (see codes16), and their negatives.
+struct Kv4Tops {
+  uint32_t even, odd, minus_even, minus_odd, float128;
+};
+inline Kv4Tops kv4_tops(bool bf16) {
+  return bf16 ? Kv4Tops{0x43004300u, 0x43004300u, 0xC300C300u, 0xC300C300u, 0x43000000u}
+              : Kv4Tops{0x5C005C00u, 0x4C004C00u, 0xDC00DC00u, 0xCC00CC00u, 0x43000000u};
+}
+
 struct Kv4Params {
+  Kv4Tops tops;
   const uint16_t* q;
   long long q_sb, q_sh, q_sn;
   uint16_t* o;
@@ -84,7 +101,7 @@ struct Kv4Cfg {
   static constexpr int STAGE_BYTES = SB * BLOCK_BYTES;
   static constexpr int Q_PITCH = D * 2 + 16;  // bytes; +16: fragment loads hit all banks
   static constexpr int Q_BYTES = ROWS * Q_PITCH;
-  static constexpr int SUMQ_BYTES = NG * ROWS * 4;
+  static constexpr int SUMQ_BYTES = NG * ROWS * 4 * (BF16 ? 1 : 3);  // sum(q); fp16: and the MMAs' start values
   static constexpr int P_PITCH = 20;          // floats of a row's 16 probabilities
   static constexpr int P_BYTES = TB * ROWS * P_PITCH * 4;  // one of two buffers
   static constexpr int M_BYTES = 8 * ROWS * 4;             // one of two buffers
@@ -95,6 +112,10 @@ struct Kv4Cfg {
   static constexpr int NST = NST_FIT < 12 ? NST_FIT : 12;
   static constexpr int SMEM_BYTES = NST * STAGE_BYTES + MISC_BYTES;
   static constexpr int THREADS = 288;
+  // A row's reference maximum is raised when a score passes it by more than
+  // this (log2 units). bf16 P' keeps its relative precision up to 2^8; fp16
+  // would overflow at large scales, so its P stays at most 1.
+  static constexpr float SLACK = BF16 ? 8.f : 0.f;
   static_assert(NST >= 4, "two stages of keys and two of values");
   // the slices' sums are joined through the P buffers
   static_assert(KS == 1 || (KS / 2) * ROWS * D * 4 <= 2 * P_BYTES, "slice exchange");
@@ -222,25 +243,65 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
   }
 }
 
-// 16 + code for nibble I of both 16-bit halves of w: in [16, 32) the code is
-// the top four mantissa bits (bf16 bits 3..6, fp16 bits 6..9).
-template <bool BF16, int I>
-__device__ __forceinline__ uint32_t code16(uint32_t w) {
-  constexpr int SH = (BF16 ? 3 : 6) - 4 * I;
-  const uint32_t x = SH >= 0 ? (w << (SH >= 0 ? SH : 0)) : (w >> (SH < 0 ? -SH : 0));
-  return BF16 ? ((x & 0x00780078u) | 0x41804180u) : ((x & 0x03C003C0u) | 0x4C004C00u);
-}
-// -(16 + zero point) of two packed meta words, as 16-bit numbers.
+// d = a * b (no accumulator to clear).
 template <bool BF16>
-__device__ __forceinline__ uint32_t minus_zero16(uint32_t w) {
-  const uint32_t z = w & 0x000F000Fu;
-  return BF16 ? ((z << 3) | 0xC180C180u) : ((z << 6) | 0xCC00CC00u);
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1, const float4 c) {
+  if constexpr (BF16) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
+  }
 }
-__device__ __forceinline__ float scale_lo(uint32_t w) { return __uint_as_float((w << 16) & 0xFFF00000u); }
-__device__ __forceinline__ float scale_hi(uint32_t w) { return __uint_as_float(w & 0xFFF00000u); }
-// 16 + zero point in fp32.
-__device__ __forceinline__ float zero_lo(uint32_t w) { return __uint_as_float(0x41800000u | ((w & 0xFu) << 19)); }
-__device__ __forceinline__ float zero_hi(uint32_t w) { return __uint_as_float(0x41800000u | ((w & 0xF0000u) << 3)); }
+
+// (x & mask) | top as one LOP3. An instruction takes one immediate: `top` comes
+// from the kernel's parameters, so it stays in a register (as a second
+// immediate it cost another instruction per MMA operand: 61 ALU instructions
+// per 16 tokens x 64 dims, the busiest pipe, at head_dim 512).
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t top) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(top));
+  return r;
+}
+
+// F + code for the four nibbles of both 16-bit halves of w. bf16: 0x4300 is
+// 128, its last mantissa bit worth 1. fp16: the even nibbles of w << 2 and
+// w >> 6 lie at bits 2..5 of 256 (0x5C00), the odd ones at bits 6..9 of 16.
+template <bool BF16>
+__device__ __forceinline__ void codes16(uint32_t w, const Kv4Tops& f, uint32_t (&a)[4]) {
+  if constexpr (BF16) {
+    a[0] = and_or(w, 0x000F000Fu, f.even);
+    a[1] = and_or(w >> 4, 0x000F000Fu, f.even);
+    a[2] = and_or(w >> 8, 0x000F000Fu, f.even);
+    a[3] = and_or(w >> 12, 0x000F000Fu, f.even);
+  } else {
+    const uint32_t l = w << 2, r = w >> 6;
+    a[0] = and_or(l, 0x003C003Cu, f.even);
+    a[1] = and_or(l, 0x03C003C0u, f.odd);
+    a[2] = and_or(r, 0x003C003Cu, f.even);
+    a[3] = and_or(r, 0x03C003C0u, f.odd);
+  }
+}
+// -(F + zero point) of two packed meta words, for even and odd nibbles.
+template <bool BF16>
+__device__ __forceinline__ uint32_t minus_zero_even(uint32_t w, const Kv4Tops& f) {
+  return BF16 ? and_or(w, 0x000F000Fu, f.minus_even) : and_or(w << 2, 0x003C003Cu, f.minus_even);
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t minus_zero_odd(uint32_t w, const Kv4Tops& f) {
+  return BF16 ? and_or(w, 0x000F000Fu, f.minus_even) : and_or(w << 6, 0x03C003C0u, f.minus_odd);
+}
+// Scale, and 128 + zero point, of the meta word in w's upper half, in fp32.
+__device__ __forceinline__ float meta_scale(uint32_t w) { return __uint_as_float(w & 0xFFF00000u); }
+__device__ __forceinline__ float meta_zero128(uint32_t w, const Kv4Tops& f) {
+  return __uint_as_float(and_or(w, 0x000F0000u, f.float128));
+}
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile(
@@ -263,9 +324,11 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
   float* sM = sP + 2 * C::P_BYTES / 4;                                 // [2][8 warps][ROWS]
   uint8_t* sQ = reinterpret_cast<uint8_t*>(sM + 2 * 8 * ROWS);         // [ROWS] rows of Q_PITCH bytes
   float* sSum = reinterpret_cast<float*>(sQ + C::Q_BYTES);             // [NG][ROWS]
-  int2* sMask = reinterpret_cast<int2*>(sSum + NG * ROWS);             // [ROWS]: first key, number of keys
+  float* sStart = sSum + NG * ROWS;                                    // fp16: [NG][ROWS / 2] (a, b, a, b)
+  int2* sMask = reinterpret_cast<int2*>(sSum + C::SUMQ_BYTES / 4);     // [ROWS]: first key, number of keys
   uint64_t* bars = reinterpret_cast<uint64_t*>(sMask + ROWS);
   __shared__ int scratch[40];
+  __shared__ __align__(16) int raised[2][8];  // warps that published a maximum for a tile
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
 
@@ -374,6 +437,9 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
   // ======================= compute warps =======================
   const int gid = lane >> 2, tig = lane & 3;
   const int dg = warp % NG, ks = warp / NG;  // value side: dim group, slice of the blocks
+  const Kv4Tops tops = p.tops;
+  const uint32_t ring = smem_u32(sRing);
+  const uint32_t qbase = smem_u32(sQ + gid * C::Q_PITCH + tig * 32);
   uint32_t cnt = 0;
   int buf = 0;
   auto wait_full = [&](int slot, uint32_t c) {
@@ -399,11 +465,25 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
         v = *reinterpret_cast<const uint4*>(p.q + u.b * p.q_sb + hq * p.q_sh + n * p.q_sn + c * 8);
       }
       *reinterpret_cast<uint4*>(sQ + i * C::Q_PITCH + c * 16) = v;
-      float s = unpack_lo<BF16>(v.x) + unpack_hi<BF16>(v.x) + unpack_lo<BF16>(v.y) + unpack_hi<BF16>(v.y) +
-                unpack_lo<BF16>(v.z) + unpack_hi<BF16>(v.z) + unpack_lo<BF16>(v.w) + unpack_hi<BF16>(v.w);
+      // sums over dims 0, 1, 4, 5 (even nibbles) and 2, 3, 6, 7 (odd) of each eight
+      float even = unpack_lo<BF16>(v.x) + unpack_hi<BF16>(v.x) + unpack_lo<BF16>(v.z) + unpack_hi<BF16>(v.z);
+      float odd = unpack_lo<BF16>(v.y) + unpack_hi<BF16>(v.y) + unpack_lo<BF16>(v.w) + unpack_hi<BF16>(v.w);
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if ((c & 7) == 0) sSum[(c >> 3) * ROWS + i] = s;
+      for (int o = 1; o < 8; o <<= 1) {
+        even += __shfl_xor_sync(0xffffffffu, even, o);
+        odd += __shfl_xor_sync(0xffffffffu, odd, o);
+      }
+      if ((c & 7) == 0) {
+        const int g = c >> 3;
+        sSum[g * ROWS + i] = even + odd;
+        if constexpr (!BF16) {
+          // start value: 128 sum(q) - q . F, so that (128 + z) sum(q) is left to subtract
+          const float start = -128.f * even + 112.f * odd;
+          float* d = sStart + (g * (ROWS / 2) + (i >> 1)) * 4 + (i & 1);
+          d[0] = start;
+          d[2] = start;
+        }
+      }
     }
     if (threadIdx.x < ROWS) {
       const int r = r0 + threadIdx.x;
@@ -421,25 +501,25 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
     const int all_hi = p.causal ? min(u.len, off + r0 / p.G + 1) : u.len;
     const int all_lo = (p.causal && p.window > 0) ? max(0, off + nlast - p.window + 1) : 0;
 
-    float acc[NT][4][4], wz[NT][4];
-    float m_run[NT][2], l_run[NT][2];  // score side: this warp's blocks, rows 2 tig, 2 tig + 1
-    float m_all[NT];                   // value side: row gid, over all warps
+    float acc[NT][4][4];
+    // Rows 2 tig, 2 tig + 1: reference maximum (the same in all warps) and sum
+    // of P over this warp's blocks.
+    float mref[NT][2], l_run[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        wz[nt][j] = 0.f;
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[nt][j][e] = 0.f;
-      }
-      m_run[nt][0] = m_run[nt][1] = -INFINITY;
+      mref[nt][0] = mref[nt][1] = -INFINITY;
       l_run[nt][0] = l_run[nt][1] = 0.f;
-      m_all[nt] = -INFINITY;
     }
 
     for (int tile = t0; tile < t1; ++tile) {
       const int nv = min(TB, u.nblk - tile * TB);
       const int key_tile = (u.b0 + tile * TB) * 16;
+      // some row of the unit does not see all of the tile's keys
+      const bool edge = key_tile < all_lo || key_tile + nv * 16 > all_hi;
       // ---------------- scores ----------------
       float s[KB][NT][4];
 #pragma unroll
@@ -447,34 +527,37 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
         const int slot = cnt % NST;
         wait_full(slot, cnt);
         ++cnt;
-        const uint32_t stage = smem_u32(sRing + slot * C::STAGE_BYTES);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           const int blk = warp + 8 * kb;
           if (blk / SB != half || blk >= nv) continue;
-          const uint32_t base = stage + (blk - half * SB) * BB;
+          const uint32_t base = ring + slot * C::STAGE_BYTES + (blk - half * SB) * BB;
+          const uint32_t codes = base + lane * 16, metas = base + NG * KV4_CODE_BYTES + gid * 4;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[kb][nt][e] = 0.f;
-#pragma unroll(NG > 2 ? 2 : NG)
+#pragma unroll(NT > 1 ? 2 : 4)
           for (int g = 0; g < NG; ++g) {
-            const uint4 w = lds128(base + g * KV4_CODE_BYTES + lane * 16);
-            const uint32_t meta = lds32(base + NG * KV4_CODE_BYTES + g * KV4_META_BYTES + gid * 4);
-            const float s0 = scale_lo(meta), s1 = scale_hi(meta), z0 = zero_lo(meta), z1 = zero_hi(meta);
+            const uint4 w = lds128(codes + g * KV4_CODE_BYTES);
+            const uint32_t m1 = lds32(metas + g * KV4_META_BYTES), m0 = m1 << 16;
+            const float s0 = meta_scale(m0), s1 = meta_scale(m1), z0 = meta_zero128(m0, tops), z1 = meta_zero128(m1, tops);
+            uint32_t ax[4], ay[4], az[4], aw[4];
+            codes16<BF16>(w.x, tops, ax);
+            codes16<BF16>(w.y, tops, ay);
+            codes16<BF16>(w.z, tops, az);
+            codes16<BF16>(w.w, tops, aw);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              const uint32_t qa = smem_u32(sQ + (nt * 8 + gid) * C::Q_PITCH + g * 128 + tig * 32);
+              const uint32_t qa = qbase + nt * 8 * C::Q_PITCH + g * 128;
               const uint4 q0 = lds128(qa), q1 = lds128(qa + 16);
-              float t[4] = {0.f, 0.f, 0.f, 0.f};
-              mma16816<BF16>(t, code16<BF16, 0>(w.x), code16<BF16, 0>(w.z), code16<BF16, 1>(w.x),
-                             code16<BF16, 1>(w.z), q0.x, q0.y);
-              mma16816<BF16>(t, code16<BF16, 2>(w.x), code16<BF16, 2>(w.z), code16<BF16, 3>(w.x),
-                             code16<BF16, 3>(w.z), q0.z, q0.w);
-              mma16816<BF16>(t, code16<BF16, 0>(w.y), code16<BF16, 0>(w.w), code16<BF16, 1>(w.y),
-                             code16<BF16, 1>(w.w), q1.x, q1.y);
-              mma16816<BF16>(t, code16<BF16, 2>(w.y), code16<BF16, 2>(w.w), code16<BF16, 3>(w.y),
-                             code16<BF16, 3>(w.w), q1.z, q1.w);
+              float4 c = make_float4(0.f, 0.f, 0.f, 0.f);
+              if constexpr (!BF16) c = *reinterpret_cast<const float4*>(sStart + (g * (ROWS / 2) + nt * 4 + tig) * 4);
+              float t[4];
+              mma16816_first<BF16>(t, ax[0], az[0], ax[1], az[1], q0.x, q0.y, c);
+              mma16816<BF16>(t, ax[2], az[2], ax[3], az[3], q0.z, q0.w);
+              mma16816<BF16>(t, ay[0], aw[0], ay[1], aw[1], q1.x, q1.y);
+              mma16816<BF16>(t, ay[2], aw[2], ay[3], aw[3], q1.z, q1.w);
               const float2 sq = *reinterpret_cast<const float2*>(sSum + g * ROWS + nt * 8 + 2 * tig);
               s[kb][nt][0] = fmaf(s0, fmaf(-z0, sq.x, t[0]), s[kb][nt][0]);
               s[kb][nt][1] = fmaf(s0, fmaf(-z0, sq.y, t[1]), s[kb][nt][1]);
@@ -489,37 +572,51 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
       // ---------------- softmax over this warp's blocks ----------------
       float* P = sP + buf * (C::P_BYTES / 4);
       float* M = sM + buf * 8 * ROWS;
+      bool above = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int4 mk = *reinterpret_cast<const int4*>(sMask + nt * 8 + 2 * tig);  // two rows' (first, count)
-        float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           const int blk = warp + 8 * kb;
           if (blk >= nv) continue;
-          const int key = key_tile + blk * 16 + gid;
-          const bool edge = (key_tile + blk * 16 < all_lo) || (key_tile + blk * 16 + 16 > all_hi);
           float* v = s[kb][nt];
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] *= p.scale_log2;
           if (edge) {
+            const int4 mk = *reinterpret_cast<const int4*>(sMask + nt * 8 + 2 * tig);  // two rows' (first, count)
+            const int key = key_tile + blk * 16 + gid;
             if (static_cast<unsigned>(key - mk.x) >= static_cast<unsigned>(mk.y)) v[0] = -INFINITY;
             if (static_cast<unsigned>(key - mk.z) >= static_cast<unsigned>(mk.w)) v[1] = -INFINITY;
             if (static_cast<unsigned>(key + 8 - mk.x) >= static_cast<unsigned>(mk.y)) v[2] = -INFINITY;
             if (static_cast<unsigned>(key + 8 - mk.z) >= static_cast<unsigned>(mk.w)) v[3] = -INFINITY;
           }
-          mx0 = fmaxf(mx0, fmaxf(v[0], v[2]));
-          mx1 = fmaxf(mx1, fmaxf(v[1], v[3]));
+          above |= fmaxf(v[0], v[2]) > mref[nt][0] + C::SLACK || fmaxf(v[1], v[3]) > mref[nt][1] + C::SLACK;
         }
+      }
+      const bool raise = __any_sync(0xffffffffu, above);
+      if (lane == 0) raised[buf][warp] = raise;
+      const int perm = (gid >> 1) * 4 + (gid & 1);  // order (2t, 2t+1, 2t+8, 2t+9) of the value side
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o));
-          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o));
+      for (int nt = 0; nt < NT; ++nt) {
+        float f0 = mref[nt][0], f1 = mref[nt][1];
+        if (raise) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) {
+            if (warp + 8 * kb >= nv) continue;
+            f0 = fmaxf(f0, fmaxf(s[kb][nt][0], s[kb][nt][2]));
+            f1 = fmaxf(f1, fmaxf(s[kb][nt][1], s[kb][nt][3]));
+          }
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            f0 = fmaxf(f0, __shfl_xor_sync(0xffffffffu, f0, o));
+            f1 = fmaxf(f1, __shfl_xor_sync(0xffffffffu, f1, o));
+          }
+          l_run[nt][0] *= ex2(mref[nt][0] - finite_or_zero(f0));
+          l_run[nt][1] *= ex2(mref[nt][1] - finite_or_zero(f1));
+          if (gid == 0) *reinterpret_cast<float2*>(M + warp * ROWS + nt * 8 + 2 * tig) = make_float2(f0, f1);
         }
-        const float n0 = fmaxf(m_run[nt][0], mx0), n1 = fmaxf(m_run[nt][1], mx1);
-        const float f0 = finite_or_zero(n0), f1 = finite_or_zero(n1);
-        float l0 = 0.f, l1 = 0.f;
-        const int perm = (gid >> 1) * 4 + (gid & 1);  // order (2t, 2t+1, 2t+8, 2t+9) of the value side
+        f0 = finite_or_zero(f0);
+        f1 = finite_or_zero(f1);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           const int blk = warp + 8 * kb;
@@ -529,42 +626,41 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
           v[1] = ex2(v[1] - f1);
           v[2] = ex2(v[2] - f0);
           v[3] = ex2(v[3] - f1);
-          l0 += v[0] + v[2];
-          l1 += v[1] + v[3];
+          l_run[nt][0] += v[0] + v[2];
+          l_run[nt][1] += v[1] + v[3];
           float* d = P + (blk * ROWS + nt * 8 + 2 * tig) * PP + perm;
           d[0] = v[0];
           d[2] = v[2];
           d[PP] = v[1];
           d[PP + 2] = v[3];
         }
-        l_run[nt][0] = l_run[nt][0] * ex2(m_run[nt][0] - f0) + l0;
-        l_run[nt][1] = l_run[nt][1] * ex2(m_run[nt][1] - f1) + l1;
-        m_run[nt][0] = n0;
-        m_run[nt][1] = n1;
-        if (gid == 0) *reinterpret_cast<float2*>(M + warp * ROWS + nt * 8 + 2 * tig) = make_float2(n0, n1);
       }
       compute_barrier();
 
-      // ---------------- values ----------------
-      // Reference maximum of every row over the eight warps; the accumulators
-      // follow it when it grows.
-      float fm[NT], up[NT];
-      bool grew = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float m = m_all[nt];
-#pragma unroll
-        for (int w = 0; w < 8; ++w) m = fmaxf(m, M[w * ROWS + nt * 8 + gid]);
-        fm[nt] = finite_or_zero(m);
-        grew |= m > m_all[nt];
-        up[nt] = ex2(m_all[nt] - fm[nt]);
-        m_all[nt] = m;
-      }
-      if (__any_sync(0xffffffffu, grew)) {
+      // ---------------- new maxima, if any warp published some ----------------
+      const int4 ra = *reinterpret_cast<const int4*>(&raised[buf][0]);
+      const int4 rb = *reinterpret_cast<const int4*>(&raised[buf][4]);
+      const bool rescale = (ra.x | ra.y | ra.z | ra.w | rb.x | rb.y | rb.z | rb.w) != 0;
+      // A warp's P refers to its own published maximum, or to the old one: in
+      // the value loop row gid's factor brings it to the new one.
+      float vold[NT], vnew[NT];
+      if (rescale) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float a = up[nt];
-          const float a0 = __shfl_sync(0xffffffffu, a, 8 * tig), a1 = __shfl_sync(0xffffffffu, a, 8 * tig + 4);
+          float m0 = mref[nt][0], m1 = mref[nt][1];
+#pragma unroll
+          for (int w = 0; w < 8; ++w) {
+            if (raised[buf][w]) {
+              const float2 x = *reinterpret_cast<const float2*>(M + w * ROWS + nt * 8 + 2 * tig);
+              m0 = fmaxf(m0, x.x);
+              m1 = fmaxf(m1, x.y);
+            }
+          }
+          float2 mine = make_float2(mref[nt][0], mref[nt][1]);
+          if (raise) mine = *reinterpret_cast<const float2*>(M + warp * ROWS + nt * 8 + 2 * tig);
+          l_run[nt][0] *= ex2(mine.x - finite_or_zero(m0));
+          l_run[nt][1] *= ex2(mine.y - finite_or_zero(m1));
+          const float a0 = ex2(mref[nt][0] - finite_or_zero(m0)), a1 = ex2(mref[nt][1] - finite_or_zero(m1));
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             acc[nt][j][0] *= a0;
@@ -572,69 +668,100 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
             acc[nt][j][2] *= a0;
             acc[nt][j][3] *= a1;
           }
-          wz[nt][0] *= a0;
-          wz[nt][1] *= a1;
-          wz[nt][2] *= a0;
-          wz[nt][3] *= a1;
+          // row gid belongs to lanes with tig = gid / 2
+          const float o0 = __shfl_sync(0xffffffffu, mref[nt][0], gid >> 1), o1 = __shfl_sync(0xffffffffu, mref[nt][1], gid >> 1);
+          const float n0 = __shfl_sync(0xffffffffu, m0, gid >> 1), n1 = __shfl_sync(0xffffffffu, m1, gid >> 1);
+          vold[nt] = (gid & 1) ? o1 : o0;
+          vnew[nt] = finite_or_zero((gid & 1) ? n1 : n0);
+          mref[nt][0] = m0;
+          mref[nt][1] = m1;
         }
       }
+
+      // ---------------- values ----------------
+      float wz[NT][4];  // -sum (F + z) P' of this tile
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) wz[nt][e] = 0.f;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int slot = cnt % NST;
         wait_full(slot, cnt);
         ++cnt;
-        const uint32_t stage = smem_u32(sRing + slot * C::STAGE_BYTES);
-#pragma unroll(SB / KS > 4 ? 4 : SB / KS)
-        for (int i = 0; i < SB / KS; ++i) {
-          const int sblk = i * KS + ks, blk = half * SB + sblk;
-          if (blk >= nv) break;
-          const uint32_t base = stage + sblk * BB;
-          const uint2 mv = lds64(base + NG * KV4_CODE_BYTES + dg * KV4_META_BYTES + tig * 8);
-          const uint4 c = lds128(base + dg * KV4_CODE_BYTES + (tig * 8 + (gid ^ (2 * tig))) * 16);
-          const uint32_t m0 = __byte_perm(c.x, c.y, 0x5410), m1 = __byte_perm(c.x, c.y, 0x7632);
-          const uint32_t m2 = __byte_perm(c.z, c.w, 0x5410), m3 = __byte_perm(c.z, c.w, 0x7632);
-          const uint32_t nz0 = minus_zero16<BF16>(mv.x), nz1 = minus_zero16<BF16>(mv.y);
-          const float s0 = scale_lo(mv.x), s1 = scale_hi(mv.x), s2 = scale_lo(mv.y), s3 = scale_hi(mv.y);
-          const bool edge = (key_tile + blk * 16 < all_lo) || (key_tile + blk * 16 + 16 > all_hi);
+        const uint32_t stage = ring + slot * C::STAGE_BYTES;
+        const uint32_t codes = stage + dg * KV4_CODE_BYTES + (tig * 8 + (gid ^ (2 * tig))) * 16;
+        const uint32_t metas = stage + NG * KV4_CODE_BYTES + dg * KV4_META_BYTES + tig * 8;
+        const float* prow = P + (half * SB * ROWS + gid) * PP + tig * 4;
+        auto block = [&](int sblk, auto special) {
+          constexpr bool SPECIAL = decltype(special)::value;
+          const uint2 mv = lds64(metas + sblk * BB);
+          const uint4 c = lds128(codes + sblk * BB);
+          uint32_t x0[4], x1[4], x2[4], x3[4];  // nibbles 0..3 and 4..7, tokens (2t, 2t+1) and (2t+8, 2t+9)
+          codes16<BF16>(__byte_perm(c.x, c.y, 0x5410), tops, x0);
+          codes16<BF16>(__byte_perm(c.x, c.y, 0x7632), tops, x1);
+          codes16<BF16>(__byte_perm(c.z, c.w, 0x5410), tops, x2);
+          codes16<BF16>(__byte_perm(c.z, c.w, 0x7632), tops, x3);
+          const float s0 = meta_scale(mv.x << 16), s1 = meta_scale(mv.x), s2 = meta_scale(mv.y << 16),
+                      s3 = meta_scale(mv.y);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const uint4 pr = lds128(smem_u32(P + (blk * ROWS + nt * 8 + gid) * PP + tig * 4));
-            const float f = ex2(M[(blk & 7) * ROWS + nt * 8 + gid] - fm[nt]);
-            float p0 = __uint_as_float(pr.x) * f, p1 = __uint_as_float(pr.y) * f;
-            float p2 = __uint_as_float(pr.z) * f, p3 = __uint_as_float(pr.w) * f;
-            if (edge) {
+            float4 pr = *reinterpret_cast<const float4*>(prow + (sblk * ROWS + nt * 8) * PP);
+            if constexpr (SPECIAL) {
+              if (rescale) {
+                const int w = (half * SB + sblk) & 7;
+                const float from = raised[buf][w] ? M[w * ROWS + nt * 8 + gid] : vold[nt];
+                const float f = ex2(finite_or_zero(from) - vnew[nt]);
+                pr.x *= f;
+                pr.y *= f;
+                pr.z *= f;
+                pr.w *= f;
+              }
               // a masked token's scale may be anything (a slot never written): its product must be 0
-              p0 = p0 == 0.f ? 0.f : p0 * s0;
-              p1 = p1 == 0.f ? 0.f : p1 * s1;
-              p2 = p2 == 0.f ? 0.f : p2 * s2;
-              p3 = p3 == 0.f ? 0.f : p3 * s3;
+              pr.x = pr.x == 0.f ? 0.f : pr.x * s0;
+              pr.y = pr.y == 0.f ? 0.f : pr.y * s1;
+              pr.z = pr.z == 0.f ? 0.f : pr.z * s2;
+              pr.w = pr.w == 0.f ? 0.f : pr.w * s3;
             } else {
-              p0 *= s0;
-              p1 *= s1;
-              p2 *= s2;
-              p3 *= s3;
+              pr.x *= s0;
+              pr.y *= s1;
+              pr.z *= s2;
+              pr.w *= s3;
             }
-            const uint32_t b0 = pack2<BF16>(p0, p1), b1 = pack2<BF16>(p2, p3);
-            mma16816<BF16>(acc[nt][0], code16<BF16, 0>(m0), code16<BF16, 1>(m0), code16<BF16, 0>(m2),
-                           code16<BF16, 1>(m2), b0, b1);
-            mma16816<BF16>(acc[nt][1], code16<BF16, 2>(m0), code16<BF16, 3>(m0), code16<BF16, 2>(m2),
-                           code16<BF16, 3>(m2), b0, b1);
-            mma16816<BF16>(acc[nt][2], code16<BF16, 0>(m1), code16<BF16, 1>(m1), code16<BF16, 0>(m3),
-                           code16<BF16, 1>(m3), b0, b1);
-            mma16816<BF16>(acc[nt][3], code16<BF16, 2>(m1), code16<BF16, 3>(m1), code16<BF16, 2>(m3),
-                           code16<BF16, 3>(m3), b0, b1);
-            mma16816<BF16>(wz[nt], nz0, nz0, nz1, nz1, b0, b1);
+            const uint32_t b0 = pack2<BF16>(pr.x, pr.y), b1 = pack2<BF16>(pr.z, pr.w);
+            mma16816<BF16>(acc[nt][0], x0[0], x0[1], x2[0], x2[1], b0, b1);
+            mma16816<BF16>(acc[nt][1], x0[2], x0[3], x2[2], x2[3], b0, b1);
+            mma16816<BF16>(acc[nt][2], x1[0], x1[1], x3[0], x3[1], b0, b1);
+            mma16816<BF16>(acc[nt][3], x1[2], x1[3], x3[2], x3[3], b0, b1);
+            mma16816<BF16>(wz[nt], minus_zero_even<BF16>(mv.x, tops), minus_zero_odd<BF16>(mv.x, tops),
+                           minus_zero_even<BF16>(mv.y, tops), minus_zero_odd<BF16>(mv.y, tops), b0, b1);
+          }
+        };
+        if (!rescale && !edge && nv == TB) {
+#pragma unroll(SB / KS > 4 ? 4 : SB / KS)
+          for (int i = 0; i < SB / KS; ++i) block(i * KS + ks, std::false_type{});
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < SB / KS; ++i) {
+            if (half * SB + i * KS + ks >= nv) break;
+            block(i * KS + ks, std::true_type{});
           }
         }
         release(slot);
       }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[nt][j][e] += wz[nt][e];
       buf ^= 1;
     }
 
     // ---------------- epilogue of the piece ----------------
-    // sums of the eight warps' l, relative to the common maximum
+    // every warp has the rows' maximum; the sums of the eight warps' l
     compute_barrier();  // all value-side reads of P and M are done
-    float* xM = sM;             // [8][ROWS] maxima
+    float* xM = sM;             // [ROWS] maxima
     float* xL = sM + 8 * ROWS;  // [8][ROWS] sums
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -645,16 +772,11 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
         l1 += __shfl_xor_sync(0xffffffffu, l1, o);
       }
       if (gid == 0) {
-        *reinterpret_cast<float2*>(xM + warp * ROWS + nt * 8 + 2 * tig) = make_float2(m_run[nt][0], m_run[nt][1]);
+        if (warp == 0)
+          *reinterpret_cast<float2*>(xM + nt * 8 + 2 * tig) = make_float2(mref[nt][0], mref[nt][1]);
         *reinterpret_cast<float2*>(xL + warp * ROWS + nt * 8 + 2 * tig) = make_float2(l0, l1);
       }
     }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[nt][j][e] += wz[nt][e];
     // value-side slices: halve their number until one is left
     if constexpr (KS > 1) {
 #pragma unroll
@@ -695,11 +817,10 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
 #pragma unroll
         for (int e = 0; e < 2; ++e) {  // rows 2 tig, 2 tig + 1
           const int i = nt * 8 + 2 * tig + e, r = r0 + i;
-          float m = -INFINITY, l = 0.f;
+          const float m = xM[i];
+          float l = 0.f;
 #pragma unroll
-          for (int w = 0; w < 8; ++w) m = fmaxf(m, xM[w * ROWS + i]);
-#pragma unroll
-          for (int w = 0; w < 8; ++w) l += xL[w * ROWS + i] * ex2(xM[w * ROWS + i] - finite_or_zero(m));
+          for (int w = 0; w < 8; ++w) l += xL[w * ROWS + i];
           // dims 64 dg + 8 gid + (0..7): MMA rows gid and gid + 8 of tile j are dims 2j and 2j + 1
           if (whole) {
             if (r < rows) {
