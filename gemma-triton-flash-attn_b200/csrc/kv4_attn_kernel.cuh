@@ -3,22 +3,27 @@
 //   O[n] = sum_j softmax_j(scale * q_n . k_j) v_j over the keys j that the
 //   causal mask and the window leave to token n, k and v read from the codes.
 //
-// Mathematics. A code c goes into the MMAs as the 16-bit number F + c: with the
-// code in the low mantissa bits of a power of two F this is one AND-OR of a
-// (shifted) code word, no conversion. bf16: F = 128 for every nibble. fp16:
-// F = 256 and 16 for even and odd nibbles, so that one shift serves two. The
-// offsets leave the results through linear terms:
-//   scores: a group's part is s * (q . (F + c) - q . F - z * sum(q)), scale
-//     and zero point applied once per group to the fp32 MMA result;
-//   values: P' = round16(s * P) is the B operand, and one more MMA subtracts
-//     sum_j (F + z_j) P'_j with the same rounded P', so the offset cancels
-//     exactly and only P' itself is rounded. The two accumulators are joined
-//     after every tile: F * sum(P') would otherwise outgrow the result over a
-//     long cache and cost it its low bits.
+// Mathematics. Scores run on integer MMAs: two ANDs and a shift split a word of
+// eight codes into two registers of bytes, and the query goes to the other
+// operand as two signed bytes, round(q * 32512 / max|q|) = 256 hi + lo, off by
+// at most 2^-16 of its row's largest value. A group's part of a score is then
+// s * (256 q_hi . c + q_lo . c - z * sum(q)) with an exact integer in the
+// brackets; scales are applied in fp32. (16-bit operands took 28 ALU
+// instructions per 16 tokens x 64 dims to make instead of 12, and the ALU is
+// the busiest pipe; fp8 MMAs of this shape are not native on sm_100.)
+//
+// Values: P' = round16(s * P) is the B operand (integers have not the range of
+// a softmax's tail), a code is set into a 16-bit number F + c, F a power of two,
+// by one AND-OR of a (shifted) word. bf16: F = 128 for every nibble. fp16:
+// F = 256 and 16 for even and odd nibbles, so that one shift serves two. One
+// more MMA subtracts sum_j (F + z_j) P'_j with the same rounded P', so the
+// offset cancels exactly and only P' itself is rounded. The two accumulators
+// are joined after every tile: F * sum(P') would otherwise outgrow the result
+// over a long cache and cost it its low bits.
 //
 // Shape. A decode step has G = H_Q / H_KV query rows per KV head, far below
 // the 128 rows of a tcgen05 tile, and reads each cached byte once: it is bound
-// by HBM. The products therefore run transposed on m16n8k16 MMAs with the
+// by HBM. The products therefore run transposed on m16n8 MMAs with the
 // CACHE as the A operand (16 tokens, or 16 dims, by 8 query rows): padding
 // costs at most 8 rows, and the codes go from shared memory to registers to
 // the tensor cores without a dequantised copy in between.
@@ -49,11 +54,11 @@ namespace gqafa {
 
 // The powers of two that codes are set into (see codes16), and their negatives.
 struct Kv4Tops {
-  uint32_t even, odd, minus_even, minus_odd, float128;
+  uint32_t even, odd, minus_even, minus_odd;
 };
 inline Kv4Tops kv4_tops(bool bf16) {
-  return bf16 ? Kv4Tops{0x43004300u, 0x43004300u, 0xC300C300u, 0xC300C300u, 0x43000000u}
-              : Kv4Tops{0x5C005C00u, 0x4C004C00u, 0xDC00DC00u, 0xCC00CC00u, 0x43000000u};
+  return bf16 ? Kv4Tops{0x43004300u, 0x43004300u, 0xC300C300u, 0xC300C300u}
+              : Kv4Tops{0x5C005C00u, 0x4C004C00u, 0xDC00DC00u, 0xCC00CC00u};
 }
 
 struct Kv4Params {
@@ -101,11 +106,11 @@ struct Kv4Cfg {
   static constexpr int STAGE_BYTES = SB * BLOCK_BYTES;
   static constexpr int Q_PITCH = D * 2 + 16;  // bytes; +16: fragment loads hit all banks
   static constexpr int Q_BYTES = ROWS * Q_PITCH;
-  static constexpr int SUMQ_BYTES = NG * ROWS * 4 * (BF16 ? 1 : 3);  // sum(q); fp16: and the MMAs' start values
+  static constexpr int SUMQ_BYTES = NG * ROWS * 4;
   static constexpr int P_PITCH = 20;          // floats of a row's 16 probabilities
   static constexpr int P_BYTES = TB * ROWS * P_PITCH * 4;  // one of two buffers
   static constexpr int M_BYTES = 8 * ROWS * 4;             // one of two buffers
-  static constexpr int MISC_BYTES = 2 * P_BYTES + 2 * M_BYTES + Q_BYTES + SUMQ_BYTES + ROWS * 8 + 256;
+  static constexpr int MISC_BYTES = 2 * P_BYTES + 2 * M_BYTES + Q_BYTES + SUMQ_BYTES + ROWS * 16 + 256;
   static constexpr int CTAS_PER_SM = NT == 1 ? 2 : 1;
   static constexpr int SMEM_BUDGET = CTAS_PER_SM == 2 ? 115000 : 232448;
   static constexpr int NST_FIT = (SMEM_BUDGET - MISC_BYTES) / STAGE_BYTES;
@@ -243,21 +248,13 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
   }
 }
 
-// d = a * b (no accumulator to clear).
-template <bool BF16>
-__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                               uint32_t b0, uint32_t b1, const float4 c) {
-  if constexpr (BF16) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
-  } else {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
-  }
+// Bytes: d = a (unsigned) * b (signed) + c.
+__device__ __forceinline__ void imma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
 }
 
 // (x & mask) | top as one LOP3. An instruction takes one immediate: `top` comes
@@ -297,11 +294,8 @@ template <bool BF16>
 __device__ __forceinline__ uint32_t minus_zero_odd(uint32_t w, const Kv4Tops& f) {
   return BF16 ? and_or(w, 0x000F000Fu, f.minus_even) : and_or(w << 6, 0x03C003C0u, f.minus_odd);
 }
-// Scale, and 128 + zero point, of the meta word in w's upper half, in fp32.
+// Scale of the meta word in w's upper half.
 __device__ __forceinline__ float meta_scale(uint32_t w) { return __uint_as_float(w & 0xFFF00000u); }
-__device__ __forceinline__ float meta_zero128(uint32_t w, const Kv4Tops& f) {
-  return __uint_as_float(and_or(w, 0x000F0000u, f.float128));
-}
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile(
@@ -323,10 +317,11 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
   float* sP = reinterpret_cast<float*>(smem + NST * C::STAGE_BYTES);  // [2][TB][ROWS][PP]
   float* sM = sP + 2 * C::P_BYTES / 4;                                 // [2][8 warps][ROWS]
   uint8_t* sQ = reinterpret_cast<uint8_t*>(sM + 2 * 8 * ROWS);         // [ROWS] rows of Q_PITCH bytes
-  float* sSum = reinterpret_cast<float*>(sQ + C::Q_BYTES);             // [NG][ROWS]
-  float* sStart = sSum + NG * ROWS;                                    // fp16: [NG][ROWS / 2] (a, b, a, b)
+  int* sSum = reinterpret_cast<int*>(sQ + C::Q_BYTES);                 // [NG][ROWS] sum of the integer query
   int2* sMask = reinterpret_cast<int2*>(sSum + C::SUMQ_BYTES / 4);     // [ROWS]: first key, number of keys
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sMask + ROWS);
+  float* sScale = reinterpret_cast<float*>(sMask + ROWS);              // [ROWS]: log2 units of score per unit of MMA result
+  int* sMost = reinterpret_cast<int*>(sScale + ROWS);                  // [ROWS]: largest |q|, as bits
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sMost + ROWS);
   __shared__ int scratch[40];
   __shared__ __align__(16) int raised[2][8];  // warps that published a maximum for a tile
   __shared__ int abort_word;
@@ -453,36 +448,67 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
 
   pieces([&](const Kv4Unit& u, int h, int t0, int t1) {
     // ---- queries of the unit, their sums per group, the rows' key ranges
+    if (threadIdx.x < ROWS) sMost[threadIdx.x] = 0;  // last read before the previous piece's last barrier
     compute_barrier();  // the previous piece's readers are done
     const int r0 = u.rt * ROWS, rows = p.G * u.qlen, off = u.len - u.qlen;
-    constexpr int CH = D / 8, RSTEP = 256 / CH;
-#pragma unroll 2
-    for (int i = threadIdx.x / CH; i < ROWS; i += RSTEP) {
-      const int c = threadIdx.x % CH, r = r0 + i;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (r < rows) {
-        const int n = r / p.G, hq = h * p.G + r - n * p.G;
-        v = *reinterpret_cast<const uint4*>(p.q + u.b * p.q_sb + hq * p.q_sh + n * p.q_sn + c * 8);
-      }
-      *reinterpret_cast<uint4*>(sQ + i * C::Q_PITCH + c * 16) = v;
-      // sums over dims 0, 1, 4, 5 (even nibbles) and 2, 3, 6, 7 (odd) of each eight
-      float even = unpack_lo<BF16>(v.x) + unpack_hi<BF16>(v.x) + unpack_lo<BF16>(v.z) + unpack_hi<BF16>(v.z);
-      float odd = unpack_lo<BF16>(v.y) + unpack_hi<BF16>(v.y) + unpack_lo<BF16>(v.w) + unpack_hi<BF16>(v.w);
+    constexpr int CH = D / 8, RSTEP = 256 / CH, RN = (ROWS + RSTEP - 1) / RSTEP;
+    const int qc = threadIdx.x % CH, qi = threadIdx.x / CH;
+    uint4 raw[RN];
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) {
-        even += __shfl_xor_sync(0xffffffffu, even, o);
-        odd += __shfl_xor_sync(0xffffffffu, odd, o);
+    for (int k = 0; k < RN; ++k) {
+      const int i = qi + k * RSTEP, r = r0 + i;
+      raw[k] = make_uint4(0, 0, 0, 0);
+      if (i < ROWS && r < rows) {
+        const int n = r / p.G, hq = h * p.G + r - n * p.G;
+        raw[k] = *reinterpret_cast<const uint4*>(p.q + u.b * p.q_sb + hq * p.q_sh + n * p.q_sn + qc * 8);
       }
-      if ((c & 7) == 0) {
-        const int g = c >> 3;
-        sSum[g * ROWS + i] = even + odd;
-        if constexpr (!BF16) {
-          // start value: 128 sum(q) - q . F, so that (128 + z) sum(q) is left to subtract
-          const float start = -128.f * even + 112.f * odd;
-          float* d = sStart + (g * (ROWS / 2) + (i >> 1)) * 4 + (i & 1);
-          d[0] = start;
-          d[2] = start;
+    }
+    auto load8 = [](const uint4& v, float (&x)[8]) {
+      x[0] = unpack_lo<BF16>(v.x), x[1] = unpack_hi<BF16>(v.x), x[2] = unpack_lo<BF16>(v.y), x[3] = unpack_hi<BF16>(v.y);
+      x[4] = unpack_lo<BF16>(v.z), x[5] = unpack_hi<BF16>(v.z), x[6] = unpack_lo<BF16>(v.w), x[7] = unpack_hi<BF16>(v.w);
+    };
+#pragma unroll
+    for (int k = 0; k < RN; ++k) {
+      float x[8];
+      load8(raw[k], x);
+      int most = 0;  // magnitudes order like their bits, infinities and NaNs last
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = max(most, static_cast<int>(__float_as_uint(x[e]) & 0x7FFFFFFFu));
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+      if ((qc & 7) == 0 && qi + k * RSTEP < ROWS) atomicMax(&sMost[qi + k * RSTEP], most);
+    }
+    compute_barrier();
+#pragma unroll
+    for (int k = 0; k < RN; ++k) {
+      const int i = qi + k * RSTEP;
+      const int bits = sMost[min(i, ROWS - 1)];
+      const float most = __int_as_float(bits);
+      const float up = fminf(32512.f / most, 1e38f);  // 1e38 for a row of zeros: its integers are 0
+      float x[8];
+      load8(raw[k], x);
+      int v[8], sum = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] = __float2int_rn(x[e] * up);
+        sum += v[e];
+      }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (i < ROWS) {
+        uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          // byte order of a word's nibbles: even ones dims 0, 4, 1, 5, odd ones 2, 6, 3, 7
+          const int reg = (e >> 1) & 1, byte = (e & 1) * 2 + (e >> 2);
+          const int vh = (v[e] + 128) >> 8;
+          hi[reg] |= (static_cast<uint32_t>(vh) & 0xFFu) << (8 * byte);
+          lo[reg] |= (static_cast<uint32_t>(v[e] - (vh << 8)) & 0xFFu) << (8 * byte);
         }
+        *reinterpret_cast<uint4*>(sQ + i * C::Q_PITCH + qc * 16) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
+        if ((qc & 7) == 0) sSum[(qc >> 3) * ROWS + i] = sum;
+        // a row with an infinity or a NaN has no finite scores
+        if (qc == 0) sScale[i] = bits >= 0x7F800000 ? NAN : p.scale_log2 * (most / 32512.f);
       }
     }
     if (threadIdx.x < ROWS) {
@@ -540,29 +566,28 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
 #pragma unroll(NT > 1 ? 2 : 4)
           for (int g = 0; g < NG; ++g) {
             const uint4 w = lds128(codes + g * KV4_CODE_BYTES);
-            const uint32_t m1 = lds32(metas + g * KV4_META_BYTES), m0 = m1 << 16;
-            const float s0 = meta_scale(m0), s1 = meta_scale(m1), z0 = meta_zero128(m0, tops), z1 = meta_zero128(m1, tops);
-            uint32_t ax[4], ay[4], az[4], aw[4];
-            codes16<BF16>(w.x, tops, ax);
-            codes16<BF16>(w.y, tops, ay);
-            codes16<BF16>(w.z, tops, az);
-            codes16<BF16>(w.w, tops, aw);
+            const uint32_t m = lds32(metas + g * KV4_META_BYTES);  // tokens gid, gid + 8
+            const float s0 = meta_scale(m << 16), s1 = meta_scale(m);
+            const int z0 = m & 15, z1 = (m >> 16) & 15;
+            const uint32_t xl = w.x & 0x0F0F0F0Fu, xh = (w.x >> 4) & 0x0F0F0F0Fu;  // token gid, word 2 tig
+            const uint32_t yl = w.y & 0x0F0F0F0Fu, yh = (w.y >> 4) & 0x0F0F0F0Fu;  // token gid, word 2 tig + 1
+            const uint32_t zl = w.z & 0x0F0F0F0Fu, zh = (w.z >> 4) & 0x0F0F0F0Fu;  // token gid + 8
+            const uint32_t wl = w.w & 0x0F0F0F0Fu, wh = (w.w >> 4) & 0x0F0F0F0Fu;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               const uint32_t qa = qbase + nt * 8 * C::Q_PITCH + g * 128;
               const uint4 q0 = lds128(qa), q1 = lds128(qa + 16);
-              float4 c = make_float4(0.f, 0.f, 0.f, 0.f);
-              if constexpr (!BF16) c = *reinterpret_cast<const float4*>(sStart + (g * (ROWS / 2) + nt * 4 + tig) * 4);
-              float t[4];
-              mma16816_first<BF16>(t, ax[0], az[0], ax[1], az[1], q0.x, q0.y, c);
-              mma16816<BF16>(t, ax[2], az[2], ax[3], az[3], q0.z, q0.w);
-              mma16816<BF16>(t, ay[0], aw[0], ay[1], aw[1], q1.x, q1.y);
-              mma16816<BF16>(t, ay[2], aw[2], ay[3], aw[3], q1.z, q1.w);
-              const float2 sq = *reinterpret_cast<const float2*>(sSum + g * ROWS + nt * 8 + 2 * tig);
-              s[kb][nt][0] = fmaf(s0, fmaf(-z0, sq.x, t[0]), s[kb][nt][0]);
-              s[kb][nt][1] = fmaf(s0, fmaf(-z0, sq.y, t[1]), s[kb][nt][1]);
-              s[kb][nt][2] = fmaf(s1, fmaf(-z1, sq.x, t[2]), s[kb][nt][2]);
-              s[kb][nt][3] = fmaf(s1, fmaf(-z1, sq.y, t[3]), s[kb][nt][3]);
+              int th[4], tl[4];
+              imma16832(th, xl, zl, xh, zh, q0.x, q0.y, 0, 0, 0, 0);
+              imma16832(tl, xl, zl, xh, zh, q0.z, q0.w, 0, 0, 0, 0);
+              imma16832(th, yl, wl, yh, wh, q1.x, q1.y, th[0], th[1], th[2], th[3]);
+              imma16832(tl, yl, wl, yh, wh, q1.z, q1.w, tl[0], tl[1], tl[2], tl[3]);
+              const int2 sq = *reinterpret_cast<const int2*>(sSum + g * ROWS + nt * 8 + 2 * tig);
+              float* v = s[kb][nt];
+              v[0] = fmaf(s0, static_cast<float>(th[0] * 256 + (tl[0] - z0 * sq.x)), v[0]);
+              v[1] = fmaf(s0, static_cast<float>(th[1] * 256 + (tl[1] - z0 * sq.y)), v[1]);
+              v[2] = fmaf(s1, static_cast<float>(th[2] * 256 + (tl[2] - z1 * sq.x)), v[2]);
+              v[3] = fmaf(s1, static_cast<float>(th[3] * 256 + (tl[3] - z1 * sq.y)), v[3]);
             }
           }
         }
@@ -580,8 +605,11 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
           const int blk = warp + 8 * kb;
           if (blk >= nv) continue;
           float* v = s[kb][nt];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] *= p.scale_log2;
+          const float2 sc = *reinterpret_cast<const float2*>(sScale + nt * 8 + 2 * tig);
+          v[0] *= sc.x;
+          v[1] *= sc.y;
+          v[2] *= sc.x;
+          v[3] *= sc.y;
           if (edge) {
             const int4 mk = *reinterpret_cast<const int4*>(sMask + nt * 8 + 2 * tig);  // two rows' (first, count)
             const int key = key_tile + blk * 16 + gid;

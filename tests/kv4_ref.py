@@ -112,8 +112,10 @@ def attention(q, k, v, kv_lens, q_lens, causal, window, scale):
       output       u |O|;
       s * P        u per key: u sum_j P_j |v_j| (the rounded products cancel the offset exactly);
       scores       fp32 sums of up to D / 16 + groups + 8 steps of terms |q_d| s (16 + 15): a score is off by at most
-                   e * steps * scale * 31 * sum_d |q_d| s, and P by twice that, relative;
-      accumulation fp32 sums over keys of terms s P (16 + 15), at most L / 16 + 64 steps;
+                   e * steps * scale * 31 * sum_d |q_d| s, and P by twice that, relative; the query's 16-bit integers
+                   are half a step off, 2^-16 of its row's largest value: 2^-16 * scale * max|q| * sum_d |k_d|;
+      accumulation fp32 sums over keys of terms s P (F + 15), joined after every tile of up to 32 MMA steps: at
+                   most e * 32 * (256 + 15) s P in a tile, and L / 16 + 64 steps of the joined sums (31 s P);
       exp2 and the joins of parts: 16 steps of fp32 relative to P."""
     B, Hq, N, D = q.shape
     G = Hq // k.shape[1]
@@ -139,6 +141,7 @@ def attention(q, k, v, kv_lens, q_lens, causal, window, scale):
         qq = q[b, :, :n].double()
         s = (qq @ kk.transpose(-1, -2) * scale).masked_fill(~ok, -math.inf)
         off = e * (D / 16 + D / 64 + 8) * scale * 31 * (qq.abs() @ kstep.transpose(-1, -2))
+        off = off + 2.0 ** -16 * scale * qq.abs().amax(-1, keepdim=True) * kk.abs().sum(-1).unsqueeze(-2)
         off = off.masked_fill(~ok, 0).amax(-1, keepdim=True) + 16 * e
         top = s.amax(-1, keepdim=True)
         seen = ~torch.isinf(top)
@@ -149,7 +152,7 @@ def attention(q, k, v, kv_lens, q_lens, causal, window, scale):
         size = p @ vv.abs()
         O[b, :, :n] = o
         lse[b, :, :n] = torch.where(l > 0, torch.log(l) + torch.where(seen, top, 0.0), -math.inf).squeeze(-1)
-        bound[b, :, :n] = u * o.abs() + 1.01 * u * size + 2 * off * size + e * (L / 16 + 64) * 31 * (p @ step)
+        bound[b, :, :n] = u * o.abs() + 1.01 * u * size + 2 * off * size + e * ((L / 16 + 64) * 31 + 32 * 271) * (p @ step)
         # numbers too small for the type round to its smallest step
         bound[b, :, :n] += torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps + (2.0 ** -25 * (p > 0).sum(-1, keepdim=True) * 31 if q.dtype == torch.float16 else 0.0)
     return O, lse, bound
