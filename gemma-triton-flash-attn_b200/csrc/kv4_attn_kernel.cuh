@@ -89,7 +89,7 @@ struct Kv4Params {
 // Blocks per warp and tile: enough work between barriers at small head_dim,
 // within the shared memory that P takes (it grows with the rows).
 __host__ __device__ constexpr int kv4_warp_blocks(int D, int NT) {
-  return D >= 256 ? 1 : (D == 128 || NT > 1 ? 2 : 4);
+  return D >= 256 || (D == 128 && NT > 2) ? 1 : (D == 128 || NT > 1 ? 2 : 4);
 }
 
 template <int D_, int NT_, bool BF16_>
@@ -117,10 +117,13 @@ struct Kv4Cfg {
   static constexpr int NST = NST_FIT < 12 ? NST_FIT : 12;
   static constexpr int SMEM_BYTES = NST * STAGE_BYTES + MISC_BYTES;
   static constexpr int THREADS = 288;
-  // A row's reference maximum is raised when a score passes it by more than
-  // this (log2 units). bf16 P' keeps its relative precision up to 2^8; fp16
-  // would overflow at large scales, so its P stays at most 1.
-  static constexpr float SLACK = BF16 ? 8.f : 0.f;
+  // Reference of a row's softmax: its largest score so far plus RAISE when it
+  // was last raised, and it is raised again when a score passes it by more than
+  // SLACK (log2 units), so P stays within 2^SLACK. bf16 P' has the range for
+  // that; fp16 P' = s * P must stay below 65504 (s is at most 8736) and loses
+  // low bits below 2^-14.
+  static constexpr float RAISE = BF16 ? 8.f : 3.f;
+  static constexpr float SLACK = BF16 ? 8.f : 2.f;
   static_assert(NST >= 4, "two stages of keys and two of values");
   // the slices' sums are joined through the P buffers
   static_assert(KS == 1 || (KS / 2) * ROWS * D * 4 <= 2 * P_BYTES, "slice exchange");
@@ -304,6 +307,24 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
       : "memory");
 }
 __device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+// The same barrier; returns whether any thread brought a true predicate.
+__device__ __forceinline__ bool compute_barrier_or(bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, 256, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(v))
+      : "memory");
+  return r != 0;
+}
+// The slow side of a wait, out of line: the fast side is one try_wait.
+__device__ __noinline__ void kv4_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
+                                           long long limit) {
+  mbar_wait(bar, parity, abort_flag, status, ST_TIMEOUT_RING_FULL, limit);
+}
 
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 
@@ -435,15 +456,23 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
   const Kv4Tops tops = p.tops;
   const uint32_t ring = smem_u32(sRing);
   const uint32_t qbase = smem_u32(sQ + gid * C::Q_PITCH + tig * 32);
-  uint32_t cnt = 0;
-  int buf = 0;
-  auto wait_full = [&](int slot, uint32_t c) {
-    mbar_wait(FULL(slot), (c / NST) & 1u, abort_flag, p.status, ST_TIMEOUT_RING_FULL, p.wait_limit);
+  int slot = 0, buf = 0;  // next ring stage, P buffer
+  uint32_t phase = 0;
+  auto wait_full = [&]() {
+    if (!mbar_try_wait(FULL(slot), phase)) kv4_wait_slow(FULL(slot), phase, abort_flag, p.status, p.wait_limit);
     __syncwarp();
   };
-  auto release = [&](int slot) {
+  // Gives the stage back and moves on. A warp that has nothing to read in a
+  // key stage gives it back unseen: it cannot come round to the same stage
+  // again before the others, there is a barrier in every tile and a tile is
+  // four stages, the ring's least length.
+  auto release = [&]() {
     __syncwarp();
     if (lane == 0) mbar_arrive(EMPTY(slot));
+    if (++slot == NST) {
+      slot = 0;
+      phase ^= 1;
+    }
   };
 
   pieces([&](const Kv4Unit& u, int h, int t0, int t1) {
@@ -550,9 +579,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
       float s[KB][NT][4];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int slot = cnt % NST;
-        wait_full(slot, cnt);
-        ++cnt;
+        if (KB > 1 || warp / SB == half) wait_full();
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           const int blk = warp + 8 * kb;
@@ -591,7 +618,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
             }
           }
         }
-        release(slot);
+        release();
       }
 
       // ---------------- softmax over this warp's blocks ----------------
@@ -631,8 +658,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb) {
             if (warp + 8 * kb >= nv) continue;
-            f0 = fmaxf(f0, fmaxf(s[kb][nt][0], s[kb][nt][2]));
-            f1 = fmaxf(f1, fmaxf(s[kb][nt][1], s[kb][nt][3]));
+            f0 = fmaxf(f0, fmaxf(s[kb][nt][0], s[kb][nt][2]) + C::RAISE);
+            f1 = fmaxf(f1, fmaxf(s[kb][nt][1], s[kb][nt][3]) + C::RAISE);
           }
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
@@ -663,12 +690,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
           d[PP + 2] = v[3];
         }
       }
-      compute_barrier();
-
       // ---------------- new maxima, if any warp published some ----------------
-      const int4 ra = *reinterpret_cast<const int4*>(&raised[buf][0]);
-      const int4 rb = *reinterpret_cast<const int4*>(&raised[buf][4]);
-      const bool rescale = (ra.x | ra.y | ra.z | ra.w | rb.x | rb.y | rb.z | rb.w) != 0;
+      const bool rescale = compute_barrier_or(raise);
       // A warp's P refers to its own published maximum, or to the old one: in
       // the value loop row gid's factor brings it to the new one.
       float vold[NT], vnew[NT];
@@ -714,9 +737,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
         for (int e = 0; e < 4; ++e) wz[nt][e] = 0.f;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int slot = cnt % NST;
-        wait_full(slot, cnt);
-        ++cnt;
+        wait_full();
         const uint32_t stage = ring + slot * C::STAGE_BYTES;
         const uint32_t codes = stage + dg * KV4_CODE_BYTES + (tig * 8 + (gid ^ (2 * tig))) * 16;
         const uint32_t metas = stage + NG * KV4_CODE_BYTES + dg * KV4_META_BYTES + tig * 8;
@@ -775,7 +796,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
             block(i * KS + ks, std::true_type{});
           }
         }
-        release(slot);
+        release();
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
