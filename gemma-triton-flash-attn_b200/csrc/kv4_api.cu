@@ -96,11 +96,12 @@ int launch_status(const char* what) {
 
 struct AttendShape {
   int B, Hq, Hkv, N, D, G;
-  int NT, rows, row_tiles, ctas;
+  int row_tiles, ctas, join_blocks;
+  long long units;
 };
 
-// Query rows of a unit (8 * NT), row tiles and CTAs. G * N rows up to 8 and 16
-// take one row tile of that height; more rows take tiles of 32.
+// Units of 8 query rows, and the CTAs of the launch: two per SM, fewer where there
+// are fewer tiles.
 AttendShape attend_shape(int B, int Hq, int Hkv, int N, int D, int max_len, int window, int sms) {
   AttendShape s{};
   s.B = B;
@@ -110,20 +111,22 @@ AttendShape attend_shape(int B, int Hq, int Hkv, int N, int D, int max_len, int 
   s.D = D;
   s.G = Hq / Hkv;
   const long long rows = static_cast<long long>(s.G) * N;
-  s.NT = rows <= 8 ? 1 : (rows <= 16 ? 2 : 4);
-  s.rows = 8 * s.NT;
-  s.row_tiles = static_cast<int>((rows + s.rows - 1) / s.rows);
-  const int tile_tokens = 8 * 16 * kv4_warp_blocks(D, s.NT);
+  s.row_tiles = static_cast<int>((rows + 7) / 8);
+  const int tile_tokens = 8 * 16 * kv4_warp_blocks(D);
   long long span = max_len;
-  if (window > 0) span = std::min<long long>(span, static_cast<long long>(window) + s.rows / s.G + 1);
+  if (window > 0) span = std::min<long long>(span, static_cast<long long>(window) + 8 / s.G + 1);
   const long long tiles = (span + 15 + tile_tokens - 1) / tile_tokens + 1;
-  const long long units = static_cast<long long>(B) * s.row_tiles * Hkv;
-  s.ctas = static_cast<int>(std::min<long long>(static_cast<long long>(sms) * (s.NT == 1 ? 2 : 1), units * tiles));
+  s.units = static_cast<long long>(B) * s.row_tiles * Hkv;
+  s.ctas = static_cast<int>(std::min<long long>(2LL * sms, s.units * tiles));
+  // the join: at most two CTAs per SM, all of them where few units are cut into many parts
+  s.join_blocks = 1;
+  while (s.join_blocks < 8 * D / 128 && s.join_blocks * s.units <= sms) s.join_blocks *= 2;
   return s;
 }
 
+// Parts [2 * ctas][8][D] fp32, their maxima and sums [2 * ctas][8].
 long long attend_workspace(const AttendShape& s) {
-  return 2LL * s.ctas * s.rows * (static_cast<long long>(s.D) * 4 + 8) + 256;
+  return 2LL * s.ctas * 8 * (static_cast<long long>(s.D) * 4 + 8) + 256;
 }
 
 template <class C>
@@ -138,18 +141,16 @@ int launch_attend(Kv4Params p, cudaStream_t st) {
     if (e != cudaSuccess) return fail(GQAFA_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     attr_done_mask.fetch_or(bit);
   }
-  const long long rows_here = std::min<long long>(C::ROWS, static_cast<long long>(p.G) * p.N);
-  const long long blocks =
-      static_cast<long long>(p.B) * p.row_tiles * p.Hkv * rows_here * (C::D < 128 ? 1 : C::D / 128);
+  const long long blocks = static_cast<long long>(p.B) * p.row_tiles * p.Hkv * p.join_blocks;
   if (blocks > INT_MAX) return fail(GQAFA_ERR_INVALID, "grid size %lld out of range", blocks);
   kv4_attn_kernel<C><<<p.ctas, C::THREADS, C::SMEM_BYTES, st>>>(p);
-  int rc = launch_status("4-bit cache attention");
+  const int rc = launch_status("4-bit cache attention");
   if (rc) return rc;
   // The join starts while the attention's last CTAs run (programmatic
   // dependent launch): it reads the lengths and then waits for them.
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(512);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -161,20 +162,13 @@ int launch_attend(Kv4Params p, cudaStream_t st) {
   return GQAFA_OK;
 }
 
-template <int D, bool BF16>
-int attend_rows(int nt, const Kv4Params& p, cudaStream_t st) {
-  if (nt == 1) return launch_attend<Kv4Cfg<D, 1, BF16>>(p, st);
-  if (nt == 2) return launch_attend<Kv4Cfg<D, 2, BF16>>(p, st);
-  return launch_attend<Kv4Cfg<D, 4, BF16>>(p, st);
-}
-
 template <bool BF16>
-int attend_dim(int D, int nt, const Kv4Params& p, cudaStream_t st) {
+int attend_dim(int D, const Kv4Params& p, cudaStream_t st) {
   switch (D) {
-    case 64: return attend_rows<64, BF16>(nt, p, st);
-    case 128: return attend_rows<128, BF16>(nt, p, st);
-    case 256: return attend_rows<256, BF16>(nt, p, st);
-    default: return attend_rows<512, BF16>(nt, p, st);
+    case 64: return launch_attend<Kv4Cfg<64, BF16>>(p, st);
+    case 128: return launch_attend<Kv4Cfg<128, BF16>>(p, st);
+    case 256: return launch_attend<Kv4Cfg<256, BF16>>(p, st);
+    default: return launch_attend<Kv4Cfg<512, BF16>>(p, st);
   }
 }
 
@@ -437,12 +431,12 @@ extern "C" int gqafa_kv4_attend(const void* q, const long long* q_strides, const
   p.row_tiles = s.row_tiles;
   p.ctas = s.ctas;
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) +
-                                        2LL * s.ctas * s.rows * static_cast<long long>(s.D) * 4);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + 2LL * s.ctas * 8 * s.D);
+  p.join_blocks = s.join_blocks;
   p.status = status_ptr();
   if (!p.status) return fail(GQAFA_ERR_CUDA, "cannot resolve the device status word");
   p.wait_limit = wait_limit_setting();
   p.no_loads = no_loads_setting();
-  return dtype == GQAFA_DTYPE_BF16 ? attend_dim<true>(head_dim, s.NT, p, st)
-                                   : attend_dim<false>(head_dim, s.NT, p, st);
+  return dtype == GQAFA_DTYPE_BF16 ? attend_dim<true>(head_dim, p, st)
+                                   : attend_dim<false>(head_dim, p, st);
 }

@@ -43,7 +43,11 @@
 // long request both fill the GPU. A unit inside one share is written straight
 // to the output; parts of a cut unit go to a workspace (fp32, with maximum and
 // sum) and kv4_combine_kernel joins them in list order, so results do not
-// depend on timing.
+// depend on timing. (The last CTA to arrive joining them inside this kernel was
+// slower: 16 parts of 16 KB take one CTA 10 us.) A unit has at most 8 rows; more
+// rows take more units, which read the keys again from L2: units of 16 and 32
+// rows (more registers, one CTA per SM) were slower, 50 and 67 us against 41
+// for 20 rows at head_dim 128.
 #pragma once
 #include <type_traits>
 
@@ -81,25 +85,23 @@ struct Kv4Params {
   int ctas;       // CTAs of the attention launch (the combine launch needs it)
   float* part_o;  // [2 * ctas][8 * NT][D]
   float2* part_ml;  // [2 * ctas][8 * NT]: maximum (log2 units), sum
+  int join_blocks;  // CTAs of the join per unit
   int* status;
   long long wait_limit;
   int no_loads;
 };
 
-// Blocks per warp and tile: enough work between barriers at small head_dim,
-// within the shared memory that P takes (it grows with the rows).
-__host__ __device__ constexpr int kv4_warp_blocks(int D, int NT) {
-  return D >= 256 || (D == 128 && NT > 2) ? 1 : (D == 128 || NT > 1 ? 2 : 4);
-}
+// Blocks per warp and tile: enough work between barriers at small head_dim.
+__host__ __device__ constexpr int kv4_warp_blocks(int D) { return D >= 256 ? 1 : (D == 128 ? 2 : 4); }
 
-template <int D_, int NT_, bool BF16_>
+template <int D_, bool BF16_>
 struct Kv4Cfg {
-  static constexpr int D = D_, NT = NT_;
+  static constexpr int D = D_;
   static constexpr bool BF16 = BF16_;
-  static constexpr int ROWS = 8 * NT;         // query rows of a unit
+  static constexpr int ROWS = 8;              // query rows of a unit
   static constexpr int NG = D / KV4_GROUP;    // groups of a token
   static constexpr int KS = 8 / NG;           // value-side slices of a tile's blocks
-  static constexpr int KB = kv4_warp_blocks(D, NT);
+  static constexpr int KB = kv4_warp_blocks(D);
   static constexpr int TB = 8 * KB;           // blocks per tile
   static constexpr int SB = TB / 2;           // blocks per stage
   static constexpr int BLOCK_BYTES = kv4_block_bytes(D);
@@ -111,9 +113,8 @@ struct Kv4Cfg {
   static constexpr int P_BYTES = TB * ROWS * P_PITCH * 4;  // one of two buffers
   static constexpr int M_BYTES = 8 * ROWS * 4;             // one of two buffers
   static constexpr int MISC_BYTES = 2 * P_BYTES + 2 * M_BYTES + Q_BYTES + SUMQ_BYTES + ROWS * 16 + 256;
-  static constexpr int CTAS_PER_SM = NT == 1 ? 2 : 1;
-  static constexpr int SMEM_BUDGET = CTAS_PER_SM == 2 ? 115000 : 232448;
-  static constexpr int NST_FIT = (SMEM_BUDGET - MISC_BYTES) / STAGE_BYTES;
+  static constexpr int CTAS_PER_SM = 2;
+  static constexpr int NST_FIT = (115000 - MISC_BYTES) / STAGE_BYTES;
   static constexpr int NST = NST_FIT < 12 ? NST_FIT : 12;
   static constexpr int SMEM_BYTES = NST * STAGE_BYTES + MISC_BYTES;
   static constexpr int THREADS = 288;
@@ -330,7 +331,7 @@ __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY
 
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(const Kv4Params p) {
-  constexpr int D = C::D, NT = C::NT, NG = C::NG, KS = C::KS, KB = C::KB, TB = C::TB, SB = C::SB, ROWS = C::ROWS;
+  constexpr int D = C::D, NT = 1, NG = C::NG, KS = C::KS, KB = C::KB, TB = C::TB, SB = C::SB, ROWS = C::ROWS;
   constexpr int NST = C::NST, BB = C::BLOCK_BYTES, PP = C::P_PITCH;
   constexpr bool BF16 = C::BF16;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -368,8 +369,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
   const int first_tile = static_cast<int>(begin);
   const int last_tile = min(share.total, first_tile + per);
 
-  // Walk the pieces of the share: f(unit, entry's first tile, head, tile
-  // range inside the unit). Producer and compute warps walk the same way.
+  // Walk the pieces of the share: f(unit, head, tile range inside the unit). Producer and compute warps walk the same way.
   auto pieces = [&](auto&& f) {
     int entry = share.entry, base = share.base, at = first_tile;
     while (at < last_tile) {
@@ -900,112 +900,123 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
 }
 
 // Joins the parts of units that several CTAs worked on, and writes zeros for
-// rows that no unit covers. One CTA per (unit, row, 128 dims): warp w adds parts w,
-// w + 8, ...; then the eight partial sums are added in order. For a unit that
-// one CTA did alone there is nothing to do.
+// rows that no unit covers (no token, or no key to see): join_blocks CTAs per
+// unit, each a slice of its [rows][D] output, every lane four neighbouring
+// floats. Where a slice is narrower than the CTA, groups of warps take every
+// n-th part and are added up in order at the end; four parts are in flight per
+// warp, so a unit cut into 148 parts takes a few memory latencies.
 template <class C>
-__global__ void __launch_bounds__(256) kv4_combine_kernel(const Kv4Params p) {
-  constexpr int D = C::D, ROWS = C::ROWS, DC = D < 128 ? D : 128;
-  __shared__ int scratch[40];
-  __shared__ float4 sum[8][32];
-  __shared__ float2 ml[8];
+__global__ void __launch_bounds__(512, 2) kv4_combine_kernel(const Kv4Params p) {
+  constexpr int D = C::D, ROWS = C::ROWS;
+  __shared__ float4 sAcc[16][32];
+  __shared__ float2 sMl[16][32];
+  __shared__ int scratch[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int idx = blockIdx.x;
-  const int dc = idx % (D / DC);
-  idx /= (D / DC);
-  const int rows_here = min(ROWS, p.G * p.N);
-  const int i = idx % rows_here;
-  idx /= rows_here;
-  const int h = idx % p.Hkv, entry = idx / p.Hkv;
-  const Kv4Unit u = kv4_unit<C>(p, entry);
-  const int r = u.rt * ROWS + i;
-  if (r >= p.G * p.N) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    return;
-  }
-  const int n = r / p.G, hq = h * p.G + r - n * p.G;
-  uint16_t* o = p.o + u.b * p.o_sb + hq * p.o_sh + n * p.o_sn + dc * DC + lane * 4;
-  float* lse = (p.lse && dc == 0) ? p.lse + (static_cast<long long>(u.b) * p.Hq + hq) * p.N + n : nullptr;
-  const bool unseen = u.tiles == 0 || n >= u.qlen;
-  // first tile of the unit: tiles of all entries before it, then of its heads
+  const int unit = blockIdx.x / p.join_blocks, slice = blockIdx.x - unit * p.join_blocks;
+  const int entry = unit / p.Hkv, h = unit - entry * p.Hkv;
+  // Where the unit lies in the list of tiles. This reads the lengths only,
+  // which the attention launch does not write: it may run beside it.
   const int entries = p.B * p.row_tiles;
   int before = 0, total = 0;
-  for (int e = threadIdx.x; e < entries; e += 256) {
+  for (int e = threadIdx.x; e < entries; e += 512) {
     const int t = kv4_unit<C>(p, e).tiles * p.Hkv;
     total += t;
     if (e < entry) before += t;
   }
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, s);
-    total += __shfl_xor_sync(0xffffffffu, total, s);
-  }
+  before = __reduce_add_sync(0xffffffffu, before);
+  total = __reduce_add_sync(0xffffffffu, total);
   if (lane == 0) {
     scratch[warp] = before;
-    scratch[8 + warp] = total;
+    scratch[16 + warp] = total;
   }
   __syncthreads();
-  before = total = 0;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    before += scratch[w];
-    total += scratch[8 + w];
-  }
-  // only the lengths, which the attention launch does not write, are read before it ends
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (unseen) {
-    if (warp == 0) {
-      if (lane * 4 < DC) *reinterpret_cast<uint2*>(o) = make_uint2(0, 0);
-      if (lse && lane == 0) *lse = -INFINITY;
-    }
-    return;
-  }
+  before = __reduce_add_sync(0xffffffffu, lane < 16 ? scratch[lane] : 0);
+  total = __reduce_add_sync(0xffffffffu, lane < 16 ? scratch[16 + lane] : 0);
+  const Kv4Unit u = kv4_unit<C>(p, entry);
   const int per = max(1, (total + p.ctas - 1) / p.ctas);
-  const int first = before + h * u.tiles, last = first + u.tiles - 1;
-  const int c0 = first / per, c1 = last / per;
-  if (c0 == c1) return;  // written by its one CTA
+  const int begin = before + h * u.tiles;
+  const int c0 = begin / per, c1 = u.tiles == 0 ? c0 : (begin + u.tiles - 1) / per;
+  const int limit = min(ROWS, p.G * p.N - u.rt * ROWS);                      // rows of the output
+  const int rows = u.tiles == 0 ? 0 : min(limit, p.G * u.qlen - u.rt * ROWS);  // of them with keys
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (c0 == c1 && rows == limit) return;  // written by its one CTA
+  // columns of 128 floats; the slice's are [first, first + columns)
+  const int columns = (ROWS * D / 128) / p.join_blocks, first = slice * columns;
+  const int groups = columns < 16 ? 16 / columns : 1;  // warps per column
   // part of CTA c: its share's first piece unless the unit starts there
-  auto part_of = [&](int c) { return 2 * c + (c == c0 ? 1 : 0); };
-  float m = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, p.part_ml[static_cast<long long>(part_of(c)) * ROWS + i].x);
+  auto part_of = [&](int c) { return static_cast<long long>(2 * c + (c == c0 ? 1 : 0)); };
+  for (int k = warp / groups; k < columns; k += 16 / groups) {
+    const int at = ((first + k) * 32 + lane) * 4, i = at / D, d = at - i * D;
+    const int grp = warp % groups;
+    float m = -INFINITY, l = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i < rows && c0 < c1) {
+      constexpr int U = 4;  // parts in flight
+#pragma unroll 1
+      for (int c = c0 + grp; c <= c1; c += U * groups) {
+        float2 q[U];
+        float4 v[U];
 #pragma unroll
-  for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-  const float fm = finite_or_zero(m);
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-#pragma unroll 4
-  for (int c = c0 + warp; c <= c1; c += 8) {
-    const long long at = static_cast<long long>(part_of(c)) * ROWS + i;
-    const float2 q = p.part_ml[at];
-    const float f = ex2(q.x - fm);
-    l += q.y * f;
-    if (lane * 4 < DC) {
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * D + dc * DC + lane * 4);
-      a.x = fmaf(v.x, f, a.x);
-      a.y = fmaf(v.y, f, a.y);
-      a.z = fmaf(v.z, f, a.z);
-      a.w = fmaf(v.w, f, a.w);
+        for (int j = 0; j < U; ++j) {
+          const long long row = part_of(min(c + j * groups, c1)) * ROWS + i;
+          q[j] = __ldcg(p.part_ml + row);
+          v[j] = __ldcg(reinterpret_cast<const float4*>(p.part_o + row * D + d));
+        }
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+          if (c + j * groups > c1) q[j] = make_float2(-INFINITY, 0.f);
+          top = fmaxf(top, q[j].x);
+        }
+        const float ft = finite_or_zero(top), f0 = ex2(m - ft);
+        m = top;
+        l *= f0;
+        a.x *= f0, a.y *= f0, a.z *= f0, a.w *= f0;
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+          if (c + j * groups <= c1) {
+            const float f = ex2(q[j].x - ft);
+            l = fmaf(q[j].y, f, l);
+            a.x = fmaf(v[j].x, f, a.x);
+            a.y = fmaf(v[j].y, f, a.y);
+            a.z = fmaf(v[j].z, f, a.z);
+            a.w = fmaf(v[j].w, f, a.w);
+          }
+        }
+      }
+    }
+    if (groups > 1) {  // then every warp has exactly one column
+      sAcc[warp][lane] = a;
+      sMl[warp][lane] = make_float2(m, l);
+      __syncthreads();
+      if (grp != 0) return;
+      float top = m;
+      for (int w = 1; w < groups; ++w) top = fmaxf(top, sMl[warp + w][lane].x);
+      const float ft = finite_or_zero(top), f0 = ex2(m - ft);
+      m = top;
+      l *= f0;
+      a.x *= f0, a.y *= f0, a.z *= f0, a.w *= f0;
+      for (int w = 1; w < groups; ++w) {
+        const float2 q = sMl[warp + w][lane];
+        const float4 v = sAcc[warp + w][lane];
+        const float f = ex2(q.x - ft);
+        l = fmaf(q.y, f, l);
+        a.x = fmaf(v.x, f, a.x);
+        a.y = fmaf(v.y, f, a.y);
+        a.z = fmaf(v.z, f, a.z);
+        a.w = fmaf(v.w, f, a.w);
+      }
+    }
+    if (i < limit && (i >= rows || c0 < c1)) {
+      const int r = u.rt * ROWS + i, n = r / p.G, hq = h * p.G + r - n * p.G;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      *reinterpret_cast<uint2*>(p.o + u.b * p.o_sb + hq * p.o_sh + n * p.o_sn + d) =
+          make_uint2(pack2<C::BF16>(a.x * inv, a.y * inv), pack2<C::BF16>(a.z * inv, a.w * inv));
+      if (p.lse && d == 0)
+        p.lse[(static_cast<long long>(u.b) * p.Hq + hq) * p.N + n] =
+            l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
     }
   }
-  sum[warp][lane] = a;
-  if (lane == 0) ml[warp] = make_float2(l, 0.f);
-  __syncthreads();
-  if (warp != 0) return;
-  a = make_float4(0.f, 0.f, 0.f, 0.f);
-  l = 0.f;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    const float4 v = sum[w][lane];
-    a.x += v.x;
-    a.y += v.y;
-    a.z += v.z;
-    a.w += v.w;
-    l += ml[w].x;
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (lane * 4 < DC)
-    *reinterpret_cast<uint2*>(o) = make_uint2(pack2<C::BF16>(a.x * inv, a.y * inv), pack2<C::BF16>(a.z * inv, a.w * inv));
-  if (lse && lane == 0) *lse = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
 }
 
 }  // namespace gqafa
