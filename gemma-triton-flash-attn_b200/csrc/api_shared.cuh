@@ -18,4 +18,22 @@ int* status_ptr();
 long long wait_limit_setting();
 int no_loads_setting();
 
+// Forward whose batch elements have their own lengths (int32 device arrays,
+// see ragged_lens): q [B, Hq, N, D] with strides, k and v contiguous
+// [B, Hkv, Nk, D], lse (may be null) [B, Hq, N]. Arguments are the caller's to
+// check; the device is bound.
+struct RaggedForward {
+  const void* q;
+  const long long* q_strides;
+  const void *k, *v;
+  void* o;
+  const long long* o_strides;
+  float* lse;
+  const int *kv_lens, *q_lens;
+  int B, Hq, Hkv, N, Nk, D, kv_cap, causal, window;
+  float scale;
+  bool bf16;
+};
+int ragged_forward(const RaggedForward& r, cudaStream_t stream);
+
 }  // namespace gqafa

@@ -85,6 +85,35 @@ struct KParams {
   // dK / dV outputs (out, out2 of the DK, DV and dK+dV roles) are fp32 rather
   // than the input dtype: partial sums that a caller adds up before rounding.
   int out_f32;
+  // Ragged forward (Ragged<...> configurations): batch element b has its own
+  // lengths, read on the device. See ragged_lens.
+  const int* kv_lens;
+  const int* q_lens;  // null: N rows each
+  int kv_cap;         // kv_lens are at most this
+};
+
+// Lengths of batch element b in the ragged forward. K and V hold, from row 0
+// on, the keys from position `start` to the request's last: all of them, or
+// (window) from the block of 16 that holds the first key a row can see. N is
+// the number of query rows, which are the last of the Nk keys.
+struct RaggedLens {
+  int N, Nk, start;
+};
+__device__ __forceinline__ RaggedLens ragged_lens(const int* kv_lens, const int* q_lens, int b, int cap, int rows,
+                                                  int window) {
+  RaggedLens r;
+  const int len = min(max(kv_lens[b], 0), cap);
+  r.N = q_lens ? min(max(q_lens[b], 0), rows) : rows;
+  r.start = window > 0 ? max(0, len - r.N - window + 1) & ~15 : 0;
+  r.Nk = len - r.start;
+  return r;
+}
+
+// A forward configuration whose batch elements have their own lengths. Rows
+// without a token, and rows that see no key, are written as zeros (LSE -inf).
+template <class Base>
+struct Ragged : Base {
+  static constexpr bool RAGGED = true;
 };
 
 // Indices of the wait-cycle diagnostics counters.
@@ -134,6 +163,7 @@ struct Cfg {
   static constexpr int NSTAGES = NSTAGES_, YGROUP = YGROUP_;
   static constexpr bool BF16 = BF16_;
   static constexpr bool PAIR = false;
+  static constexpr bool RAGGED = false;
   static constexpr int MP = M;  // rows of one grid tile
   static constexpr bool HAS_DP = (ROLE == ROLE_DQ || ROLE == ROLE_DK);
   static constexpr bool ROWS_ARE_Q = (ROLE == ROLE_FWD || ROLE == ROLE_DQ);
@@ -329,15 +359,23 @@ __global__ void __launch_bounds__(256, 1)
   // FWD/DQ: the last q tiles carry the most causal work, launch them first.
   const int tile = p.tile_begin + (C::ROWS_ARE_Q ? (p.num_row_tiles - 1 - idx) : idx);
   const int r0 = tile * M;
-  const int N = p.N, G = p.G;
+  int N = p.N, Nk = p.Nk, qoff = p.qoff;
+  if constexpr (C::RAGGED) {
+    const RaggedLens len = ragged_lens(p.kv_lens, p.q_lens, b, p.kv_cap, p.N, p.window);
+    N = len.N;
+    Nk = len.Nk;
+    qoff = Nk - N;
+  }
+  const int G = p.G;
   const bool swa = p.causal && p.window > 0;
 
   int jlo, jn, n_items;
   if constexpr (C::ROWS_ARE_Q) {
-    const int kv_hi = p.causal ? min(p.Nk, r0 + M + p.qoff) : p.Nk;
-    const int kv_lo = swa ? max(0, r0 + p.qoff - p.window + 1) : 0;
+    const int kv_hi = p.causal ? min(Nk, r0 + M + qoff) : Nk;
+    const int kv_lo = swa ? max(0, r0 + qoff - p.window + 1) : 0;
     jlo = kv_lo / BN;
     jn = (kv_hi + BN - 1) / BN - jlo;
+    if (C::RAGGED && (r0 >= N || kv_hi <= kv_lo)) jn = 0;
     n_items = jn;
   } else {
     const int q_lo = p.causal ? r0 : 0;
@@ -503,7 +541,7 @@ __global__ void __launch_bounds__(256, 1)
     // per-row state
     float m_run = -INFINITY, l_run = 0.f;      // FWD
     float row_lse2 = 0.f, row_delta = 0.f;     // DQ
-    const long long rowbase_q = (static_cast<long long>(b) * p.Hq + (C::ROWS_ARE_Q ? h : 0)) * N;
+    const long long rowbase_q = (static_cast<long long>(b) * p.Hq + (C::ROWS_ARE_Q ? h : 0)) * p.N;
 
     if constexpr (C::ROLE == ROLE_DQ) {
       // delta = rowsum(dO o O), one warp per row, coalesced 16-byte loads.
@@ -526,14 +564,14 @@ __global__ void __launch_bounds__(256, 1)
       const uint32_t dp_col = C::S_COL0 + (NS + sb) * BN;
       bool need_mask;
       if constexpr (C::ROWS_ARE_Q) {
-        need_mask = (c0 + BN > p.Nk) || (p.causal && c0 + BN - 1 > r0 + p.qoff) ||
-                    (swa && r0 + p.qoff + M - 1 - c0 >= p.window);
+        need_mask = (c0 + BN > Nk) || (p.causal && c0 + BN - 1 > r0 + qoff) ||
+                    (swa && r0 + qoff + M - 1 - c0 >= p.window) || (C::RAGGED && r0 + M > N);
       } else {
         need_mask = (c0 + BN > N) || (p.causal && r0 + M - 1 > c0) ||
                     (swa && c0 + BN - 1 - r0 >= p.window);
       }
       int lo_abs, hi_abs;
-      attended_interval(C::ROWS_ARE_Q, r0 + srow, N, p.Nk, p.qoff, p.causal, p.window, lo_abs, hi_abs);
+      attended_interval(C::ROWS_ARE_Q, r0 + srow, N, Nk, qoff, p.causal, p.window, lo_abs, hi_abs);
       const int lo_rel = lo_abs - c0;
       const unsigned span = span_of(lo_rel, hi_abs - c0);
       auto valid = [&](int c) { return static_cast<unsigned>(c - lo_rel) < span; };
@@ -683,15 +721,26 @@ __global__ void __launch_bounds__(256, 1)
         tmem_ld32(tq + 32 * k, r);
         float v[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * mul;
-        if (orow < N) store_out32<C::BF16>(p.out, obase + 32 * k, v, !C::ROWS_ARE_Q && p.out_f32);
+        for (int j = 0; j < 32; ++j) {
+          v[j] = __uint_as_float(r[j]) * mul;
+          if (C::RAGGED && l_run == 0.f) v[j] = 0.f;
+        }
+        if (orow < (C::RAGGED ? p.N : N))
+          store_out32<C::BF16>(p.out, obase + 32 * k, v, !C::ROWS_ARE_Q && p.out_f32);
       }
       if constexpr (C::ROLE == ROLE_FWD) {
-        if (p.lse != nullptr && orow < N) {
+        if (p.lse != nullptr && orow < (C::RAGGED ? p.N : N)) {
           const float LN2 = 0.6931471805599453f;
           p.lse[rowbase_q + orow] = (l_run > 0.f) ? (m_run + __log2f(l_run)) * LN2 : -INFINITY;
         }
       }
+    } else if (C::RAGGED && n_items == 0 && r0 + srow < p.N) {
+      const long long obase = static_cast<long long>(b) * p.out_sb + static_cast<long long>(h) * p.out_sh +
+                              static_cast<long long>(r0 + srow) * p.out_sn;
+      const float zero[32] = {};
+#pragma unroll 1
+      for (int k = 0; k < C::D / 32; ++k) store_row32<C::BF16>(p.out, obase + 32 * k, zero);
+      if (p.lse != nullptr) p.lse[rowbase_q + r0 + srow] = -INFINITY;
     }
   }
 

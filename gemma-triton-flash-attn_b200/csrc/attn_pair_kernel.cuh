@@ -38,6 +38,7 @@ struct PairCfg {
   static constexpr int THREADS = 128 + 128 * RW;
   static constexpr bool BF16 = BF16_;
   static constexpr bool PAIR = true;
+  static constexpr bool RAGGED = false;
   static constexpr int M = 64;     // rows per CTA
   static constexpr int MP = 128;   // rows per pair
   static constexpr int NCHUNK = 1;
@@ -150,15 +151,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
   const int tile = p.tile_begin + (C::ROWS_ARE_Q ? (p.num_row_tiles - 1 - idx) : idx);
   const int pr0 = tile * MP;
   const int r0 = pr0 + M * static_cast<int>(rank);
-  const int N = p.N, G = p.G;
+  int N = p.N, Nk = p.Nk, qoff = p.qoff;
+  if constexpr (C::RAGGED) {
+    const RaggedLens len = ragged_lens(p.kv_lens, p.q_lens, b, p.kv_cap, p.N, p.window);
+    N = len.N;
+    Nk = len.Nk;
+    qoff = Nk - N;
+  }
+  const int G = p.G;
   const bool swa = p.causal && p.window > 0;
 
   int jlo, jn, n_items;
   if constexpr (C::ROWS_ARE_Q) {
-    const int kv_hi = p.causal ? min(p.Nk, pr0 + MP + p.qoff) : p.Nk;
-    const int kv_lo = swa ? max(0, pr0 + p.qoff - p.window + 1) : 0;
+    const int kv_hi = p.causal ? min(Nk, pr0 + MP + qoff) : Nk;
+    const int kv_lo = swa ? max(0, pr0 + qoff - p.window + 1) : 0;
     jlo = kv_lo / BN;
     jn = (kv_hi + BN - 1) / BN - jlo;
+    if (C::RAGGED && (pr0 >= N || kv_hi <= kv_lo)) jn = 0;
     n_items = jn;
   } else {
     const int q_lo = p.causal ? pr0 : 0;
@@ -422,7 +431,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
     const float sl2 = p.scale_log2;
     bool ok = true;
     float row_lse2 = 0.f, row_delta = 0.f;
-    const long long rowbase_q = (static_cast<long long>(b) * p.Hq + (C::ROWS_ARE_Q ? h : 0)) * N;
+    const long long rowbase_q = (static_cast<long long>(b) * p.Hq + (C::ROWS_ARE_Q ? h : 0)) * p.N;
     const uint32_t pready_l0 = mapa_shared(BAR_PREADY(0), 0);
     const uint32_t sfree_l0 = mapa_shared(BAR_SFREE(0), 0);
 
@@ -471,7 +480,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
         // all columns would multiply the code size, and the instruction cache
         // is shared with the MMA-issuing thread.
         int lo_abs, hi_abs;
-        attended_interval(true, r0 + row, N, p.Nk, p.qoff, p.causal, p.window, lo_abs, hi_abs);
+        attended_interval(true, r0 + row, N, Nk, qoff, p.causal, p.window, lo_abs, hi_abs);
         const int lo_rel = lo_abs - cb;
         const unsigned span = span_of(lo_rel, hi_abs - cb);
         float mx = -INFINITY;
@@ -597,14 +606,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
             tmem_ld32(tq + g * 128 + 32 * k, r);
             float v[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * mul;
-            if (orow < N) store_row32<C::BF16>(p.out, obase + 256 * g + 128 * half + 32 * k, v);
+            for (int j = 0; j < 32; ++j) {
+              v[j] = __uint_as_float(r[j]) * mul;
+              if (C::RAGGED && l_tot == 0.f) v[j] = 0.f;
+            }
+            if (orow < (C::RAGGED ? p.N : N))
+              store_row32<C::BF16>(p.out, obase + 256 * g + 128 * half + 32 * k, v);
           }
         }
-        if (p.lse != nullptr && part == 0 && orow < N) {
+        if (p.lse != nullptr && part == 0 && orow < (C::RAGGED ? p.N : N)) {
           const float LN2 = 0.6931471805599453f;
           p.lse[rowbase_q + orow] = (l_tot > 0.f) ? (m_run + __log2f(l_tot)) * LN2 : -INFINITY;
         }
+      } else if (C::RAGGED && n_items == 0 && r0 + row < p.N) {
+        const long long obase = static_cast<long long>(b) * p.out_sb + static_cast<long long>(h) * p.out_sh +
+                                static_cast<long long>(r0 + row) * p.out_sn;
+        const float zero[32] = {};
+#pragma unroll 1
+        for (int e = cs * (4 * C::NACC / RW); e < (cs + 1) * (4 * C::NACC / RW); ++e)
+          store_row32<C::BF16>(p.out, obase + 256 * (e >> 2) + 128 * half + 32 * (e & 3), zero);
+        if (p.lse != nullptr && part == 0) p.lse[rowbase_q + r0 + row] = -INFINITY;
       }
       tock(WC_ROW_EPILOGUE, t_epi);
     } else {
@@ -676,7 +697,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
         if (ok) {
           tc_fence_after();
           int lo_abs, hi_abs;
-          attended_interval(C::ROWS_ARE_Q, r0 + row, N, p.Nk, p.qoff, p.causal, p.window, lo_abs, hi_abs);
+          attended_interval(C::ROWS_ARE_Q, r0 + row, N, Nk, qoff, p.causal, p.window, lo_abs, hi_abs);
           const int lo_rel = lo_abs - cb;
           const unsigned span = span_of(lo_rel, hi_abs - cb);
 #pragma unroll

@@ -326,6 +326,46 @@ int fwd_impl(const Problem& pr, const TensorDesc& q, const TensorDesc& k, const 
   return launch<CF>(maps, p, st);
 }
 
+// The ragged forward (api_shared.cuh) over dense K and V.
+template <bool BF16, class CF>
+int ragged_impl(const RaggedForward& r, const TensorDesc& q, const TensorDesc& od, cudaStream_t st) {
+  using C = Ragged<CF>;
+  Problem pr{};
+  pr.B = r.B;
+  pr.Hq = r.Hq;
+  pr.Hkv = r.Hkv;
+  pr.N = r.N;
+  pr.Nk = r.Nk;
+  pr.D = r.D;
+  pr.causal = r.causal;
+  pr.window = r.window;
+  pr.scale = r.scale;
+  pr.row_end = r.N;
+  TensorDesc kd{r.k, (long long)r.Hkv * r.Nk * r.D, (long long)r.Nk * r.D, r.D, r.Hkv}, vd = kd;
+  vd.ptr = r.v;
+  CUtensorMap maps[6];
+  int rc, cbox = C::BN, ybox = C::BN;
+  if constexpr (C::PAIR) {
+    cbox = C::C_BOX;
+    ybox = C::Y_BOX;
+  }
+  if ((rc = encode_map(&maps[0], q, pr.B, pr.N, pr.D, C::M, BF16))) return rc;
+  if ((rc = encode_map(&maps[2], kd, pr.B, pr.Nk, pr.D, cbox, BF16))) return rc;
+  if ((rc = encode_map(&maps[4], vd, pr.B, pr.Nk, pr.D, ybox, BF16))) return rc;
+  maps[1] = maps[0];
+  maps[3] = maps[2];
+  maps[5] = maps[0];
+  KParams p = base_params(pr);
+  set_out(p, r.o, od);
+  p.lse = r.lse;
+  p.status = status_ptr();
+  if (!p.status) return fail(GQAFA_ERR_CUDA, "cannot resolve the device status word");
+  p.kv_lens = r.kv_lens;
+  p.q_lens = r.q_lens;
+  p.kv_cap = r.kv_cap;
+  return launch<C>(maps, p, st);
+}
+
 template <bool BF16, class CQ, class CK, class CV>
 int bwd_impl(const Problem& pr, const TensorDesc& q, const TensorDesc& k, const TensorDesc& v,
              const TensorDesc& o, const TensorDesc& dout, const float* lse, void* dq, const TensorDesc& dqd,
@@ -559,6 +599,31 @@ static int fwd_entry(int row_begin, int row_end, const void* q, const long long*
   return pr.bf16 ? fwd_impl<true, Fwd512<true>>(pr, qd, kd, vd, o, od, lse, st)
                  : fwd_impl<false, Fwd512<false>>(pr, qd, kd, vd, o, od, lse, st);
 }
+
+namespace gqafa {
+
+int ragged_forward(const RaggedForward& r, cudaStream_t st) {
+  TensorDesc qd, od;
+  int rc;
+  if ((rc = check_tensor("q", r.q, r.q_strides, r.B, r.Hq, r.N, r.D, &qd))) return rc;
+  if ((rc = check_tensor("o", r.o, r.o_strides, r.B, r.Hq, r.N, r.D, &od))) return rc;
+  if (r.bf16) {
+    switch (r.D) {
+      case 64: return ragged_impl<true, Fwd64<true>>(r, qd, od, st);
+      case 128: return ragged_impl<true, Fwd128<true>>(r, qd, od, st);
+      case 256: return ragged_impl<true, Fwd256<true>>(r, qd, od, st);
+      default: return ragged_impl<true, Fwd512<true>>(r, qd, od, st);
+    }
+  }
+  switch (r.D) {
+    case 64: return ragged_impl<false, Fwd64<false>>(r, qd, od, st);
+    case 128: return ragged_impl<false, Fwd128<false>>(r, qd, od, st);
+    case 256: return ragged_impl<false, Fwd256<false>>(r, qd, od, st);
+    default: return ragged_impl<false, Fwd512<false>>(r, qd, od, st);
+  }
+}
+
+}  // namespace gqafa
 
 extern "C" int gqafa_fwd(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
                          const void* v, const long long* v_strides, void* o, const long long* o_strides,

@@ -69,8 +69,8 @@ int check_rows(const char* name, const void* ptr, const long long* st, int B, in
   const int size[3] = {B, H, N};
   for (int i = 0; i < 3; ++i) {
     out[i] = size[i] == 1 ? 0 : st[i];
-    if (out[i] < 0 || out[i] % 8 != 0)
-      return fail(GQAFA_ERR_INVALID, "%s: strides must be multiples of 8 elements (16 bytes), got (%lld, %lld, %lld, %lld)",
+    if ((size[i] > 1 && out[i] <= 0) || out[i] % 8 != 0)
+      return fail(GQAFA_ERR_INVALID, "%s: strides must be positive multiples of 8 elements (16 bytes), got (%lld, %lld, %lld, %lld)",
                   name, st[0], st[1], st[2], st[3]);
   }
   return GQAFA_OK;
@@ -98,7 +98,22 @@ struct AttendShape {
   int B, Hq, Hkv, N, D, G;
   int row_tiles, ctas, join_blocks;
   long long units;
+  // Dense path (0 requests: not taken): rows of K and V, requests at a time.
+  int dense_rows, dense_batch;
 };
+
+// Bytes of K and V in 16 bits that the dense path holds at a time; it goes over
+// the batch in groups of requests beyond that (one at least).
+constexpr long long kDenseBytes = 2LL << 30;
+
+// Many query rows per KV head are bound by the products, not by the cache: then
+// the keys and values are written out in 16 bits once (exactly) and the tcgen05
+// forward of dense caches runs over them, with the lengths of each request.
+// Its tiles hold 128 tokens of one query head; the MMAs above take 8 rows of
+// all heads of a group.
+bool dense_path(int G, int N) {
+  return static_cast<long long>(G) * N > 23LL * G * ((N + 127) / 128) + 40;
+}
 
 // Units of 8 query rows, and the CTAs of the launch: two per SM, fewer where there
 // are fewer tiles.
@@ -120,12 +135,21 @@ AttendShape attend_shape(int B, int Hq, int Hkv, int N, int D, int max_len, int 
   s.ctas = static_cast<int>(std::min<long long>(2LL * sms, s.units * tiles));
   // the join: at most two CTAs per SM, all of them where few units are cut into many parts
   s.join_blocks = 1;
+  if (dense_path(s.G, N)) {
+    long long held = max_len;
+    if (window > 0) held = std::min<long long>(held, static_cast<long long>(window) + N + 15);
+    s.dense_rows = static_cast<int>((std::max<long long>(held, 1) + 15) / 16 * 16);
+    s.dense_batch = static_cast<int>(
+        std::min<long long>(B, std::max<long long>(1, kDenseBytes / (4LL * Hkv * s.dense_rows * D))));
+  }
   while (s.join_blocks < 8 * D / 128 && s.join_blocks * s.units <= sms) s.join_blocks *= 2;
   return s;
 }
 
-// Parts [2 * ctas][8][D] fp32, their maxima and sums [2 * ctas][8].
+// Dense path: K and V [dense_batch][Hkv][dense_rows][D] 16-bit. Else parts
+// [2 * ctas][8][D] fp32, their maxima and sums [2 * ctas][8].
 long long attend_workspace(const AttendShape& s) {
+  if (s.dense_batch) return 4LL * s.dense_batch * s.Hkv * s.dense_rows * s.D + 256;
   return 2LL * s.ctas * 8 * (static_cast<long long>(s.D) * 4 + 8) + 256;
 }
 
@@ -170,6 +194,31 @@ int attend_dim(int D, const Kv4Params& p, cudaStream_t st) {
     case 256: return launch_attend<Kv4Cfg<256, BF16>>(p, st);
     default: return launch_attend<Kv4Cfg<512, BF16>>(p, st);
   }
+}
+
+template <bool RAGGED>
+int launch_read(Kv4ReadParams p, int head_dim, bool bf16, cudaStream_t st) {
+  const int NG = head_dim / KV4_GROUP;
+  // n tokens from any start touch at most (n + 15 + 15) / 16 blocks
+  const long long items = ((p.n + 30LL) / 16) * NG;
+  const long long xblocks = (items + 7) / 8, blocks = xblocks * p.B * p.Hkv;
+  if (blocks > INT_MAX) return fail(GQAFA_ERR_INVALID, "grid size %lld out of range", blocks);
+  p.xblocks = static_cast<int>(xblocks);
+  const dim3 grid(static_cast<unsigned>(blocks), 2);
+#define GQAFA_LAUNCH(DIM)                                         \
+  if (bf16)                                                       \
+    kv4_read_kernel<DIM, true, RAGGED><<<grid, 256, 0, st>>>(p);  \
+  else                                                            \
+    kv4_read_kernel<DIM, false, RAGGED><<<grid, 256, 0, st>>>(p); \
+  break
+  switch (head_dim) {
+    case 64: GQAFA_LAUNCH(64);
+    case 128: GQAFA_LAUNCH(128);
+    case 256: GQAFA_LAUNCH(256);
+    default: GQAFA_LAUNCH(512);
+  }
+#undef GQAFA_LAUNCH
+  return launch_status("read");
 }
 
 int check_attend(int batch, int heads_q, int heads_kv, int seqlen_q, int head_dim, int page_size, int dtype) {
@@ -327,28 +376,7 @@ extern "C" int gqafa_kv4_read(const void* pages, long long num_pages, const int*
   p.num_pages = static_cast<int>(num_pages);
   p.status = status_ptr();
   if (!p.status) return fail(GQAFA_ERR_CUDA, "cannot resolve the device status word");
-  const int NG = head_dim / KV4_GROUP;
-  // n tokens from any start touch at most (n + 15 + 15) / 16 blocks
-  const long long items = ((seqlen + 30LL) / 16) * NG;
-  const long long xblocks = (items + 7) / 8, blocks = xblocks * batch * heads_kv;
-  if (blocks > INT_MAX) return fail(GQAFA_ERR_INVALID, "grid size %lld out of range", blocks);
-  p.xblocks = static_cast<int>(xblocks);
-  const dim3 grid(static_cast<unsigned>(blocks), 2);
-  const bool bf16 = dtype == GQAFA_DTYPE_BF16;
-#define GQAFA_LAUNCH(DIM)                                 \
-  if (bf16)                                               \
-    kv4_read_kernel<DIM, true><<<grid, 256, 0, st>>>(p);  \
-  else                                                    \
-    kv4_read_kernel<DIM, false><<<grid, 256, 0, st>>>(p); \
-  break
-  switch (head_dim) {
-    case 64: GQAFA_LAUNCH(64);
-    case 128: GQAFA_LAUNCH(128);
-    case 256: GQAFA_LAUNCH(256);
-    default: GQAFA_LAUNCH(512);
-  }
-#undef GQAFA_LAUNCH
-  return launch_status("read");
+  return launch_read<false>(p, head_dim, dtype == GQAFA_DTYPE_BF16, st);
 }
 
 extern "C" long long gqafa_kv4_attend_workspace_size(int batch, int heads_q, int heads_kv, int seqlen_q, int head_dim,
@@ -401,6 +429,57 @@ extern "C" int gqafa_kv4_attend(const void* q, const long long* q_strides, const
     return fail(GQAFA_ERR_INVALID, "workspace of %lld bytes needed, got %lld", need, workspace_bytes);
   if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
     return fail(GQAFA_ERR_INVALID, "workspace must be 256-byte aligned");
+  if (s.dense_batch) {
+    Kv4ReadParams rd{};
+    rd.pages = static_cast<const uint8_t*>(pages);
+    rd.Hkv = heads_kv;
+    rd.n = s.dense_rows;
+    rd.cols = cols;
+    rd.table_stride = table_stride;
+    rd.page_shift = log2_of(page_size);
+    rd.num_pages = static_cast<int>(num_pages);
+    rd.ragged = 1;
+    rd.q_rows = seqlen_q;
+    rd.window = win;
+    rd.status = status_ptr();
+    if (!rd.status) return fail(GQAFA_ERR_CUDA, "cannot resolve the device status word");
+    const bool bf16 = dtype == GQAFA_DTYPE_BF16;
+    for (int b = 0; b < batch; b += s.dense_batch) {
+      const int nb = std::min(s.dense_batch, batch - b);
+      uint16_t* k = static_cast<uint16_t*>(workspace);
+      uint16_t* v = k + static_cast<long long>(nb) * heads_kv * s.dense_rows * head_dim;
+      rd.B = nb;
+      rd.table = block_table + b * table_stride;
+      rd.kv_lens = kv_lens + b;
+      rd.q_lens = q_lens ? q_lens + b : nullptr;
+      rd.out[0] = k;
+      rd.out[1] = v;
+      if ((rc = launch_read<true>(rd, head_dim, bf16, st))) return rc;
+      RaggedForward f{};
+      f.q = static_cast<const uint16_t*>(q) + b * qs[0];
+      f.q_strides = q_strides;
+      f.k = k;
+      f.v = v;
+      f.o = static_cast<uint16_t*>(o) + b * os[0];
+      f.o_strides = o_strides;
+      f.lse = lse ? lse + static_cast<long long>(b) * heads_q * seqlen_q : nullptr;
+      f.kv_lens = rd.kv_lens;
+      f.q_lens = rd.q_lens;
+      f.B = nb;
+      f.Hq = heads_q;
+      f.Hkv = heads_kv;
+      f.N = seqlen_q;
+      f.Nk = s.dense_rows;
+      f.D = head_dim;
+      f.kv_cap = static_cast<int>(capacity);
+      f.causal = causal ? 1 : 0;
+      f.window = win;
+      f.scale = softmax_scale;
+      f.bf16 = bf16;
+      if ((rc = ragged_forward(f, st))) return rc;
+    }
+    return GQAFA_OK;
+  }
   Kv4Params p{};
   p.tops = kv4_tops(dtype == GQAFA_DTYPE_BF16);
   p.q = static_cast<const uint16_t*>(q);

@@ -2,8 +2,8 @@
 // slots and positions from the requests' lengths), the quantised write of new
 // tokens and the read back of cached ones. Formats: kv4_layout.cuh.
 #pragma once
+#include "attn_kernel.cuh"
 #include "kv4_layout.cuh"
-#include "ptx_sm100.cuh"
 
 namespace gqafa {
 
@@ -292,6 +292,10 @@ struct Kv4ReadParams {
   int B, Hkv, n, cols, page_shift, num_pages;
   int xblocks;  // CTAs per request and head
   int* status;
+  // For the ragged forward: the keys it reads (ragged_lens), and zeros only up
+  // to the end of its last key block.
+  int ragged, q_rows, window;
+  const int* q_lens;
 };
 
 // Eight values of a word as 16 bytes of 16-bit values, exactly s * (c - z).
@@ -313,7 +317,11 @@ __device__ __forceinline__ uint4 kv4_values(uint32_t codes, uint32_t meta) {
 // writes 16 tokens x 64 values: 128 contiguous bytes per token. blockIdx.x:
 // request, head and eight (block, group) pairs; blockIdx.y: keys / values. Rows
 // behind a request's last token become zeros.
-template <int D, bool BF16>
+//
+// For the ragged forward, whose MMAs also multiply masked keys' values by P = 0,
+// a token with a NaN among its values goes out with NaN keys and zero values:
+// rows that see it become NaN, the others stay clean.
+template <int D, bool BF16, bool RAGGED>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
   constexpr int NG = D / KV4_GROUP;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -326,11 +334,18 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
     if (threadIdx.x == 0) atomicCAS(p.status, 0, ST_KV4_LENGTH);
     len = capacity;
   }
-  const int start = p.starts ? max(p.starts[b], 0) : 0;
+  int start = p.starts ? max(p.starts[b], 0) : 0, n = p.n;
+  if constexpr (RAGGED) {
+    const RaggedLens r = ragged_lens(p.kv_lens, p.q_lens, b, capacity, p.q_rows, p.window);
+    start = r.start;
+    if (r.Nk > p.n && threadIdx.x == 0) atomicCAS(p.status, 0, ST_KV4_LENGTH);  // beyond the given bound
+    n = min(p.n, (r.Nk + 255) & ~255);
+  }
   const int item = (blockIdx.x - bh * p.xblocks) * 8 + warp;
   const int g = item % NG;
   const long long pos0 = (static_cast<long long>(start) / 16 + item / NG) * 16;  // first token of the block
-  if (pos0 >= static_cast<long long>(start) + p.n) return;
+  if (pos0 >= static_cast<long long>(start) + n) return;
+  uint32_t bad = 0;  // tokens with a NaN among their values
   uint4 codes = make_uint4(0, 0, 0, 0);
   uint32_t meta[4] = {0, 0, 0, 0};
   if (pos0 < len) {
@@ -357,13 +372,26 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
         meta[2] = w.y & 0xFFFFu;
         meta[3] = w.y >> 16;
       }
+      if constexpr (RAGGED) {
+        const uint8_t* vals = src + (kind == 0 ? (static_cast<long long>(p.Hkv) << blocks_shift) * kv4_block_bytes(D) : 0);
+        const uint16_t* w = reinterpret_cast<const uint16_t*>(vals + NG * KV4_CODE_BYTES);
+        for (int e = lane; e < NG * KV4_TOKENS; e += 32) {
+          const int at = e & 15, r = (at >> 2) * 2 + (at & 1) + ((at >> 1) & 1) * 8;  // inverse of kv4_value_meta
+          if ((__ldg(w + e) & 0xFFF0u) == KV4_META_NAN) bad |= 1u << r;
+        }
+        bad = __reduce_or_sync(0xffffffffu, bad);
+      }
     }
   }
   uint16_t* out = p.out[kind] + (static_cast<long long>(b) * p.Hkv + h) * p.n * D + g * KV4_GROUP;
   auto store = [&](int r, int j, uint32_t c, uint32_t m) {
     const long long i = pos0 + r - start;
-    if (i < 0 || i >= p.n) return;
-    const uint4 v = (pos0 + r < len) ? kv4_values<BF16>(c, m) : make_uint4(0, 0, 0, 0);
+    if (i < 0 || i >= n) return;
+    uint4 v = (pos0 + r < len) ? kv4_values<BF16>(c, m) : make_uint4(0, 0, 0, 0);
+    if (RAGGED && pos0 + r < len && ((bad >> r) & 1u)) {
+      const uint32_t x = kind == 0 ? 0x7FFF7FFFu : 0u;
+      v = make_uint4(x, x, x, x);
+    }
     *reinterpret_cast<uint4*>(out + i * D + j * 8) = v;
   };
   if (kind == 0) {

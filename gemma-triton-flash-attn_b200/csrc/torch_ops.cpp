@@ -176,6 +176,12 @@ void check_rows(const at::Tensor& t, const char* name, const Pages& pg, const at
   TORCH_CHECK_VALUE(t.size(3) == pg.dim, "gqafa: ", name, " has head_dim ", t.size(3), ", the cache ", pg.dim);
   TORCH_CHECK_VALUE(t.numel() > 0, "gqafa: ", name, " is empty");
 }
+// As abi_ready, and a broadcast tensor (stride 0) becomes a whole one.
+at::Tensor rows_ready(const at::Tensor& t) {
+  bool ok = true;
+  for (int i = 0; i < 3; ++i) ok = ok && (t.stride(i) > 0 || t.size(i) == 1);
+  return abi_ready(ok ? t : t.contiguous());
+}
 int to_int(int64_t v, const char* name) {
   TORCH_CHECK_VALUE(v >= INT32_MIN && v <= INT32_MAX, "gqafa: ", name, " out of range: ", v);
   return static_cast<int>(v);
@@ -225,7 +231,7 @@ void kv4_append(at::Tensor pages, const at::Tensor& k_in, const at::Tensor& v_in
                     "gqafa: k and v must have shape (B, ", pg.heads, ", N, ", pg.dim, ")");
   TORCH_CHECK_TYPE(k_in.scalar_type() == v_in.scalar_type(), "gqafa: k and v must share a dtype");
   c10::cuda::CUDAGuard guard(dev);
-  const at::Tensor k = abi_ready(k_in), v = abi_ready(v_in);
+  const at::Tensor k = rows_ready(k_in), v = rows_ready(v_in);
   const int64_t B = k.size(0), N = k.size(2);
   const at::Tensor slots = rows_int32(slot_map, "slot_map", B, dev);
   TORCH_CHECK_VALUE(slots.size(1) == N, "gqafa: slot_map must have shape (", B, ", ", N, ")");
@@ -268,7 +274,7 @@ std::tuple<at::Tensor, at::Tensor> kv4_attend(const at::Tensor& q_in, const at::
   const Pages pg = check_pages(pages, page_size, dev);
   check_rows(q_in, "q", pg, dev);
   c10::cuda::CUDAGuard guard(dev);
-  const at::Tensor q = abi_ready(q_in);
+  const at::Tensor q = rows_ready(q_in);
   const int64_t B = q.size(0), Hq = q.size(1), N = q.size(2);
   const at::Tensor lens = vector_int32(kv_lens, "kv_lens", B, dev), table = rows_int32(block_table, "block_table", B, dev);
   at::Tensor rows;

@@ -240,3 +240,29 @@ def test_attention_over_a_long_ragged_batch(D, dtype):
     q = rand((5, 8, 2, D), 6, dtype, 2.0).to(DEV)
     check(q, cache, table, held, lens, [2, 1, 0, 2, 2], True, 0)
     check(q, cache, table, held, lens, None, True, 3000, scale=0.01)
+
+
+# ------------------------------------------------------------------ many rows: the dense path
+CHUNKS = [
+    # B, Hq, Hkv, N, lens, q_lens, page, causal, window
+    (1, 4, 1, 130, [130], None, 64, True, 0),                        # a prompt with nothing before it
+    (3, 8, 2, 200, [1000, 200, 300], [200, 77, 0], 16, True, 0),     # ragged, one request without rows
+    (2, 4, 4, 150, [0, 150], [150, 150], 32, True, 0),               # nothing cached: zeros
+    (2, 8, 4, 257, [2000, 600], [257, 129], 64, True, 300),          # window shorter than the cache
+    (2, 4, 2, 128, [1500, 700], None, 128, True, 1),                 # each row sees only itself
+    (2, 6, 2, 140, [600, 90], [140, 90], 64, False, 0),              # every row sees all keys
+    (2, 4, 1, 150, [100, 700], [150, 150], 64, True, 0),             # more rows than keys
+]
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("shape", CHUNKS, ids=lambda s: "B{}_H{}-{}_N{}_L{}_q{}_p{}_c{}_w{}".format(*s).replace(" ", ""))
+def test_chunks_within_the_rounding_bound(D, dtype, shape):
+    B, Hq, Hkv, N, lens, q_lens, page, causal, window = shape
+    cache, table, held = filled(B, Hkv, D, max(max(lens), 1), page, dtype, 31)
+    q = rand((B, N, Hq, D), 7, dtype).to(DEV).transpose(1, 2)
+    o, lse = check(q, cache, table, held, lens, q_lens, causal, window)
+    for b in range(B):
+        n = N if q_lens is None else q_lens[b]
+        assert (o[b, :, n:] == 0).all() and torch.isinf(lse[b, :, n:]).all()
