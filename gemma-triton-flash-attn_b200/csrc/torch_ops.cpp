@@ -12,6 +12,8 @@
 // the per-call Python marshalling of ~30 arguments and stride arrays. No CUDA
 // code is compiled here: every kernel lives in libgqa_fa_b200.so.
 #include <ATen/ATen.h>
+#include <ATen/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -182,6 +184,40 @@ at::Tensor rows_ready(const at::Tensor& t) {
   for (int i = 0; i < 3; ++i) ok = ok && (t.stride(i) > 0 || t.size(i) == 1);
   return abi_ready(ok ? t : t.contiguous());
 }
+// Outputs and scratch of these operators come from the caching allocator
+// directly: a step of a few microseconds on the GPU would otherwise wait for
+// the dispatcher's at::empty, 1.6 us a tensor (the plan has seven).
+at::Tensor new_tensor(at::IntArrayRef size, at::ScalarType type) {
+  return at::detail::empty_generic(size, c10::cuda::CUDACachingAllocator::get(),
+                                   c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt);
+}
+at::Tensor new_like(const at::Tensor& t) {  // with t's layout where it is dense (HF's (B, N, H, D) storage)
+  if (!t.is_non_overlapping_and_dense()) return new_tensor(t.sizes(), t.scalar_type());
+  return at::detail::empty_strided_generic(t.sizes(), t.strides(), c10::cuda::CUDACachingAllocator::get(),
+                                           c10::DispatchKeySet(c10::DispatchKey::CUDA), t.scalar_type());
+}
+// Contiguous int32 tensors cut from one allocation, each 16-byte aligned.
+class Int32Pack {
+ public:
+  explicit Int32Pack(int64_t ints) {
+    auto* alloc = c10::cuda::CUDACachingAllocator::get();
+    const size_t bytes = static_cast<size_t>(ints) * 4;
+    storage_ = c10::Storage(c10::Storage::use_byte_size_t(), bytes, alloc->allocate(bytes), alloc, false);
+  }
+  static int64_t room(int64_t n) { return (n + 3) / 4 * 4; }
+  at::Tensor cut(at::IntArrayRef size) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(
+        c10::Storage(storage_), c10::DispatchKeySet(c10::DispatchKey::CUDA), caffe2::TypeMeta::Make<int32_t>());
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(size);
+    t.unsafeGetTensorImpl()->set_storage_offset(at_);
+    at_ += room(t.numel());
+    return t;
+  }
+
+ private:
+  c10::Storage storage_;
+  int64_t at_ = 0;
+};
 int to_int(int64_t v, const char* name) {
   TORCH_CHECK_VALUE(v >= INT32_MIN && v <= INT32_MAX, "gqafa: ", name, " out of range: ", v);
   return static_cast<int>(v);
@@ -204,13 +240,9 @@ Plan kv4_plan(const at::Tensor& kv_lens, const at::Tensor& new_lens, const at::T
   TORCH_CHECK_VALUE(free_pages.dim() == 1 && free_pages.size(0) > 0 && free_pages.is_contiguous(),
                     "gqafa: free_pages must be a contiguous vector (it is written to)");
   const int64_t cols = table.size(1);
-  const auto opt = lens.options();
-  // one allocation for the small outputs, cut into views
-  at::Tensor small = at::empty({3 * B + 2}, opt);
-  at::Tensor out_table = at::empty({B, cols}, opt), slots = at::empty({B, max_new}, opt),
-             positions = at::empty({B, max_new}, opt);
-  at::Tensor out_lens = small.narrow(0, 0, B), out_new = small.narrow(0, B, B), accepted = small.narrow(0, 2 * B, B),
-             out_state = small.narrow(0, 3 * B, 2);
+  Int32Pack pack(Int32Pack::room(B * cols) + 2 * Int32Pack::room(B * max_new) + 3 * Int32Pack::room(B) + 4);
+  at::Tensor out_table = pack.cut({B, cols}), slots = pack.cut({B, max_new}), positions = pack.cut({B, max_new}),
+             out_lens = pack.cut({B}), out_new = pack.cut({B}), accepted = pack.cut({B}), out_state = pack.cut({2});
   check(gqafa_kv4_plan(lens.data_ptr<int>(), add.data_ptr<int>(), table.data_ptr<int>(), table.stride(0),
                        free_pages.data_ptr<int>(), state.data_ptr<int>(), to_int(B, "B"), to_int(cols, "columns"),
                        to_int(free_pages.size(0), "free_pages"), to_int(page_size, "page_size"),
@@ -255,7 +287,7 @@ std::tuple<at::Tensor, at::Tensor> kv4_read(const at::Tensor& pages, const at::T
   const at::Tensor lens = vector_int32(kv_lens, "kv_lens", B, dev), table = rows_int32(block_table, "block_table", B, dev);
   at::Tensor from;
   if (starts.has_value() && starts->defined()) from = vector_int32(*starts, "starts", B, dev);
-  at::Tensor k = at::empty({B, pg.heads, n, pg.dim}, pages.options().dtype(dtype)), v = at::empty_like(k);
+  at::Tensor k = new_tensor({B, pg.heads, n, pg.dim}, dtype), v = new_tensor({B, pg.heads, n, pg.dim}, dtype);
   check(gqafa_kv4_read(pages.data_ptr(), pg.count, table.data_ptr<int>(), table.stride(0),
                        to_int(table.size(1), "columns"), lens.data_ptr<int>(),
                        from.defined() ? from.data_ptr<int>() : nullptr, k.data_ptr(), v.data_ptr(), to_int(B, "B"),
@@ -279,8 +311,8 @@ std::tuple<at::Tensor, at::Tensor> kv4_attend(const at::Tensor& q_in, const at::
   const at::Tensor lens = vector_int32(kv_lens, "kv_lens", B, dev), table = rows_int32(block_table, "block_table", B, dev);
   at::Tensor rows;
   if (q_lens.has_value() && q_lens->defined()) rows = vector_int32(*q_lens, "q_lens", B, dev);
-  at::Tensor o = abi_ready(at::empty_like(q));  // keeps q's layout
-  at::Tensor lse = at::empty({want_lse ? B : 0, Hq, N}, q.options().dtype(at::kFloat));
+  at::Tensor o = new_like(q);
+  at::Tensor lse = new_tensor({want_lse ? B : 0, Hq, N}, at::kFloat);
   const int b = to_int(B, "B"), hq = to_int(Hq, "H_Q"), hkv = to_int(pg.heads, "H_KV"), n = to_int(N, "N"),
             d = to_int(pg.dim, "head_dim"), win = to_int(causal ? window : 0, "window");
   const int64_t capacity = table.size(1) * page_size;
@@ -291,13 +323,13 @@ std::tuple<at::Tensor, at::Tensor> kv4_attend(const at::Tensor& q_in, const at::
     TORCH_CHECK_NOT_IMPLEMENTED(d == 64 || d == 128 || d == 256 || d == 512, msg);
     TORCH_CHECK_VALUE(false, msg);
   }
-  at::Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
   const Strides sq(q), so(o);
   check(gqafa_kv4_attend(q.data_ptr(), sq.s, pages.data_ptr(), pg.count, table.data_ptr<int>(), table.stride(0),
                          to_int(table.size(1), "columns"), lens.data_ptr<int>(),
                          rows.defined() ? rows.data_ptr<int>() : nullptr, o.data_ptr(), so.s,
                          want_lse ? lse.data_ptr<float>() : nullptr, b, hq, hkv, n, d, to_int(page_size, "page_size"),
-                         longest, (float)scale, causal ? 1 : 0, win, dtype_code(q), ws.data_ptr(), bytes,
+                         longest, (float)scale, causal ? 1 : 0, win, dtype_code(q), ws.get(), bytes,
                          c10::cuda::getCurrentCUDAStream(dev.index()).stream()));
   return {o, lse};
 }
