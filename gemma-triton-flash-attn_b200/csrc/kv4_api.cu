@@ -201,7 +201,7 @@ int launch_read(Kv4ReadParams p, int head_dim, bool bf16, cudaStream_t st) {
   const int NG = head_dim / KV4_GROUP;
   // n tokens from any start touch at most (n + 15 + 15) / 16 blocks
   const long long items = ((p.n + 30LL) / 16) * NG;
-  const long long xblocks = (items + 7) / 8, blocks = xblocks * p.B * p.Hkv;
+  const long long xblocks = (items + 8 * KV4_READ_UNITS - 1) / (8 * KV4_READ_UNITS), blocks = xblocks * p.B * p.Hkv;
   if (blocks > INT_MAX) return fail(GQAFA_ERR_INVALID, "grid size %lld out of range", blocks);
   p.xblocks = static_cast<int>(xblocks);
   const dim3 grid(static_cast<unsigned>(blocks), 2);
@@ -325,7 +325,8 @@ extern "C" int gqafa_kv4_append(const void* k, const long long* k_strides, const
   p.status = status_ptr();
   if (!p.status) return fail(GQAFA_ERR_CUDA, "cannot resolve the device status word");
   const long long octets = static_cast<long long>(batch) * seqlen * heads_kv * (head_dim / KV4_GROUP);
-  const dim3 grid(static_cast<unsigned>(std::min<long long>((octets + 31) / 32, 1 << 20)), 2);
+  if (octets + 32 > INT_MAX) return fail(GQAFA_ERR_INVALID, "B * N * heads_kv * head_dim out of range");
+  const unsigned grid = static_cast<unsigned>((octets + 31) / 32);
   const bool bf16 = dtype == GQAFA_DTYPE_BF16;
 #define GQAFA_LAUNCH(DIM)                                   \
   if (bf16)                                                 \

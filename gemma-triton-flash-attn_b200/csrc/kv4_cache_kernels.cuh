@@ -155,37 +155,38 @@ __device__ __forceinline__ constexpr float kv4_max_finite() {
   return BF16 ? 3.3895313892515355e38f : 65504.f;
 }
 
-// Quantise the eight values of this lane's word of a group whose other words
-// are held by the octet's seven other lanes. Returns the codes (value i of the
-// word in nibble i) and the group's meta word.
+// Pairwise maximum of 16-bit values that keeps NaNs.
 template <bool BF16>
-__device__ __forceinline__ uint32_t kv4_quantise(const uint4 raw, uint32_t& meta) {
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (BF16)
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Quantise the eight values of this lane's word of a group whose other words
+// are held by the octet's seven other lanes: the word as the cache holds it
+// (keys or values) and the group's meta word.
+template <bool BF16>
+__device__ __forceinline__ uint32_t kv4_quantise(const uint4 raw, bool keys, uint32_t& meta) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  float x[8];
+  // largest x and largest -x, in the halves of one word
+  constexpr uint32_t SIGNS = 0x80008000u;
+  uint32_t up = max2_nan<BF16>(max2_nan<BF16>(w[0], w[1]), max2_nan<BF16>(w[2], w[3]));
+  uint32_t dn = max2_nan<BF16>(max2_nan<BF16>(w[0] ^ SIGNS, w[1] ^ SIGNS), max2_nan<BF16>(w[2] ^ SIGNS, w[3] ^ SIGNS));
+  uint32_t top = max2_nan<BF16>(__byte_perm(up, dn, 0x5410), __byte_perm(up, dn, 0x7632));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = unpack_lo<BF16>(w[i]);
-    x[2 * i + 1] = unpack_hi<BF16>(w[i]);
-  }
+  for (int o = 1; o < 8; o <<= 1) top = max2_nan<BF16>(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float most = kv4_max_finite<BF16>();
-  float hi = 0.f, lo = 0.f;
-  bool odd = false;  // an infinity or a NaN
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    hi = fmaxf(hi, x[i]);
-    lo = fminf(lo, x[i]);
-    odd |= !(fabsf(x[i]) <= most);
-  }
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-  }
-  const uint32_t odd_lanes = __ballot_sync(0xffffffffu, odd);
-  if ((odd_lanes >> (threadIdx.x & 24)) & 0xffu) {
+  float hi = unpack_lo<BF16>(top), lo = -unpack_hi<BF16>(top);
+  if (!(hi <= most && lo >= -most && lo <= most && hi >= -most)) {  // an infinity or a NaN in the group
     meta = KV4_META_NAN;
     return 0;
   }
+  hi = fmaxf(hi, 0.f);
+  lo = fminf(lo, 0.f);
   // up to 4 significant bits: clear the 20 low mantissa bits, rounding up
   const float step = __fdiv_rn(hi * 0.5f - lo * 0.5f, 7.5f);
   const float s = fmaxf(__uint_as_float((__float_as_uint(step) + 0xFFFFFu) & ~0xFFFFFu),
@@ -196,34 +197,32 @@ __device__ __forceinline__ uint32_t kv4_quantise(const uint4 raw, uint32_t& meta
   // by less than 2^-19, so a bias of 2^-17 decides every case rightly. Adding
   // 1.5 * 2^23 then rounds to the nearest integer in the low mantissa bits.
   constexpr float EPS = 7.62939453125e-6f, MAGIC = 12582912.f;
-  const float zr = fmaf(-lo, inv, EPS) + MAGIC;
-  const uint32_t z = __float_as_uint(zr) & 15u;
-  const float zb = static_cast<float>(z) + EPS;
+  const uint32_t z = __float_as_uint(fmaf(-lo, inv, EPS) + MAGIC) & 15u;
+  const float zf = static_cast<float>(z), zb = zf + EPS;
   meta = (__float_as_uint(s) >> 16) | z;
-  const bool far = fmaxf(hi, -lo) > most - s;  // a code may pass the largest number
-  uint32_t codes = 0;
+  uint32_t c[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float y = fminf(fmaf(x[i], inv, zb) + MAGIC, MAGIC + 15.f);
-    if (far) {
-      const float v = s * (y - MAGIC - static_cast<float>(z));
-      y += (v > most) ? -1.f : (v < -most) ? 1.f : 0.f;
-    }
-    codes |= (__float_as_uint(y) & 15u) << (4 * i);
+    const float x = (i & 1) ? unpack_hi<BF16>(w[i >> 1]) : unpack_lo<BF16>(w[i >> 1]);
+    c[i] = __float_as_uint(fminf(fmaf(x, inv, zb) + MAGIC, MAGIC + 15.f));
   }
-  return codes;
+  if (fmaxf(hi, -lo) > most - s) {  // a code may pass the largest number
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float y = __uint_as_float(c[i]), v = s * (y - MAGIC - zf);
+      c[i] = __float_as_uint(y + ((v > most) ? -1.f : (v < -most) ? 1.f : 0.f));
+    }
+  }
+  // codes are the low bytes of c: nibbles 0, 2, 4, 6 and 1, 3, 5, 7 of the word
+  auto bytes = [](uint32_t a, uint32_t b, uint32_t d, uint32_t e) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(d, e, 0x0040), 0x5410);
+  };
+  const uint32_t even = keys ? bytes(c[0], c[4], c[1], c[5]) : bytes(c[0], c[2], c[4], c[6]);
+  const uint32_t odd = keys ? bytes(c[2], c[6], c[3], c[7]) : bytes(c[1], c[3], c[5], c[7]);
+  return (even & 0x0F0F0F0Fu) | ((odd & 0x0F0F0F0Fu) << 4);
 }
 
-// Value order -> key word order (nibble i: dim 2i, nibble 4+i: dim 2i+1).
-__device__ __forceinline__ uint32_t kv4_key_nibbles(uint32_t c) {
-  // two 4-step perfect-unshuffle moves of nibbles inside the word
-  uint32_t t = (c ^ (c >> 4)) & 0x00F000F0u;
-  c ^= t ^ (t << 4);
-  t = (c ^ (c >> 8)) & 0x0000FF00u;
-  c ^= t ^ (t << 8);
-  return c;
-}
-// Inverse of kv4_key_nibbles.
+// Key word order (nibble i: dim 2i, nibble 4+i: dim 2i+1) -> value order.
 __device__ __forceinline__ uint32_t kv4_key_values(uint32_t c) {
   uint32_t t = (c ^ (c >> 8)) & 0x0000FF00u;
   c ^= t ^ (t << 8);
@@ -232,52 +231,51 @@ __device__ __forceinline__ uint32_t kv4_key_values(uint32_t c) {
   return c;
 }
 
-// Eight lanes (an octet) hold one group, 16 bytes of input each: the group's
-// extremes are a shuffle reduction, and nothing else is shared. blockIdx.y: 0
-// keys, 1 values.
+// Eight lanes (an octet) hold one group of a token, 16 bytes of keys and 16 of
+// values each: the group's extremes are a shuffle reduction over packed pairs,
+// and nothing else is shared. The rows are loaded beside the slot, not behind it.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p) {
   constexpr int NG = D / KV4_GROUP;
-  const int kind = blockIdx.y;
   const int j = threadIdx.x & 7;
-  const long long octets = static_cast<long long>(p.B) * p.N * p.Hkv * NG;
-  const long long stride = static_cast<long long>(gridDim.x) * 32;
   const int blocks_shift = p.page_shift - 4;
-  // every lane of a warp runs the same number of rounds: the shuffles need all
-  for (long long first = (static_cast<long long>(blockIdx.x) * 256 + (threadIdx.x & ~31)) >> 3; first < octets;
-       first += stride) {
-    const long long o = first + ((threadIdx.x & 31) >> 3);
-    const bool live = o < octets;
-    const int g = static_cast<int>(o % NG);
-    long long rest = o / NG;
-    const int h = static_cast<int>(rest % p.Hkv);
-    rest /= p.Hkv;
-    const int n = static_cast<int>(rest % p.N);
-    const int b = static_cast<int>(rest / p.N);
-    long long slot = -1;
-    if (live) slot = p.slots[b * p.slots_stride + n];
-    if (slot >= p.num_slots || slot < -1) {
-      if (j == 0) atomicCAS(p.status, 0, ST_KV4_SLOT);
-      slot = -1;
-    }
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (slot >= 0)
-      raw = *reinterpret_cast<const uint4*>(p.x[kind] + b * p.sb[kind] + h * p.sh[kind] + n * p.sn[kind] +
-                                            g * KV4_GROUP + j * 8);
+  const unsigned octet = blockIdx.x * 32u + (threadIdx.x >> 3);  // group of a head of a token
+  const int g = octet % NG;
+  const unsigned row = octet / NG, token = row / p.Hkv;
+  const int h = row - token * p.Hkv;
+  const unsigned b = token / p.N;
+  const int n = token - b * p.N;
+  const bool live = b < static_cast<unsigned>(p.B);  // the shuffles need all lanes
+  uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  long long slot = -1;
+  if (live) {
+    slot = p.slots[b * p.slots_stride + n];
+#pragma unroll
+    for (int kind = 0; kind < 2; ++kind)
+      raw[kind] = __ldcs(reinterpret_cast<const uint4*>(p.x[kind] + b * p.sb[kind] + h * p.sh[kind] + n * p.sn[kind] +
+                                                        g * KV4_GROUP + j * 8));
+  }
+  if (slot >= p.num_slots || slot < -1) {
+    if (j == 0) atomicCAS(p.status, 0, ST_KV4_SLOT);
+    slot = -1;
+  }
+  const int r = static_cast<int>(slot & 15);
+  const int blk = static_cast<int>(slot >> 4) & ((1 << blocks_shift) - 1);
+  uint8_t* page = p.pages + (((slot >> p.page_shift) * 2 * p.Hkv + h) << blocks_shift) * kv4_block_bytes(D) +
+                  blk * kv4_block_bytes(D);
+#pragma unroll
+  for (int kind = 0; kind < 2; ++kind) {
     uint32_t meta;
-    uint32_t codes = kv4_quantise<BF16>(raw, meta);
-    if (slot < 0) continue;
-    const int r = static_cast<int>(slot & 15);
-    const long long page = slot >> p.page_shift;
-    const int blk = static_cast<int>(slot >> 4) & ((1 << blocks_shift) - 1);
-    uint8_t* dst = p.pages + ((((page * 2 + kind) * p.Hkv + h) << blocks_shift) + blk) * kv4_block_bytes(D);
-    if (kind == 0) codes = kv4_key_nibbles(codes);
-    *reinterpret_cast<uint32_t*>(dst + g * KV4_CODE_BYTES + (kind == 0 ? kv4_key_word(r, j) : kv4_value_word(r, j))) =
-        codes;
-    if (j == 0)
-      reinterpret_cast<uint16_t*>(dst + NG * KV4_CODE_BYTES + g * KV4_META_BYTES)[kind == 0 ? kv4_key_meta(r)
-                                                                                           : kv4_value_meta(r)] =
-          static_cast<uint16_t>(meta);
+    const uint32_t codes = kv4_quantise<BF16>(raw[kind], kind == 0, meta);
+    if (slot >= 0) {
+      uint8_t* dst = page + (kind == 0 ? 0 : (static_cast<long long>(p.Hkv) << blocks_shift) * kv4_block_bytes(D));
+      *reinterpret_cast<uint32_t*>(dst + g * KV4_CODE_BYTES + (kind == 0 ? kv4_key_word(r, j) : kv4_value_word(r, j))) =
+          codes;
+      if (j == 0)
+        reinterpret_cast<uint16_t*>(dst + NG * KV4_CODE_BYTES + g * KV4_META_BYTES)[kind == 0 ? kv4_key_meta(r)
+                                                                                             : kv4_value_meta(r)] =
+            static_cast<uint16_t>(meta);
+    }
   }
 }
 
@@ -298,6 +296,8 @@ struct Kv4ReadParams {
   const int* q_lens;
 };
 
+constexpr int KV4_READ_UNITS = 4;  // groups of a block a warp reads
+
 // Eight values of a word as 16 bytes of 16-bit values, exactly s * (c - z).
 template <bool BF16>
 __device__ __forceinline__ uint4 kv4_values(uint32_t codes, uint32_t meta) {
@@ -313,10 +313,11 @@ __device__ __forceinline__ uint4 kv4_values(uint32_t codes, uint32_t meta) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A warp reads one group's codes of one block (16 bytes a lane, as stored) and
-// writes 16 tokens x 64 values: 128 contiguous bytes per token. blockIdx.x:
-// request, head and eight (block, group) pairs; blockIdx.y: keys / values. Rows
-// behind a request's last token become zeros.
+// A warp reads UNITS consecutive groups of 16-token blocks (16 bytes a lane and
+// group, as stored; all loads in flight together) and writes 16 tokens x 64
+// values of each: 128 contiguous bytes per token. blockIdx.x: request, head and
+// 8 * UNITS (block, group) pairs; blockIdx.y: keys / values. Rows behind a
+// request's last token become zeros.
 //
 // For the ragged forward, whose MMAs also multiply masked keys' values by P = 0,
 // a token with a NaN among its values goes out with NaN keys and zero values:
@@ -341,71 +342,75 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
     if (r.Nk > p.n && threadIdx.x == 0) atomicCAS(p.status, 0, ST_KV4_LENGTH);  // beyond the given bound
     n = min(p.n, (r.Nk + 255) & ~255);
   }
-  const int item = (blockIdx.x - bh * p.xblocks) * 8 + warp;
-  const int g = item % NG;
-  const long long pos0 = (static_cast<long long>(start) / 16 + item / NG) * 16;  // first token of the block
-  if (pos0 >= static_cast<long long>(start) + n) return;
-  uint32_t bad = 0;  // tokens with a NaN among their values
-  uint4 codes = make_uint4(0, 0, 0, 0);
-  uint32_t meta[4] = {0, 0, 0, 0};
-  if (pos0 < len) {
+  const int item0 = ((blockIdx.x - bh * p.xblocks) * 8 + warp) * KV4_READ_UNITS;
+  const int blocks_shift = p.page_shift - 4;
+  const long long end = static_cast<long long>(start) + n;
+  uint4 codes[KV4_READ_UNITS];
+  uint2 metas[KV4_READ_UNITS];
+  uint32_t bad[KV4_READ_UNITS];  // tokens with a NaN among their values
+#pragma unroll
+  for (int k = 0; k < KV4_READ_UNITS; ++k) {
+    const int g = (item0 + k) % NG;
+    const long long pos0 = (static_cast<long long>(start) / 16 + (item0 + k) / NG) * 16;  // first token of the block
+    codes[k] = make_uint4(0, 0, 0, 0);
+    metas[k] = make_uint2(0, 0);
+    bad[k] = 0;
+    if (pos0 >= len || pos0 >= end) continue;
     const int blk = static_cast<int>(pos0 >> 4);
-    const int blocks_shift = p.page_shift - 4;
-    int page = p.table[b * p.table_stride + (blk >> blocks_shift)];
+    const int page = __ldg(p.table + b * p.table_stride + (blk >> blocks_shift));
     if (page < 0 || page >= p.num_pages) {
       if (lane == 0) atomicCAS(p.status, 0, ST_KV4_PAGE);
-      len = 0;
-    } else {
-      const uint8_t* src = p.pages + ((((static_cast<long long>(page) * 2 + kind) * p.Hkv + h) << blocks_shift) +
-                                      (blk & ((1 << blocks_shift) - 1))) *
-                                         kv4_block_bytes(D);
-      codes = __ldg(reinterpret_cast<const uint4*>(src + g * KV4_CODE_BYTES + lane * 16));
-      const uint8_t* m = src + NG * KV4_CODE_BYTES + g * KV4_META_BYTES;
-      if (kind == 0) {
-        const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(m + (lane >> 2) * 4));
-        meta[0] = w & 0xFFFFu;
-        meta[1] = w >> 16;
-      } else {
-        const uint2 w = __ldg(reinterpret_cast<const uint2*>(m + (lane >> 3) * 8));
-        meta[0] = w.x & 0xFFFFu;
-        meta[1] = w.x >> 16;
-        meta[2] = w.y & 0xFFFFu;
-        meta[3] = w.y >> 16;
+      continue;
+    }
+    const uint8_t* src = p.pages + ((((static_cast<long long>(page) * 2 + kind) * p.Hkv + h) << blocks_shift) +
+                                    (blk & ((1 << blocks_shift) - 1))) *
+                                       kv4_block_bytes(D);
+    codes[k] = __ldg(reinterpret_cast<const uint4*>(src + g * KV4_CODE_BYTES + lane * 16));
+    const uint8_t* m = src + NG * KV4_CODE_BYTES + g * KV4_META_BYTES;
+    if (kind == 0)
+      metas[k].x = __ldg(reinterpret_cast<const uint32_t*>(m + (lane >> 2) * 4));
+    else
+      metas[k] = __ldg(reinterpret_cast<const uint2*>(m + (lane >> 3) * 8));
+    if constexpr (RAGGED) {
+      const uint8_t* vals = src + (kind == 0 ? (static_cast<long long>(p.Hkv) << blocks_shift) * kv4_block_bytes(D) : 0);
+      const uint16_t* w = reinterpret_cast<const uint16_t*>(vals + NG * KV4_CODE_BYTES);
+      for (int e = lane; e < NG * KV4_TOKENS; e += 32) {
+        const int at = e & 15, r = (at >> 2) * 2 + (at & 1) + ((at >> 1) & 1) * 8;  // inverse of kv4_value_meta
+        if ((__ldg(w + e) & 0xFFF0u) == KV4_META_NAN) bad[k] |= 1u << r;
       }
-      if constexpr (RAGGED) {
-        const uint8_t* vals = src + (kind == 0 ? (static_cast<long long>(p.Hkv) << blocks_shift) * kv4_block_bytes(D) : 0);
-        const uint16_t* w = reinterpret_cast<const uint16_t*>(vals + NG * KV4_CODE_BYTES);
-        for (int e = lane; e < NG * KV4_TOKENS; e += 32) {
-          const int at = e & 15, r = (at >> 2) * 2 + (at & 1) + ((at >> 1) & 1) * 8;  // inverse of kv4_value_meta
-          if ((__ldg(w + e) & 0xFFF0u) == KV4_META_NAN) bad |= 1u << r;
-        }
-        bad = __reduce_or_sync(0xffffffffu, bad);
-      }
+      bad[k] = __reduce_or_sync(0xffffffffu, bad[k]);
     }
   }
-  uint16_t* out = p.out[kind] + (static_cast<long long>(b) * p.Hkv + h) * p.n * D + g * KV4_GROUP;
-  auto store = [&](int r, int j, uint32_t c, uint32_t m) {
-    const long long i = pos0 + r - start;
-    if (i < 0 || i >= n) return;
-    uint4 v = (pos0 + r < len) ? kv4_values<BF16>(c, m) : make_uint4(0, 0, 0, 0);
-    if (RAGGED && pos0 + r < len && ((bad >> r) & 1u)) {
-      const uint32_t x = kind == 0 ? 0x7FFF7FFFu : 0u;
-      v = make_uint4(x, x, x, x);
+#pragma unroll
+  for (int k = 0; k < KV4_READ_UNITS; ++k) {
+    const int g = (item0 + k) % NG;
+    const long long pos0 = (static_cast<long long>(start) / 16 + (item0 + k) / NG) * 16;
+    if (pos0 >= end) return;
+    uint16_t* out = p.out[kind] + (static_cast<long long>(b) * p.Hkv + h) * p.n * D + g * KV4_GROUP;
+    auto store = [&](int r, int j, uint32_t c, uint32_t m) {
+      const long long i = pos0 + r - start;
+      if (i < 0 || i >= n) return;
+      uint4 v = (pos0 + r < len) ? kv4_values<BF16>(c, m) : make_uint4(0, 0, 0, 0);
+      if (RAGGED && pos0 + r < len && ((bad[k] >> r) & 1u)) {
+        const uint32_t x = kind == 0 ? 0x7FFF7FFFu : 0u;
+        v = make_uint4(x, x, x, x);
+      }
+      *reinterpret_cast<uint4*>(out + i * D + j * 8) = v;
+    };
+    const uint2 m = metas[k];
+    if (kind == 0) {
+      const int r = lane >> 2, t = lane & 3;
+      store(r, 2 * t, kv4_key_values(codes[k].x), m.x & 0xFFFFu);
+      store(r, 2 * t + 1, kv4_key_values(codes[k].y), m.x & 0xFFFFu);
+      store(r + 8, 2 * t, kv4_key_values(codes[k].z), m.x >> 16);
+      store(r + 8, 2 * t + 1, kv4_key_values(codes[k].w), m.x >> 16);
+    } else {
+      const int t = lane >> 3, j = (lane & 7) ^ (2 * t);
+      store(2 * t, j, codes[k].x, m.x & 0xFFFFu);
+      store(2 * t + 1, j, codes[k].y, m.x >> 16);
+      store(2 * t + 8, j, codes[k].z, m.y & 0xFFFFu);
+      store(2 * t + 9, j, codes[k].w, m.y >> 16);
     }
-    *reinterpret_cast<uint4*>(out + i * D + j * 8) = v;
-  };
-  if (kind == 0) {
-    const int r = lane >> 2, t = lane & 3;
-    store(r, 2 * t, kv4_key_values(codes.x), meta[0]);
-    store(r, 2 * t + 1, kv4_key_values(codes.y), meta[0]);
-    store(r + 8, 2 * t, kv4_key_values(codes.z), meta[1]);
-    store(r + 8, 2 * t + 1, kv4_key_values(codes.w), meta[1]);
-  } else {
-    const int t = lane >> 3, j = (lane & 7) ^ (2 * t);
-    store(2 * t, j, codes.x, meta[0]);
-    store(2 * t + 1, j, codes.y, meta[1]);
-    store(2 * t + 8, j, codes.z, meta[2]);
-    store(2 * t + 9, j, codes.w, meta[3]);
   }
 }
 
