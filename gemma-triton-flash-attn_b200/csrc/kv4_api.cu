@@ -321,18 +321,24 @@ extern "C" int gqafa_kv4_append(const void* k, const long long* k_strides, const
   p.N = seqlen;
   p.Hkv = heads_kv;
   p.page_shift = log2_of(page_size);
-  p.num_slots = num_pages * page_size;
+  p.num_slots = static_cast<int>(num_pages * page_size);
   p.status = status_ptr();
   if (!p.status) return fail(GQAFA_ERR_CUDA, "cannot resolve the device status word");
-  const long long octets = static_cast<long long>(batch) * seqlen * heads_kv * (head_dim / KV4_GROUP);
-  if (octets + 32 > INT_MAX) return fail(GQAFA_ERR_INVALID, "B * N * heads_kv * head_dim out of range");
-  const unsigned grid = static_cast<unsigned>((octets + 31) / 32);
+  const bool tiled = seqlen >= 16;
+  // tokens, or the 16-token tiles that can hold them from any first slot
+  const long long units = (tiled ? (seqlen + 30LL) / 16 * 16 : seqlen) * (head_dim / KV4_GROUP);
+  if (heads_kv > 65535 || batch > 65535 || (units + 63) / 64 > INT_MAX)
+    return fail(GQAFA_ERR_INVALID, "B (%d) and heads_kv (%d) must be at most 65535", batch, heads_kv);
+  const dim3 grid(static_cast<unsigned>((units + 63) / 64), heads_kv, batch);
   const bool bf16 = dtype == GQAFA_DTYPE_BF16;
-#define GQAFA_LAUNCH(DIM)                                   \
-  if (bf16)                                                 \
-    kv4_append_kernel<DIM, true><<<grid, 256, 0, st>>>(p);  \
-  else                                                      \
-    kv4_append_kernel<DIM, false><<<grid, 256, 0, st>>>(p); \
+#define GQAFA_LAUNCH(DIM)                                                                      \
+  if (tiled) {                                                                                 \
+    bf16 ? kv4_append_kernel<DIM, true, true><<<grid, 256, 0, st>>>(p)                         \
+         : kv4_append_kernel<DIM, false, true><<<grid, 256, 0, st>>>(p);                       \
+  } else {                                                                                     \
+    bf16 ? kv4_append_kernel<DIM, true, false><<<grid, 256, 0, st>>>(p)                        \
+         : kv4_append_kernel<DIM, false, false><<<grid, 256, 0, st>>>(p);                      \
+  }                                                                                            \
   break
   switch (head_dim) {
     case 64: GQAFA_LAUNCH(64);
@@ -357,8 +363,8 @@ extern "C" int gqafa_kv4_read(const void* pages, long long num_pages, const int*
   if (starts && (rc = check_ints("starts", starts))) return rc;
   void* out[2] = {k, v};
   for (int i = 0; i < 2; ++i)
-    if (out[i] == nullptr || reinterpret_cast<uintptr_t>(out[i]) % 16 != 0)
-      return fail(GQAFA_ERR_INVALID, "outputs must be 16-byte aligned");
+    if (out[i] == nullptr || reinterpret_cast<uintptr_t>(out[i]) % 32 != 0)
+      return fail(GQAFA_ERR_INVALID, "outputs must be 32-byte aligned");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if ((rc = bind_device(st))) return rc;
   Kv4ReadParams p{};

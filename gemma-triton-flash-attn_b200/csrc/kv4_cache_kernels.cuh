@@ -146,7 +146,7 @@ struct Kv4AppendParams {
   long long slots_stride;
   uint8_t* pages;
   int B, N, Hkv, page_shift;  // page_shift: log2 of the page's tokens
-  long long num_slots;
+  int num_slots;
   int* status;
 };
 
@@ -166,60 +166,76 @@ __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
   return r;
 }
 
-// Quantise the eight values of this lane's word of a group whose other words
-// are held by the octet's seven other lanes: the word as the cache holds it
-// (keys or values) and the group's meta word.
+// Quantise this lane's two words (16 values) of a group whose other words are
+// held by the quad's three other lanes: the words as the cache holds them (keys
+// or values) and the group's meta word.
 template <bool BF16>
-__device__ __forceinline__ uint32_t kv4_quantise(const uint4 raw, bool keys, uint32_t& meta) {
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+__device__ __forceinline__ uint2 kv4_quantise(const uint4 raw0, const uint4 raw1, bool keys, uint32_t& meta) {
+  const uint32_t w[8] = {raw0.x, raw0.y, raw0.z, raw0.w, raw1.x, raw1.y, raw1.z, raw1.w};
   // largest x and largest -x, in the halves of one word
   constexpr uint32_t SIGNS = 0x80008000u;
-  uint32_t up = max2_nan<BF16>(max2_nan<BF16>(w[0], w[1]), max2_nan<BF16>(w[2], w[3]));
-  uint32_t dn = max2_nan<BF16>(max2_nan<BF16>(w[0] ^ SIGNS, w[1] ^ SIGNS), max2_nan<BF16>(w[2] ^ SIGNS, w[3] ^ SIGNS));
+  uint32_t up = w[0], dn = w[0] ^ SIGNS;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    up = max2_nan<BF16>(up, w[i]);
+    dn = max2_nan<BF16>(dn, w[i] ^ SIGNS);
+  }
   uint32_t top = max2_nan<BF16>(__byte_perm(up, dn, 0x5410), __byte_perm(up, dn, 0x7632));
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) top = max2_nan<BF16>(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int o = 1; o < 4; o <<= 1) top = max2_nan<BF16>(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float most = kv4_max_finite<BF16>();
   float hi = unpack_lo<BF16>(top), lo = -unpack_hi<BF16>(top);
   if (!(hi <= most && lo >= -most && lo <= most && hi >= -most)) {  // an infinity or a NaN in the group
     meta = KV4_META_NAN;
-    return 0;
+    return make_uint2(0, 0);
   }
   hi = fmaxf(hi, 0.f);
   lo = fminf(lo, 0.f);
-  // up to 4 significant bits: clear the 20 low mantissa bits, rounding up
-  const float step = __fdiv_rn(hi * 0.5f - lo * 0.5f, 7.5f);
-  const float s = fmaxf(__uint_as_float((__float_as_uint(step) + 0xFFFFFu) & ~0xFFFFFu),
-                        BF16 ? 1.1754943508222875e-38f : 4.76837158203125e-7f);
-  const float inv = __frcp_rn(s);
+  // The smallest 4-bit number that is not below range / 7.5 (of half the
+  // values): from a product that is surely not above it, then one exact
+  // comparison. 20 low mantissa bits are cleared, rounding up.
+  const float range = hi * 0.5f - lo * 0.5f;
+  uint32_t sb = (__float_as_uint(range * 0.13333330f) + 0xFFFFFu) & ~0xFFFFFu;
+  if (__uint_as_float(sb) * 7.5f < range) sb += 0x100000u;
+  const float s = fmaxf(__uint_as_float(sb), BF16 ? 1.1754943508222875e-38f : 4.76837158203125e-7f);
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));  // s in [2^-126, 2^126): neither side is flushed
   // floor(x/s + 1/2) by x * (1/s): ties must go up. x/s is a tie or at least
   // 2^-14 away from one (x has at most 11 bits, s 4), and the product is off
-  // by less than 2^-19, so a bias of 2^-17 decides every case rightly. Adding
+  // by less than 2^-18, so a bias of 2^-17 decides every case rightly. Adding
   // 1.5 * 2^23 then rounds to the nearest integer in the low mantissa bits.
   constexpr float EPS = 7.62939453125e-6f, MAGIC = 12582912.f;
   const uint32_t z = __float_as_uint(fmaf(-lo, inv, EPS) + MAGIC) & 15u;
   const float zf = static_cast<float>(z), zb = zf + EPS;
   meta = (__float_as_uint(s) >> 16) | z;
-  uint32_t c[8];
+  const bool far = fmaxf(hi, -lo) > most - s;  // a code may pass the largest number
+  uint32_t word[2];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float x = (i & 1) ? unpack_hi<BF16>(w[i >> 1]) : unpack_lo<BF16>(w[i >> 1]);
-    c[i] = __float_as_uint(fminf(fmaf(x, inv, zb) + MAGIC, MAGIC + 15.f));
-  }
-  if (fmaxf(hi, -lo) > most - s) {  // a code may pass the largest number
+  for (int u = 0; u < 2; ++u) {
+    uint32_t c[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float y = __uint_as_float(c[i]), v = s * (y - MAGIC - zf);
-      c[i] = __float_as_uint(y + ((v > most) ? -1.f : (v < -most) ? 1.f : 0.f));
+      const uint32_t v = w[4 * u + (i >> 1)];
+      const float x = (i & 1) ? unpack_hi<BF16>(v) : unpack_lo<BF16>(v);
+      c[i] = __float_as_uint(fminf(fmaf(x, inv, zb) + MAGIC, MAGIC + 15.f));
     }
+    if (far) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float y = __uint_as_float(c[i]), v = s * (y - MAGIC - zf);
+        c[i] = __float_as_uint(y + ((v > most) ? -1.f : (v < -most) ? 1.f : 0.f));
+      }
+    }
+    // codes are the low bytes of c (0..15 each: the magic number's low byte is
+    // 0): nibbles 0, 2, 4, 6 and 1, 3, 5, 7 of the word
+    auto bytes = [](uint32_t a, uint32_t b, uint32_t d, uint32_t e) {
+      return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(d, e, 0x0040), 0x5410);
+    };
+    const uint32_t even = keys ? bytes(c[0], c[4], c[1], c[5]) : bytes(c[0], c[2], c[4], c[6]);
+    const uint32_t odd = keys ? bytes(c[2], c[6], c[3], c[7]) : bytes(c[1], c[3], c[5], c[7]);
+    word[u] = even | (odd << 4);
   }
-  // codes are the low bytes of c: nibbles 0, 2, 4, 6 and 1, 3, 5, 7 of the word
-  auto bytes = [](uint32_t a, uint32_t b, uint32_t d, uint32_t e) {
-    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(d, e, 0x0040), 0x5410);
-  };
-  const uint32_t even = keys ? bytes(c[0], c[4], c[1], c[5]) : bytes(c[0], c[2], c[4], c[6]);
-  const uint32_t odd = keys ? bytes(c[2], c[6], c[3], c[7]) : bytes(c[1], c[3], c[5], c[7]);
-  return (even & 0x0F0F0F0Fu) | ((odd & 0x0F0F0F0Fu) << 4);
+  return make_uint2(word[0], word[1]);
 }
 
 // Key word order (nibble i: dim 2i, nibble 4+i: dim 2i+1) -> value order.
@@ -231,47 +247,69 @@ __device__ __forceinline__ uint32_t kv4_key_values(uint32_t c) {
   return c;
 }
 
-// Eight lanes (an octet) hold one group of a token, 16 bytes of keys and 16 of
+// Four lanes (a quad) hold one group of a token, 32 bytes of keys and 32 of
 // values each: the group's extremes are a shuffle reduction over packed pairs,
-// and nothing else is shared. The rows are loaded beside the slot, not behind it.
-template <int D, bool BF16>
+// and nothing else is shared. The rows are loaded beside the slot, not behind
+// it. Bound by instructions (with eight lanes a group, the scale's arithmetic and
+// an index computed with divisions took 28 instructions a value, 65 us for 16384
+// tokens at head_dim 256). blockIdx: 64 (token, group) pairs, head, request.
+//
+// TILED (16 tokens or more): neighbouring quads take tokens whose slots end in
+// 2t, 2t+1, 2t+8, 2t+9 if the slots run on from the row's first one, so a warp's
+// stores fill whole sectors.
+template <int D, bool BF16, bool TILED>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p) {
   constexpr int NG = D / KV4_GROUP;
-  const int j = threadIdx.x & 7;
+  const int t = threadIdx.x & 3;
   const int blocks_shift = p.page_shift - 4;
-  const unsigned octet = blockIdx.x * 32u + (threadIdx.x >> 3);  // group of a head of a token
-  const int g = octet % NG;
-  const unsigned row = octet / NG, token = row / p.Hkv;
-  const int h = row - token * p.Hkv;
-  const unsigned b = token / p.N;
-  const int n = token - b * p.N;
-  const bool live = b < static_cast<unsigned>(p.B);  // the shuffles need all lanes
-  uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-  long long slot = -1;
-  if (live) {
+  const int h = blockIdx.y, b = blockIdx.z;
+  unsigned rest = blockIdx.x * 64u + (threadIdx.x >> 2);
+  int n = 0;
+  if constexpr (TILED) {
+    const unsigned q = rest & 3, pair = (rest >> 2) & 3;
+    n = static_cast<int>(2 * pair + (q & 1) + 8 * (q >> 1));
+    rest >>= 4;
+  }
+  const int g = rest % NG;
+  if constexpr (TILED) {
+    const int first = p.slots[b * p.slots_stride];
+    n += static_cast<int>(rest / NG) * 16 - (first >= 0 ? first & 15 : 0);
+  } else {
+    n = rest / NG;
+  }
+  uint4 raw[2][2] = {};
+  int slot = -1;
+  if (n >= 0 && n < p.N) {  // the shuffles need all lanes
     slot = p.slots[b * p.slots_stride + n];
 #pragma unroll
-    for (int kind = 0; kind < 2; ++kind)
-      raw[kind] = __ldcs(reinterpret_cast<const uint4*>(p.x[kind] + b * p.sb[kind] + h * p.sh[kind] + n * p.sn[kind] +
-                                                        g * KV4_GROUP + j * 8));
+    for (int kind = 0; kind < 2; ++kind) {
+      const uint4* src = reinterpret_cast<const uint4*>(p.x[kind] + b * p.sb[kind] + h * p.sh[kind] + n * p.sn[kind] +
+                                                        g * KV4_GROUP + t * 16);
+      raw[kind][0] = __ldcs(src);
+      raw[kind][1] = __ldcs(src + 1);
+    }
   }
   if (slot >= p.num_slots || slot < -1) {
-    if (j == 0) atomicCAS(p.status, 0, ST_KV4_SLOT);
+    if (t == 0) atomicCAS(p.status, 0, ST_KV4_SLOT);
     slot = -1;
   }
-  const int r = static_cast<int>(slot & 15);
-  const int blk = static_cast<int>(slot >> 4) & ((1 << blocks_shift) - 1);
-  uint8_t* page = p.pages + (((slot >> p.page_shift) * 2 * p.Hkv + h) << blocks_shift) * kv4_block_bytes(D) +
-                  blk * kv4_block_bytes(D);
+  const int r = slot & 15;
+  const int blk = (slot >> 4) & ((1 << blocks_shift) - 1);
+  uint8_t* page = p.pages + ((((static_cast<long long>(slot >> p.page_shift) * 2 * p.Hkv) + h) << blocks_shift) + blk) *
+                                kv4_block_bytes(D);
 #pragma unroll
   for (int kind = 0; kind < 2; ++kind) {
     uint32_t meta;
-    const uint32_t codes = kv4_quantise<BF16>(raw[kind], kind == 0, meta);
+    const uint2 codes = kv4_quantise<BF16>(raw[kind][0], raw[kind][1], kind == 0, meta);
     if (slot >= 0) {
       uint8_t* dst = page + (kind == 0 ? 0 : (static_cast<long long>(p.Hkv) << blocks_shift) * kv4_block_bytes(D));
-      *reinterpret_cast<uint32_t*>(dst + g * KV4_CODE_BYTES + (kind == 0 ? kv4_key_word(r, j) : kv4_value_word(r, j))) =
-          codes;
-      if (j == 0)
+      if (kind == 0) {
+        *reinterpret_cast<uint2*>(dst + g * KV4_CODE_BYTES + kv4_key_word(r, 2 * t)) = codes;
+      } else {
+        *reinterpret_cast<uint32_t*>(dst + g * KV4_CODE_BYTES + kv4_value_word(r, 2 * t)) = codes.x;
+        *reinterpret_cast<uint32_t*>(dst + g * KV4_CODE_BYTES + kv4_value_word(r, 2 * t + 1)) = codes.y;
+      }
+      if (t == 0)
         reinterpret_cast<uint16_t*>(dst + NG * KV4_CODE_BYTES + g * KV4_META_BYTES)[kind == 0 ? kv4_key_meta(r)
                                                                                              : kv4_value_meta(r)] =
             static_cast<uint16_t>(meta);
@@ -387,23 +425,32 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
     const long long pos0 = (static_cast<long long>(start) / 16 + (item0 + k) / NG) * 16;
     if (pos0 >= end) return;
     uint16_t* out = p.out[kind] + (static_cast<long long>(b) * p.Hkv + h) * p.n * D + g * KV4_GROUP;
+    auto value = [&](int r, uint32_t c, uint32_t m) {
+      if (pos0 + r >= len) return make_uint4(0, 0, 0, 0);
+      if (RAGGED && ((bad[k] >> r) & 1u)) {
+        const uint32_t x = kind == 0 ? 0x7FFF7FFFu : 0u;
+        return make_uint4(x, x, x, x);
+      }
+      return kv4_values<BF16>(c, m);
+    };
     auto store = [&](int r, int j, uint32_t c, uint32_t m) {
       const long long i = pos0 + r - start;
+      if (i >= 0 && i < n) *reinterpret_cast<uint4*>(out + i * D + j * 8) = value(r, c, m);
+    };
+    auto store_pair = [&](int r, int t, uint32_t c0, uint32_t c1, uint32_t m) {
+      const long long i = pos0 + r - start;
       if (i < 0 || i >= n) return;
-      uint4 v = (pos0 + r < len) ? kv4_values<BF16>(c, m) : make_uint4(0, 0, 0, 0);
-      if (RAGGED && pos0 + r < len && ((bad[k] >> r) & 1u)) {
-        const uint32_t x = kind == 0 ? 0x7FFF7FFFu : 0u;
-        v = make_uint4(x, x, x, x);
-      }
-      *reinterpret_cast<uint4*>(out + i * D + j * 8) = v;
+      const uint4 v = value(r, c0, m), w = value(r, c1, m);
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + i * D + t * 16), "r"(v.x),
+                   "r"(v.y), "r"(v.z), "r"(v.w), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                   : "memory");
     };
     const uint2 m = metas[k];
     if (kind == 0) {
+      // words 2t and 2t + 1 of a token in one 32-byte store: whole sectors
       const int r = lane >> 2, t = lane & 3;
-      store(r, 2 * t, kv4_key_values(codes[k].x), m.x & 0xFFFFu);
-      store(r, 2 * t + 1, kv4_key_values(codes[k].y), m.x & 0xFFFFu);
-      store(r + 8, 2 * t, kv4_key_values(codes[k].z), m.x >> 16);
-      store(r + 8, 2 * t + 1, kv4_key_values(codes[k].w), m.x >> 16);
+      store_pair(r, t, kv4_key_values(codes[k].x), kv4_key_values(codes[k].y), m.x & 0xFFFFu);
+      store_pair(r + 8, t, kv4_key_values(codes[k].z), kv4_key_values(codes[k].w), m.x >> 16);
     } else {
       const int t = lane >> 3, j = (lane & 7) ^ (2 * t);
       store(2 * t, j, codes[k].x, m.x & 0xFFFFu);

@@ -239,7 +239,7 @@ GQAFA_API int gqafa_kv4_append(const void* k, const long long* k_strides, const 
                                int heads_kv, int seqlen, int head_dim, int page_size, int dtype, void* stream);
 
 /* Cached keys and values as contiguous [batch, heads_kv, seqlen, head_dim]
- * tensors: row i of request b is position starts[b] + i (starts NULL: 0), zeros
+ * tensors (32-byte aligned): row i of request b is position starts[b] + i (starts NULL: 0), zeros
  * from kv_lens[b] on. */
 GQAFA_API int gqafa_kv4_read(const void* pages, long long num_pages, const int* block_table, long long table_stride,
                              int cols, const int* kv_lens, const int* starts, void* k, void* v, int batch,
