@@ -431,6 +431,8 @@ extern "C" int gqafa_kv4_attend(const void* q, const long long* q_strides, const
   const int sms = sm_count();
   if (sms <= 0) return fail(GQAFA_ERR_CUDA, "cannot read the device's multiprocessor count");
   const AttendShape s = attend_shape(batch, heads_q, heads_kv, seqlen_q, head_dim, max_kv_len, win, sms);
+  if (s.units * (capacity / 64 + 2) > INT_MAX)
+    return fail(GQAFA_ERR_INVALID, "B * H_Q * N times the block table's capacity out of range");
   const long long need = attend_workspace(s);
   if (workspace == nullptr || workspace_bytes < need)
     return fail(GQAFA_ERR_INVALID, "workspace of %lld bytes needed, got %lld", need, workspace_bytes);

@@ -81,10 +81,10 @@ struct Kv4Params {
   int cols, page_shift, num_pages;  // page_shift: log2 of the page's tokens
   int causal, window;
   float scale_log2;
-  int row_tiles;  // row tiles (8 * NT rows each) of G * N rows
+  int row_tiles;  // row tiles (8 rows each) of G * N rows
   int ctas;       // CTAs of the attention launch (the combine launch needs it)
-  float* part_o;  // [2 * ctas][8 * NT][D]
-  float2* part_ml;  // [2 * ctas][8 * NT]: maximum (log2 units), sum
+  float* part_o;  // [2 * ctas][8][D]
+  float2* part_ml;  // [2 * ctas][8]: maximum (log2 units), sum
   int join_blocks;  // CTAs of the join per unit
   int* status;
   long long wait_limit;
@@ -331,7 +331,7 @@ __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY
 
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(const Kv4Params p) {
-  constexpr int D = C::D, NT = 1, NG = C::NG, KS = C::KS, KB = C::KB, TB = C::TB, SB = C::SB, ROWS = C::ROWS;
+  constexpr int D = C::D, NG = C::NG, KS = C::KS, KB = C::KB, TB = C::TB, SB = C::SB, ROWS = C::ROWS;
   constexpr int NST = C::NST, BB = C::BLOCK_BYTES, PP = C::P_PITCH;
   constexpr bool BF16 = C::BF16;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -556,19 +556,16 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
     const int all_hi = p.causal ? min(u.len, off + r0 / p.G + 1) : u.len;
     const int all_lo = (p.causal && p.window > 0) ? max(0, off + nlast - p.window + 1) : 0;
 
-    float acc[NT][4][4];
+    float acc[4][4];
     // Rows 2 tig, 2 tig + 1: reference maximum (the same in all warps) and sum
     // of P over this warp's blocks.
-    float mref[NT][2], l_run[NT][2];
+    float mref[2], l_run[2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[nt][j][e] = 0.f;
-      mref[nt][0] = mref[nt][1] = -INFINITY;
-      l_run[nt][0] = l_run[nt][1] = 0.f;
-    }
+      for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+    mref[0] = mref[1] = -INFINITY;
+    l_run[0] = l_run[1] = 0.f;
 
     for (int tile = t0; tile < t1; ++tile) {
       const int nv = min(TB, u.nblk - tile * TB);
@@ -576,7 +573,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
       // some row of the unit does not see all of the tile's keys
       const bool edge = key_tile < all_lo || key_tile + nv * 16 > all_hi;
       // ---------------- scores ----------------
-      float s[KB][NT][4];
+      float s[KB][4];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         if (KB > 1 || warp / SB == half) wait_full();
@@ -587,10 +584,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
           const uint32_t base = ring + slot * C::STAGE_BYTES + (blk - half * SB) * BB;
           const uint32_t codes = base + lane * 16, metas = base + NG * KV4_CODE_BYTES + gid * 4;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[kb][nt][e] = 0.f;
-#pragma unroll(NT > 1 ? 2 : 4)
+            for (int e = 0; e < 4; ++e) s[kb][e] = 0.f;
+#pragma unroll 4
           for (int g = 0; g < NG; ++g) {
             const uint4 w = lds128(codes + g * KV4_CODE_BYTES);
             const uint32_t m = lds32(metas + g * KV4_META_BYTES);  // tokens gid, gid + 8
@@ -600,22 +595,19 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
             const uint32_t yl = w.y & 0x0F0F0F0Fu, yh = (w.y >> 4) & 0x0F0F0F0Fu;  // token gid, word 2 tig + 1
             const uint32_t zl = w.z & 0x0F0F0F0Fu, zh = (w.z >> 4) & 0x0F0F0F0Fu;  // token gid + 8
             const uint32_t wl = w.w & 0x0F0F0F0Fu, wh = (w.w >> 4) & 0x0F0F0F0Fu;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const uint32_t qa = qbase + nt * 8 * C::Q_PITCH + g * 128;
-              const uint4 q0 = lds128(qa), q1 = lds128(qa + 16);
-              int th[4], tl[4];
-              imma16832(th, xl, zl, xh, zh, q0.x, q0.y, 0, 0, 0, 0);
-              imma16832(tl, xl, zl, xh, zh, q0.z, q0.w, 0, 0, 0, 0);
-              imma16832(th, yl, wl, yh, wh, q1.x, q1.y, th[0], th[1], th[2], th[3]);
-              imma16832(tl, yl, wl, yh, wh, q1.z, q1.w, tl[0], tl[1], tl[2], tl[3]);
-              const int2 sq = *reinterpret_cast<const int2*>(sSum + g * ROWS + nt * 8 + 2 * tig);
-              float* v = s[kb][nt];
-              v[0] = fmaf(s0, static_cast<float>(th[0] * 256 + (tl[0] - z0 * sq.x)), v[0]);
-              v[1] = fmaf(s0, static_cast<float>(th[1] * 256 + (tl[1] - z0 * sq.y)), v[1]);
-              v[2] = fmaf(s1, static_cast<float>(th[2] * 256 + (tl[2] - z1 * sq.x)), v[2]);
-              v[3] = fmaf(s1, static_cast<float>(th[3] * 256 + (tl[3] - z1 * sq.y)), v[3]);
-            }
+            const uint32_t qa = qbase + g * 128;
+            const uint4 q0 = lds128(qa), q1 = lds128(qa + 16);
+            int th[4], tl[4];
+            imma16832(th, xl, zl, xh, zh, q0.x, q0.y, 0, 0, 0, 0);
+            imma16832(tl, xl, zl, xh, zh, q0.z, q0.w, 0, 0, 0, 0);
+            imma16832(th, yl, wl, yh, wh, q1.x, q1.y, th[0], th[1], th[2], th[3]);
+            imma16832(tl, yl, wl, yh, wh, q1.z, q1.w, tl[0], tl[1], tl[2], tl[3]);
+            const int2 sq = *reinterpret_cast<const int2*>(sSum + g * ROWS + 2 * tig);
+            float* v = s[kb];
+            v[0] = fmaf(s0, static_cast<float>(th[0] * 256 + (tl[0] - z0 * sq.x)), v[0]);
+            v[1] = fmaf(s0, static_cast<float>(th[1] * 256 + (tl[1] - z0 * sq.y)), v[1]);
+            v[2] = fmaf(s1, static_cast<float>(th[2] * 256 + (tl[2] - z1 * sq.x)), v[2]);
+            v[3] = fmaf(s1, static_cast<float>(th[3] * 256 + (tl[3] - z1 * sq.y)), v[3]);
           }
         }
         release();
@@ -626,115 +618,104 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
       float* M = sM + buf * 8 * ROWS;
       bool above = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          const int blk = warp + 8 * kb;
-          if (blk >= nv) continue;
-          float* v = s[kb][nt];
-          const float2 sc = *reinterpret_cast<const float2*>(sScale + nt * 8 + 2 * tig);
-          v[0] *= sc.x;
-          v[1] *= sc.y;
-          v[2] *= sc.x;
-          v[3] *= sc.y;
-          if (edge) {
-            const int4 mk = *reinterpret_cast<const int4*>(sMask + nt * 8 + 2 * tig);  // two rows' (first, count)
-            const int key = key_tile + blk * 16 + gid;
-            if (static_cast<unsigned>(key - mk.x) >= static_cast<unsigned>(mk.y)) v[0] = -INFINITY;
-            if (static_cast<unsigned>(key - mk.z) >= static_cast<unsigned>(mk.w)) v[1] = -INFINITY;
-            if (static_cast<unsigned>(key + 8 - mk.x) >= static_cast<unsigned>(mk.y)) v[2] = -INFINITY;
-            if (static_cast<unsigned>(key + 8 - mk.z) >= static_cast<unsigned>(mk.w)) v[3] = -INFINITY;
-          }
-          above |= fmaxf(v[0], v[2]) > mref[nt][0] + C::SLACK || fmaxf(v[1], v[3]) > mref[nt][1] + C::SLACK;
+      for (int kb = 0; kb < KB; ++kb) {
+        const int blk = warp + 8 * kb;
+        if (blk >= nv) continue;
+        float* v = s[kb];
+        const float2 sc = *reinterpret_cast<const float2*>(sScale + 2 * tig);
+        v[0] *= sc.x;
+        v[1] *= sc.y;
+        v[2] *= sc.x;
+        v[3] *= sc.y;
+        if (edge) {
+          const int4 mk = *reinterpret_cast<const int4*>(sMask + 2 * tig);  // two rows' (first, count)
+          const int key = key_tile + blk * 16 + gid;
+          if (static_cast<unsigned>(key - mk.x) >= static_cast<unsigned>(mk.y)) v[0] = -INFINITY;
+          if (static_cast<unsigned>(key - mk.z) >= static_cast<unsigned>(mk.w)) v[1] = -INFINITY;
+          if (static_cast<unsigned>(key + 8 - mk.x) >= static_cast<unsigned>(mk.y)) v[2] = -INFINITY;
+          if (static_cast<unsigned>(key + 8 - mk.z) >= static_cast<unsigned>(mk.w)) v[3] = -INFINITY;
         }
+        above |= fmaxf(v[0], v[2]) > mref[0] + C::SLACK || fmaxf(v[1], v[3]) > mref[1] + C::SLACK;
       }
       const bool raise = __any_sync(0xffffffffu, above);
       if (lane == 0) raised[buf][warp] = raise;
       const int perm = (gid >> 1) * 4 + (gid & 1);  // order (2t, 2t+1, 2t+8, 2t+9) of the value side
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float f0 = mref[nt][0], f1 = mref[nt][1];
-        if (raise) {
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb) {
-            if (warp + 8 * kb >= nv) continue;
-            f0 = fmaxf(f0, fmaxf(s[kb][nt][0], s[kb][nt][2]) + C::RAISE);
-            f1 = fmaxf(f1, fmaxf(s[kb][nt][1], s[kb][nt][3]) + C::RAISE);
-          }
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) {
-            f0 = fmaxf(f0, __shfl_xor_sync(0xffffffffu, f0, o));
-            f1 = fmaxf(f1, __shfl_xor_sync(0xffffffffu, f1, o));
-          }
-          l_run[nt][0] *= ex2(mref[nt][0] - finite_or_zero(f0));
-          l_run[nt][1] *= ex2(mref[nt][1] - finite_or_zero(f1));
-          if (gid == 0) *reinterpret_cast<float2*>(M + warp * ROWS + nt * 8 + 2 * tig) = make_float2(f0, f1);
-        }
-        f0 = finite_or_zero(f0);
-        f1 = finite_or_zero(f1);
+      float f0 = mref[0], f1 = mref[1];
+      if (raise) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
-          const int blk = warp + 8 * kb;
-          if (blk >= nv) continue;
-          float* v = s[kb][nt];
-          v[0] = ex2(v[0] - f0);
-          v[1] = ex2(v[1] - f1);
-          v[2] = ex2(v[2] - f0);
-          v[3] = ex2(v[3] - f1);
-          l_run[nt][0] += v[0] + v[2];
-          l_run[nt][1] += v[1] + v[3];
-          float* d = P + (blk * ROWS + nt * 8 + 2 * tig) * PP + perm;
-          d[0] = v[0];
-          d[2] = v[2];
-          d[PP] = v[1];
-          d[PP + 2] = v[3];
+          if (warp + 8 * kb >= nv) continue;
+          f0 = fmaxf(f0, fmaxf(s[kb][0], s[kb][2]) + C::RAISE);
+          f1 = fmaxf(f1, fmaxf(s[kb][1], s[kb][3]) + C::RAISE);
         }
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          f0 = fmaxf(f0, __shfl_xor_sync(0xffffffffu, f0, o));
+          f1 = fmaxf(f1, __shfl_xor_sync(0xffffffffu, f1, o));
+        }
+        l_run[0] *= ex2(mref[0] - finite_or_zero(f0));
+        l_run[1] *= ex2(mref[1] - finite_or_zero(f1));
+        if (gid == 0) *reinterpret_cast<float2*>(M + warp * ROWS + 2 * tig) = make_float2(f0, f1);
+      }
+      f0 = finite_or_zero(f0);
+      f1 = finite_or_zero(f1);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const int blk = warp + 8 * kb;
+        if (blk >= nv) continue;
+        float* v = s[kb];
+        v[0] = ex2(v[0] - f0);
+        v[1] = ex2(v[1] - f1);
+        v[2] = ex2(v[2] - f0);
+        v[3] = ex2(v[3] - f1);
+        l_run[0] += v[0] + v[2];
+        l_run[1] += v[1] + v[3];
+        float* d = P + (blk * ROWS + 2 * tig) * PP + perm;
+        d[0] = v[0];
+        d[2] = v[2];
+        d[PP] = v[1];
+        d[PP + 2] = v[3];
       }
       // ---------------- new maxima, if any warp published some ----------------
       const bool rescale = compute_barrier_or(raise);
       // A warp's P refers to its own published maximum, or to the old one: in
       // the value loop row gid's factor brings it to the new one.
-      float vold[NT], vnew[NT];
+      float vold = 0.f, vnew = 0.f;
       if (rescale) {
+        float m0 = mref[0], m1 = mref[1];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float m0 = mref[nt][0], m1 = mref[nt][1];
-#pragma unroll
-          for (int w = 0; w < 8; ++w) {
-            if (raised[buf][w]) {
-              const float2 x = *reinterpret_cast<const float2*>(M + w * ROWS + nt * 8 + 2 * tig);
-              m0 = fmaxf(m0, x.x);
-              m1 = fmaxf(m1, x.y);
-            }
+        for (int w = 0; w < 8; ++w) {
+          if (raised[buf][w]) {
+            const float2 x = *reinterpret_cast<const float2*>(M + w * ROWS + 2 * tig);
+            m0 = fmaxf(m0, x.x);
+            m1 = fmaxf(m1, x.y);
           }
-          float2 mine = make_float2(mref[nt][0], mref[nt][1]);
-          if (raise) mine = *reinterpret_cast<const float2*>(M + warp * ROWS + nt * 8 + 2 * tig);
-          l_run[nt][0] *= ex2(mine.x - finite_or_zero(m0));
-          l_run[nt][1] *= ex2(mine.y - finite_or_zero(m1));
-          const float a0 = ex2(mref[nt][0] - finite_or_zero(m0)), a1 = ex2(mref[nt][1] - finite_or_zero(m1));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            acc[nt][j][0] *= a0;
-            acc[nt][j][1] *= a1;
-            acc[nt][j][2] *= a0;
-            acc[nt][j][3] *= a1;
-          }
-          // row gid belongs to lanes with tig = gid / 2
-          const float o0 = __shfl_sync(0xffffffffu, mref[nt][0], gid >> 1), o1 = __shfl_sync(0xffffffffu, mref[nt][1], gid >> 1);
-          const float n0 = __shfl_sync(0xffffffffu, m0, gid >> 1), n1 = __shfl_sync(0xffffffffu, m1, gid >> 1);
-          vold[nt] = (gid & 1) ? o1 : o0;
-          vnew[nt] = finite_or_zero((gid & 1) ? n1 : n0);
-          mref[nt][0] = m0;
-          mref[nt][1] = m1;
         }
+        float2 mine = make_float2(mref[0], mref[1]);
+        if (raise) mine = *reinterpret_cast<const float2*>(M + warp * ROWS + 2 * tig);
+        l_run[0] *= ex2(mine.x - finite_or_zero(m0));
+        l_run[1] *= ex2(mine.y - finite_or_zero(m1));
+        const float a0 = ex2(mref[0] - finite_or_zero(m0)), a1 = ex2(mref[1] - finite_or_zero(m1));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          acc[j][0] *= a0;
+          acc[j][1] *= a1;
+          acc[j][2] *= a0;
+          acc[j][3] *= a1;
+        }
+        // row gid belongs to lanes with tig = gid / 2
+        const float o0 = __shfl_sync(0xffffffffu, mref[0], gid >> 1), o1 = __shfl_sync(0xffffffffu, mref[1], gid >> 1);
+        const float n0 = __shfl_sync(0xffffffffu, m0, gid >> 1), n1 = __shfl_sync(0xffffffffu, m1, gid >> 1);
+        vold = (gid & 1) ? o1 : o0;
+        vnew = finite_or_zero((gid & 1) ? n1 : n0);
+        mref[0] = m0;
+        mref[1] = m1;
       }
 
       // ---------------- values ----------------
-      float wz[NT][4];  // -sum (F + z) P' of this tile
+      float wz[4];  // -sum (F + z) P' of this tile
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) wz[nt][e] = 0.f;
+        for (int e = 0; e < 4; ++e) wz[e] = 0.f;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         wait_full();
@@ -753,38 +734,35 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
           codes16<BF16>(__byte_perm(c.z, c.w, 0x7632), tops, x3);
           const float s0 = meta_scale(mv.x << 16), s1 = meta_scale(mv.x), s2 = meta_scale(mv.y << 16),
                       s3 = meta_scale(mv.y);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float4 pr = *reinterpret_cast<const float4*>(prow + (sblk * ROWS + nt * 8) * PP);
-            if constexpr (SPECIAL) {
-              if (rescale) {
-                const int w = (half * SB + sblk) & 7;
-                const float from = raised[buf][w] ? M[w * ROWS + nt * 8 + gid] : vold[nt];
-                const float f = ex2(finite_or_zero(from) - vnew[nt]);
-                pr.x *= f;
-                pr.y *= f;
-                pr.z *= f;
-                pr.w *= f;
-              }
-              // a masked token's scale may be anything (a slot never written): its product must be 0
-              pr.x = pr.x == 0.f ? 0.f : pr.x * s0;
-              pr.y = pr.y == 0.f ? 0.f : pr.y * s1;
-              pr.z = pr.z == 0.f ? 0.f : pr.z * s2;
-              pr.w = pr.w == 0.f ? 0.f : pr.w * s3;
-            } else {
-              pr.x *= s0;
-              pr.y *= s1;
-              pr.z *= s2;
-              pr.w *= s3;
+          float4 pr = *reinterpret_cast<const float4*>(prow + sblk * ROWS * PP);
+          if constexpr (SPECIAL) {
+            if (rescale) {
+              const int w = (half * SB + sblk) & 7;
+              const float from = raised[buf][w] ? M[w * ROWS + gid] : vold;
+              const float f = ex2(finite_or_zero(from) - vnew);
+              pr.x *= f;
+              pr.y *= f;
+              pr.z *= f;
+              pr.w *= f;
             }
-            const uint32_t b0 = pack2<BF16>(pr.x, pr.y), b1 = pack2<BF16>(pr.z, pr.w);
-            mma16816<BF16>(acc[nt][0], x0[0], x0[1], x2[0], x2[1], b0, b1);
-            mma16816<BF16>(acc[nt][1], x0[2], x0[3], x2[2], x2[3], b0, b1);
-            mma16816<BF16>(acc[nt][2], x1[0], x1[1], x3[0], x3[1], b0, b1);
-            mma16816<BF16>(acc[nt][3], x1[2], x1[3], x3[2], x3[3], b0, b1);
-            mma16816<BF16>(wz[nt], minus_zero_even<BF16>(mv.x, tops), minus_zero_odd<BF16>(mv.x, tops),
-                           minus_zero_even<BF16>(mv.y, tops), minus_zero_odd<BF16>(mv.y, tops), b0, b1);
+            // a masked token's scale may be anything (a slot never written): its product must be 0
+            pr.x = pr.x == 0.f ? 0.f : pr.x * s0;
+            pr.y = pr.y == 0.f ? 0.f : pr.y * s1;
+            pr.z = pr.z == 0.f ? 0.f : pr.z * s2;
+            pr.w = pr.w == 0.f ? 0.f : pr.w * s3;
+          } else {
+            pr.x *= s0;
+            pr.y *= s1;
+            pr.z *= s2;
+            pr.w *= s3;
           }
+          const uint32_t b0 = pack2<BF16>(pr.x, pr.y), b1 = pack2<BF16>(pr.z, pr.w);
+          mma16816<BF16>(acc[0], x0[0], x0[1], x2[0], x2[1], b0, b1);
+          mma16816<BF16>(acc[1], x0[2], x0[3], x2[2], x2[3], b0, b1);
+          mma16816<BF16>(acc[2], x1[0], x1[1], x3[0], x3[1], b0, b1);
+          mma16816<BF16>(acc[3], x1[2], x1[3], x3[2], x3[3], b0, b1);
+          mma16816<BF16>(wz, minus_zero_even<BF16>(mv.x, tops), minus_zero_odd<BF16>(mv.x, tops),
+                         minus_zero_even<BF16>(mv.y, tops), minus_zero_odd<BF16>(mv.y, tops), b0, b1);
         };
         if (!rescale && !edge && nv == TB) {
 #pragma unroll(SB / KS > 4 ? 4 : SB / KS)
@@ -799,11 +777,9 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
         release();
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[nt][j][e] += wz[nt][e];
+          for (int e = 0; e < 4; ++e) acc[j][e] += wz[e];
       buf ^= 1;
     }
 
@@ -812,19 +788,16 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
     compute_barrier();  // all value-side reads of P and M are done
     float* xM = sM;             // [ROWS] maxima
     float* xL = sM + 8 * ROWS;  // [8][ROWS] sums
+    float l0 = l_run[0], l1 = l_run[1];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float l0 = l_run[nt][0], l1 = l_run[nt][1];
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        l0 += __shfl_xor_sync(0xffffffffu, l0, o);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, o);
-      }
-      if (gid == 0) {
-        if (warp == 0)
-          *reinterpret_cast<float2*>(xM + nt * 8 + 2 * tig) = make_float2(mref[nt][0], mref[nt][1]);
-        *reinterpret_cast<float2*>(xL + warp * ROWS + nt * 8 + 2 * tig) = make_float2(l0, l1);
-      }
+    for (int o = 4; o < 32; o <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+    }
+    if (gid == 0) {
+      if (warp == 0)
+        *reinterpret_cast<float2*>(xM + 2 * tig) = make_float2(mref[0], mref[1]);
+      *reinterpret_cast<float2*>(xL + warp * ROWS + 2 * tig) = make_float2(l0, l1);
     }
     // value-side slices: halve their number until one is left
     if constexpr (KS > 1) {
@@ -834,23 +807,19 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
         const int lane_at = ((dg * live + (ks % live)) * 32 + lane) * 4;
         if (ks >= live && ks < 2 * live) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
             for (int j = 0; j < 4; ++j)
-              *reinterpret_cast<float4*>(X + (nt * 4 + j) * (NG * live * 128) + lane_at) =
-                  make_float4(acc[nt][j][0], acc[nt][j][1], acc[nt][j][2], acc[nt][j][3]);
+              *reinterpret_cast<float4*>(X + j * (NG * live * 128) + lane_at) =
+                  make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
         }
         compute_barrier();
         if (ks < live) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const float4 v = *reinterpret_cast<const float4*>(X + (nt * 4 + j) * (NG * live * 128) + lane_at);
-              acc[nt][j][0] += v.x;
-              acc[nt][j][1] += v.y;
-              acc[nt][j][2] += v.z;
-              acc[nt][j][3] += v.w;
+              const float4 v = *reinterpret_cast<const float4*>(X + j * (NG * live * 128) + lane_at);
+              acc[j][0] += v.x;
+              acc[j][1] += v.y;
+              acc[j][2] += v.z;
+              acc[j][3] += v.w;
             }
         }
         compute_barrier();
@@ -862,37 +831,34 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
     const int part = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);  // a unit's later parts start a share
     if (ks == 0) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int e = 0; e < 2; ++e) {  // rows 2 tig, 2 tig + 1
+        const int i = 2 * tig + e, r = r0 + i;
+        const float m = xM[i];
+        float l = 0.f;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {  // rows 2 tig, 2 tig + 1
-          const int i = nt * 8 + 2 * tig + e, r = r0 + i;
-          const float m = xM[i];
-          float l = 0.f;
-#pragma unroll
-          for (int w = 0; w < 8; ++w) l += xL[w * ROWS + i];
-          // dims 64 dg + 8 gid + (0..7): MMA rows gid and gid + 8 of tile j are dims 2j and 2j + 1
-          if (whole) {
-            if (r < rows) {
-              const float inv = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
-              const int n = r / p.G, hq = h * p.G + r - n * p.G;
-              uint4 v;
-              v.x = pack2<BF16>(acc[nt][0][e] * inv, acc[nt][0][2 + e] * inv);
-              v.y = pack2<BF16>(acc[nt][1][e] * inv, acc[nt][1][2 + e] * inv);
-              v.z = pack2<BF16>(acc[nt][2][e] * inv, acc[nt][2][2 + e] * inv);
-              v.w = pack2<BF16>(acc[nt][3][e] * inv, acc[nt][3][2 + e] * inv);
-              *reinterpret_cast<uint4*>(p.o + u.b * p.o_sb + hq * p.o_sh + n * p.o_sn + dg * 64 + gid * 8) = v;
-              if (p.lse && dg == 0 && gid == 0)
-                p.lse[(static_cast<long long>(u.b) * p.Hq + hq) * p.N + n] =
-                    l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
-            }
-          } else {
-            float* d = p.part_o + (static_cast<long long>(part) * ROWS + i) * D + dg * 64 + gid * 8;
-            *reinterpret_cast<float4*>(d) =
-                make_float4(acc[nt][0][e], acc[nt][0][2 + e], acc[nt][1][e], acc[nt][1][2 + e]);
-            *reinterpret_cast<float4*>(d + 4) =
-                make_float4(acc[nt][2][e], acc[nt][2][2 + e], acc[nt][3][e], acc[nt][3][2 + e]);
-            if (dg == 0 && gid == 0) p.part_ml[static_cast<long long>(part) * ROWS + i] = make_float2(m, l);
+        for (int w = 0; w < 8; ++w) l += xL[w * ROWS + i];
+        // dims 64 dg + 8 gid + (0..7): MMA rows gid and gid + 8 of tile j are dims 2j and 2j + 1
+        if (whole) {
+          if (r < rows) {
+            const float inv = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
+            const int n = r / p.G, hq = h * p.G + r - n * p.G;
+            uint4 v;
+            v.x = pack2<BF16>(acc[0][e] * inv, acc[0][2 + e] * inv);
+            v.y = pack2<BF16>(acc[1][e] * inv, acc[1][2 + e] * inv);
+            v.z = pack2<BF16>(acc[2][e] * inv, acc[2][2 + e] * inv);
+            v.w = pack2<BF16>(acc[3][e] * inv, acc[3][2 + e] * inv);
+            *reinterpret_cast<uint4*>(p.o + u.b * p.o_sb + hq * p.o_sh + n * p.o_sn + dg * 64 + gid * 8) = v;
+            if (p.lse && dg == 0 && gid == 0)
+              p.lse[(static_cast<long long>(u.b) * p.Hq + hq) * p.N + n] =
+                  l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
           }
+        } else {
+          float* d = p.part_o + (static_cast<long long>(part) * ROWS + i) * D + dg * 64 + gid * 8;
+          *reinterpret_cast<float4*>(d) =
+              make_float4(acc[0][e], acc[0][2 + e], acc[1][e], acc[1][2 + e]);
+          *reinterpret_cast<float4*>(d + 4) =
+              make_float4(acc[2][e], acc[2][2 + e], acc[3][e], acc[3][2 + e]);
+          if (dg == 0 && gid == 0) p.part_ml[static_cast<long long>(part) * ROWS + i] = make_float2(m, l);
         }
       }
     }
@@ -938,6 +904,8 @@ __global__ void __launch_bounds__(512, 2) kv4_combine_kernel(const Kv4Params p) 
   const int c0 = begin / per, c1 = u.tiles == 0 ? c0 : (begin + u.tiles - 1) / per;
   const int limit = min(ROWS, p.G * p.N - u.rt * ROWS);                      // rows of the output
   const int rows = u.tiles == 0 ? 0 : min(limit, p.G * u.qlen - u.rt * ROWS);  // of them with keys
+  if (slice == 0 && h == 0 && threadIdx.x == 0 && p.kv_lens[u.b] > (p.cols << p.page_shift))
+    atomicCAS(p.status, 0, ST_KV4_LENGTH);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (c0 == c1 && rows == limit) return;  // written by its one CTA
   // columns of 128 floats; the slice's are [first, first + columns)

@@ -15,6 +15,11 @@ reference's hand-built stack (flash_attn/gemma4_e2e.py).
 
 Weights are random (no checkpoint is available offline); the decoder exists to
 drive the attention path at the real shapes, end to end.
+
+``Gemma4SyntheticDecoder.step`` serves from a paged 4-bit KV cache
+(``DecoderKV4Cache``): prompts, single tokens and drafted tokens of a ragged
+batch, requests coming and going. Nothing in a step synchronises with the
+host, so it can be captured into a CUDA graph and replayed.
 """
 from __future__ import annotations
 
@@ -24,7 +29,9 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-__all__ = ["Gemma4SyntheticConfig", "Gemma4SyntheticDecoder"]
+from .kv4 import attention_flash_gqa_kv4, kv4_alloc, kv4_append, kv4_plan
+
+__all__ = ["Gemma4SyntheticConfig", "Gemma4SyntheticDecoder", "DecoderKV4Cache"]
 
 
 @dataclass
@@ -75,6 +82,47 @@ def _rope_tables(n, dim, theta, device, dtype):
     return ang.cos().to(dtype)[None, :, None, :], ang.sin().to(dtype)[None, :, None, :]
 
 
+def _rope_at(positions, dim, theta, dtype):
+    """Tables of _rope_tables at int positions (B, N), for (B, N, H, D) operands."""
+    inv = 1.0 / (theta ** (torch.arange(0, dim, 2, device=positions.device, dtype=torch.float32) / dim))
+    ang = positions.clamp_min(0).float()[..., None] * inv
+    return ang.cos().to(dtype)[:, :, None, :], ang.sin().to(dtype)[:, :, None, :]
+
+
+class DecoderKV4Cache:
+    """The decoder's paged 4-bit cache: pages of every layer, and one block table for all of them (a
+    page id means the same tokens in each layer).
+
+    `max_batch` rows of at most `max_len` tokens; `num_pages` pages (default: enough for every row to
+    be full). A row holds one request at a time: tokens are added by ``plan``, and a request whose
+    new_lens entry is negative is finished, its pages go back and its row is free from then on."""
+
+    def __init__(self, cfg: Gemma4SyntheticConfig, max_batch: int, max_len: int, num_pages: int | None = None,
+                 page_size: int = 64, dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        columns = -(-max_len // page_size)
+        num_pages = max_batch * columns if num_pages is None else num_pages
+        self.max_len, self.page_size = columns * page_size, page_size
+        self.layers = []
+        for layer in range(cfg.num_layers):
+            heads, dim = ((cfg.global_kv_heads, cfg.global_head_dim) if cfg.is_global(layer)
+                          else (cfg.local_kv_heads, cfg.local_head_dim))
+            self.layers.append(kv4_alloc(num_pages, heads, dim, page_size, dtype, device))
+        i32 = dict(dtype=torch.int32, device=device)
+        self.block_table = torch.full((max_batch, columns), -1, **i32)
+        self.kv_lens = torch.zeros(max_batch, **i32)
+        self.free_pages = torch.arange(num_pages, **i32)
+        self.free_state = torch.tensor([0, num_pages], **i32)
+
+    def plan(self, new_lens, max_new: int):
+        """Plan of the next step (see kv4_plan); this cache's tables and lengths move on in place."""
+        p = kv4_plan(self.kv_lens, new_lens, self.block_table, self.free_pages, self.free_state,
+                     page_size=self.page_size, max_new=max_new)
+        self.block_table.copy_(p.block_table)
+        self.kv_lens.copy_(p.kv_lens)
+        self.free_state.copy_(p.free_state)
+        return p
+
+
 class Attention(nn.Module):
     def __init__(self, cfg: Gemma4SyntheticConfig, layer: int):
         super().__init__()
@@ -95,15 +143,28 @@ class Attention(nn.Module):
         self.q_norm = RMSNorm(self.head_dim, cfg.rms_eps)
         self.k_norm = RMSNorm(self.head_dim, cfg.rms_eps)
 
-    def forward(self, x, rope):
-        from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
-
+    def _qkv(self, x, rope):
         b, n, _ = x.shape
         q = self.q_norm(self.q_proj(x).view(b, n, self.num_heads, self.head_dim))
         k = self.k_norm(self.k_proj(x).view(b, n, self.num_kv_heads, self.head_dim))
         v = self.v_proj(x).view(b, n, self.num_kv_heads, self.head_dim)
         cos, sin = rope
-        q, k = _rope(q, cos, sin), _rope(k, cos, sin)
+        return _rope(q, cos, sin), _rope(k, cos, sin), v
+
+    def step(self, x, rope, cache, plan, max_len):
+        """New tokens x (B, N, hidden) into the layer's 4-bit cache, and their attention over it."""
+        q, k, v = self._qkv(x, rope)
+        kv4_append(cache, k.transpose(1, 2), v.transpose(1, 2), plan.slot_map)
+        out = attention_flash_gqa_kv4(q.transpose(1, 2), cache, plan.block_table, plan.kv_lens, causal=True,
+                                      slide_size=self.sliding_window or 0, q_lens=plan.new_lens,
+                                      softmax_scale=self.scaling, max_kv_len=max_len)
+        return self.o_proj(out.transpose(1, 2).reshape(x.shape[0], x.shape[1], -1))
+
+    def forward(self, x, rope):
+        from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
+
+        b, n, _ = x.shape
+        q, k, v = self._qkv(x, rope)
         attn = ALL_ATTENTION_FUNCTIONS[self.cfg.attn_implementation]
         out, _ = attn(self, q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), None,
                       dropout=0.0, scaling=self.scaling, sliding_window=self.sliding_window)
@@ -120,10 +181,15 @@ class Block(nn.Module):
         self.up_proj = nn.Linear(cfg.hidden_size, cfg.intermediate_size, bias=False)
         self.down_proj = nn.Linear(cfg.intermediate_size, cfg.hidden_size, bias=False)
 
-    def forward(self, x, rope):
-        x = x + self.attn(self.attn_norm(x), rope)
+    def _mlp(self, x):
         h = self.mlp_norm(x)
         return x + self.down_proj(F.gelu(self.gate_proj(h), approximate="tanh") * self.up_proj(h))
+
+    def step(self, x, rope, cache, plan, max_len):
+        return self._mlp(x + self.attn.step(self.attn_norm(x), rope, cache, plan, max_len))
+
+    def forward(self, x, rope):
+        return self._mlp(x + self.attn(self.attn_norm(x), rope))
 
 
 class Gemma4SyntheticDecoder(nn.Module):
@@ -157,3 +223,20 @@ class Gemma4SyntheticDecoder(nn.Module):
             x = layer(x, ropes[key])
         x = self.norm(x)
         return x @ self.embed.weight.t()
+
+    @torch.no_grad()
+    def step(self, input_ids, new_lens, cache: DecoderKV4Cache):
+        """One serving step: input_ids (B, N) holds new_lens[b] (int32 CUDA, 0..N, negative: finished) new
+        tokens of each of the cache's rows, padded to N. Returns the logits (B, N, vocab) (of padding and
+        refused requests: of no meaning) and the step's plan."""
+        n = input_ids.shape[1]
+        plan = cache.plan(new_lens, n)
+        x = self.embed(input_ids) * (self.cfg.hidden_size ** 0.5)
+        ropes = {}
+        for layer, pages in zip(self.layers, cache.layers):
+            a = layer.attn
+            key = (a.head_dim, a.rope_theta)
+            if key not in ropes:
+                ropes[key] = _rope_at(plan.positions, a.head_dim, a.rope_theta, x.dtype)
+            x = layer.step(x, ropes[key], pages, plan, cache.max_len)
+        return self.norm(x) @ self.embed.weight.t(), plan
