@@ -18,6 +18,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
+#include <string>
 #include <tuple>
 
 #include "../../include/gqa_fa_b200.h"
@@ -140,22 +141,25 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> bwd_meta(const at::Tensor& q, con
 
 // ---------------------------------------------------------------- 4-bit cache
 // Device and type checks live here, beside the launch: everything below is
-// handed to the C ABI as raw pointers.
+// handed to the C ABI as raw pointers. Messages take numbers as strings: with a
+// libstdc++ linked in statically (some toolchains do), writing a number to the
+// stream behind TORCH_CHECK mixes two copies of the library and crashes.
+std::string str(int64_t v) { return std::to_string(v); }
 void check_int32(const at::Tensor& t, const char* name, const at::Device& dev) {
   TORCH_CHECK(t.is_cuda(), "gqafa: ", name, " must be a CUDA tensor (there is no CPU path)");
-  TORCH_CHECK_VALUE(t.device() == dev, "gqafa: ", name, " is on ", t.device(), ", expected ", dev);
-  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, "gqafa: ", name, " must be int32, got ", t.scalar_type());
+  TORCH_CHECK_VALUE(t.device() == dev, "gqafa: ", name, " is on ", t.device().str(), ", expected ", dev.str());
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, "gqafa: ", name, " must be int32, got ", c10::toString(t.scalar_type()));
 }
 at::Tensor vector_int32(const at::Tensor& t, const char* name, int64_t n, const at::Device& dev) {
   check_int32(t, name, dev);
-  TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == n, "gqafa: ", name, " must have shape (", n, ",)");
+  TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == n, "gqafa: ", name, " must have shape (", str(n), ",)");
   return t.contiguous();
 }
 // A matrix whose rows are contiguous (any row stride).
 at::Tensor rows_int32(const at::Tensor& t, const char* name, int64_t rows, const at::Device& dev) {
   check_int32(t, name, dev);
-  TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == rows && t.size(1) > 0, "gqafa: ", name, " must have shape (", rows,
-                    ", n > 0)");
+  TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == rows && t.size(1) > 0, "gqafa: ", name, " must have shape (",
+                    str(rows), ", n > 0)");
   return (t.stride(1) == 1 || t.size(1) == 1) && t.stride(0) >= 0 ? t : t.contiguous();
 }
 struct Pages {
@@ -163,19 +167,20 @@ struct Pages {
 };
 Pages check_pages(const at::Tensor& pages, int64_t page_size, const at::Device& dev) {
   TORCH_CHECK(pages.is_cuda(), "gqafa: pages must be a CUDA tensor (there is no CPU path)");
-  TORCH_CHECK_VALUE(pages.device() == dev, "gqafa: pages are on ", pages.device(), ", expected ", dev);
+  TORCH_CHECK_VALUE(pages.device() == dev, "gqafa: pages are on ", pages.device().str(), ", expected ", dev.str());
   TORCH_CHECK_VALUE(pages.scalar_type() == at::kByte && pages.dim() == 5 && pages.is_contiguous() && pages.size(1) == 2,
                     "gqafa: pages must be a contiguous uint8 tensor (pages, 2, heads, blocks, block bytes)");
-  TORCH_CHECK_VALUE(page_size == 16 * pages.size(3), "gqafa: pages hold ", 16 * pages.size(3),
-                    " tokens each, page_size is ", page_size);
+  TORCH_CHECK_VALUE(page_size == 16 * pages.size(3), "gqafa: pages hold ", str(16 * pages.size(3)),
+                    " tokens each, page_size is ", str(page_size));
   const int64_t dim = pages.size(4) / 544 * 64;
   TORCH_CHECK_VALUE(pages.size(4) % 544 == 0 && dim > 0, "gqafa: a block of pages must hold 544 bytes per 64 dims");
   return {pages.size(0), pages.size(2), page_size, dim};
 }
 void check_rows(const at::Tensor& t, const char* name, const Pages& pg, const at::Device& dev) {
   check_4d(t, name);
-  TORCH_CHECK_VALUE(t.device() == dev, "gqafa: ", name, " is on ", t.device(), ", expected ", dev);
-  TORCH_CHECK_VALUE(t.size(3) == pg.dim, "gqafa: ", name, " has head_dim ", t.size(3), ", the cache ", pg.dim);
+  TORCH_CHECK_VALUE(t.device() == dev, "gqafa: ", name, " is on ", t.device().str(), ", expected ", dev.str());
+  TORCH_CHECK_VALUE(t.size(3) == pg.dim, "gqafa: ", name, " has head_dim ", str(t.size(3)), ", the cache ",
+                    str(pg.dim));
   TORCH_CHECK_VALUE(t.numel() > 0, "gqafa: ", name, " is empty");
 }
 // As abi_ready, and a broadcast tensor (stride 0) becomes a whole one.
@@ -219,7 +224,7 @@ class Int32Pack {
   int64_t at_ = 0;
 };
 int to_int(int64_t v, const char* name) {
-  TORCH_CHECK_VALUE(v >= INT32_MIN && v <= INT32_MAX, "gqafa: ", name, " out of range: ", v);
+  TORCH_CHECK_VALUE(v >= INT32_MIN && v <= INT32_MAX, "gqafa: ", name, " out of range: ", str(v));
   return static_cast<int>(v);
 }
 
@@ -260,13 +265,13 @@ void kv4_append(at::Tensor pages, const at::Tensor& k_in, const at::Tensor& v_in
   check_rows(k_in, "k", pg, dev);
   check_rows(v_in, "v", pg, dev);
   TORCH_CHECK_VALUE(k_in.sizes() == v_in.sizes() && k_in.size(1) == pg.heads,
-                    "gqafa: k and v must have shape (B, ", pg.heads, ", N, ", pg.dim, ")");
+                    "gqafa: k and v must have shape (B, ", str(pg.heads), ", N, ", str(pg.dim), ")");
   TORCH_CHECK_TYPE(k_in.scalar_type() == v_in.scalar_type(), "gqafa: k and v must share a dtype");
   c10::cuda::CUDAGuard guard(dev);
   const at::Tensor k = rows_ready(k_in), v = rows_ready(v_in);
   const int64_t B = k.size(0), N = k.size(2);
   const at::Tensor slots = rows_int32(slot_map, "slot_map", B, dev);
-  TORCH_CHECK_VALUE(slots.size(1) == N, "gqafa: slot_map must have shape (", B, ", ", N, ")");
+  TORCH_CHECK_VALUE(slots.size(1) == N, "gqafa: slot_map must have shape (", str(B), ", ", str(N), ")");
   const Strides sk(k), sv(v);
   check(gqafa_kv4_append(k.data_ptr(), sk.s, v.data_ptr(), sv.s, slots.data_ptr<int>(), slots.stride(0),
                          pages.data_ptr(), pg.count, to_int(B, "B"), to_int(pg.heads, "heads"), to_int(N, "N"),
