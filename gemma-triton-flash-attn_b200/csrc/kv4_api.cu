@@ -108,11 +108,20 @@ constexpr long long kDenseBytes = 2LL << 30;
 
 // Many query rows per KV head are bound by the products, not by the cache: then
 // the keys and values are written out in 16 bits once (exactly) and the tcgen05
-// forward of dense caches runs over them, with the lengths of each request.
-// Its tiles hold 128 tokens of one query head; the MMAs above take 8 rows of
-// all heads of a group.
-bool dense_path(int G, int N) {
-  return static_cast<long long>(G) * N > 23LL * G * ((N + 127) / 128) + 40;
+// forward of dense caches runs over them, with the lengths of each request. Its
+// CTAs (pairs at head_dim 512) take 128 tokens of one query head over all keys;
+// the MMAs above take 8 rows of all heads of a group and split the keys. Both
+// times grow with the keys: per key a unit of 8 rows costs the whole GPU 82, 52,
+// 30, 21 ps at head_dim 512, 256, 128, 64, a wave of 128-row tiles 20.6, 18.7,
+// 16.4, 18.0 ns. Measured on both sides of the rule, 2 requests of 7K keys, 32/4
+// heads, head_dim 512: 24 tokens 141 us in units and 171 us dense, 48 tokens 240
+// and 172 us; 8 requests, 16/4 heads, head_dim 64: 48 tokens 120 and 147 us, 100
+// tokens 231 and 148 us.
+bool dense_path(int B, int Hq, int Hkv, int N, int D, int sms) {
+  const long long units = static_cast<long long>(B) * Hkv * ((static_cast<long long>(Hq / Hkv) * N + 7) / 8);
+  const long long tiles = static_cast<long long>(B) * Hq * ((N + 127) / 128) * (D == 512 ? 2 : 1);
+  const int ratio = D == 512 ? 250 : (D == 256 ? 360 : (D == 128 ? 550 : 860));
+  return units > ratio * ((tiles + sms - 1) / sms);
 }
 
 // Units of 8 query rows, and the CTAs of the launch: two per SM, fewer where there
@@ -135,7 +144,7 @@ AttendShape attend_shape(int B, int Hq, int Hkv, int N, int D, int max_len, int 
   s.ctas = static_cast<int>(std::min<long long>(2LL * sms, s.units * tiles));
   // the join: at most two CTAs per SM, all of them where few units are cut into many parts
   s.join_blocks = 1;
-  if (dense_path(s.G, N)) {
+  if (dense_path(B, Hq, Hkv, N, D, sms)) {
     long long held = max_len;
     if (window > 0) held = std::min<long long>(held, static_cast<long long>(window) + N + 15);
     s.dense_rows = static_cast<int>((std::max<long long>(held, 1) + 15) / 16 * 16);

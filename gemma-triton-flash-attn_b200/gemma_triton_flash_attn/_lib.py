@@ -144,6 +144,8 @@ def load():
 def ops():
     """torch.ops.gqafa, loading libgqa_fa_ops.so on first use."""
     global _ops
+    if _ops is not None:
+        return _ops
     with _lock:
         if _ops is None:
             if not os.path.exists(OPS_PATH):

@@ -98,7 +98,15 @@ def _check_format(head_dim, page_size, dtype):
         raise NotImplementedError(f"page_size {page_size} is not implemented (supported: {PAGE_SIZES})")
 
 
-def _check_cuda(**tensors):
+def _all_cuda(*tensors):
+    try:
+        return all([t.is_cuda for t in tensors if t is not None])
+    except AttributeError:
+        return False
+
+
+def _refuse(**tensors):
+    """Name the argument that is not a CUDA tensor."""
     for name, t in tensors.items():
         if t is None:
             continue
@@ -138,11 +146,13 @@ def kv4_plan(kv_lens, new_lens, block_table, free_pages, free_state, page_size: 
     are, but for the ring's dead part, where returned pages are written: the
     next step passes the same ring and the returned ``free_state``.
     """
-    _check_cuda(kv_lens=kv_lens, new_lens=new_lens, block_table=block_table, free_pages=free_pages,
+    if not _all_cuda(kv_lens, new_lens, block_table, free_pages, free_state):
+        _refuse(kv_lens=kv_lens, new_lens=new_lens, block_table=block_table, free_pages=free_pages,
                 free_state=free_state)
     if page_size not in PAGE_SIZES:
         raise NotImplementedError(f"page_size {page_size} is not implemented (supported: {PAGE_SIZES})")
-    return KV4Plan(*_lib.ops().kv4_plan(kv_lens, new_lens, block_table, free_pages, free_state, page_size, max_new))
+    return KV4Plan._make(
+        _lib.ops().kv4_plan(kv_lens, new_lens, block_table, free_pages, free_state, page_size, max_new))
 
 
 def kv4_append(cache: KV4Cache, k, v, slot_map) -> None:
@@ -151,7 +161,8 @@ def kv4_append(cache: KV4Cache, k, v, slot_map) -> None:
     slot_map (B, N): the slot of each token, -1 to skip it. Slots must be
     distinct (those of a plan are). A group of 64 values that holds an infinity
     or a NaN reads back as NaN."""
-    _check_cuda(k=k, v=v, slot_map=slot_map)
+    if not _all_cuda(k, v, slot_map):
+        _refuse(k=k, v=v, slot_map=slot_map)
     if k.dtype != cache.dtype or v.dtype != cache.dtype:
         raise TypeError(f"k and v must have the cache's dtype {cache.dtype}, got {k.dtype}, {v.dtype}")
     _lib.ops().kv4_append(cache.pages, k, v, slot_map, cache.page_size)
@@ -164,7 +175,8 @@ def kv4_read(cache: KV4Cache, block_table, kv_lens, max_len: int, starts=None):
     kv_lens[b] on. The values are exactly those that the attention uses, so a
     prompt that attends to them through ``attention_flash_gqa`` sees what its
     later decode steps will see."""
-    _check_cuda(block_table=block_table, kv_lens=kv_lens, starts=starts)
+    if not _all_cuda(block_table, kv_lens, starts):
+        _refuse(block_table=block_table, kv_lens=kv_lens, starts=starts)
     return _lib.ops().kv4_read(cache.pages, block_table, kv_lens, max_len, starts, cache.page_size, cache.dtype)
 
 
@@ -183,7 +195,8 @@ def attention_flash_gqa_kv4(q, cache: KV4Cache, block_table, kv_lens, causal=Fal
     LSE (B, H_Q, N), -inf where no key is seen). max_kv_len: an upper bound of
     kv_lens known to the host, which sizes the launch (default: the block
     table's capacity; a bound that is too low costs speed, not results)."""
-    _check_cuda(q=q, block_table=block_table, kv_lens=kv_lens, q_lens=q_lens)
+    if not _all_cuda(q, block_table, kv_lens, q_lens):
+        _refuse(q=q, block_table=block_table, kv_lens=kv_lens, q_lens=q_lens)
     if q.dim() != 4:
         raise ValueError(f"q must be 4-D (B, H, N, D), got shape {tuple(q.shape)}")
     if q.dtype != cache.dtype:

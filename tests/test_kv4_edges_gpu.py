@@ -99,10 +99,10 @@ def test_slots_outside_the_cache_are_skipped_and_recorded():
     assert (got[0, 0, :3] == 0).all() and (got[0, 0, 4:] == 0).all()
 
 
-@pytest.mark.parametrize("N", [1, 150])
-def test_pages_outside_the_pool_and_lengths_beyond_the_table_stay_in_bounds(N):
+@pytest.mark.parametrize("Hq,N", [(4, 1), (32, 150)])  # in units of 8 rows, and dense
+def test_pages_outside_the_pool_and_lengths_beyond_the_table_stay_in_bounds(Hq, N):
     cache, table, held = small(L=200)
-    q = rand((2, 4, N, 128), 1, torch.bfloat16).to(DEV)
+    q = rand((2, Hq, N, 128), 1, torch.bfloat16).to(DEV)
     good = gfa.attention_flash_gqa_kv4(q, cache, table, i32([200, 160]), causal=True)
     for page in (-1, cache.num_pages, 2 ** 31 - 1, -2 ** 31):
         bad = table.clone()
@@ -123,11 +123,12 @@ def test_pages_outside_the_pool_and_lengths_beyond_the_table_stay_in_bounds(N):
 
 # ------------------------------------------------------------------ masked places
 @pytest.mark.parametrize("D", [64, 512])
-@pytest.mark.parametrize("N", [2, 140])
-def test_non_finite_values_do_not_leave_the_rows_that_see_them(D, N):
+@pytest.mark.parametrize("Hq,Hkv,N", [(4, 2, 2), (32, 4, 240)])  # in units of 8 rows, and dense
+def test_non_finite_values_do_not_leave_the_rows_that_see_them(D, Hq, Hkv, N):
     """Tokens whose keys or values hold a NaN or an infinity: rows that see them are NaN in that group at
     least, the others are as if the tokens were not there."""
-    B, Hq, Hkv, L, page = 1, 4, 2, 300, 16
+    B, L, page = 1, 300, 16
+    G = Hq // Hkv
     cache = gfa.kv4_alloc(-(-L // page), Hkv, D, page, torch.bfloat16, DEV)
     table = scattered_table(B, -(-L // page), cache.num_pages, 1)
     k, v = (rand((B, Hkv, L, D), s, torch.bfloat16) for s in (1, 2))
@@ -147,14 +148,18 @@ def test_non_finite_values_do_not_leave_the_rows_that_see_them(D, N):
             continue
         assert torch.equal(o[:, :, :-1], clean[:, :, :-1])
         for h in range(Hq):
-            group = slice(0, 64) if h < 2 else slice(D - 64, D)
-            assert torch.isnan(o[0, h, -1, group]).all()
-    # outside the window
+            if h // G < 2:
+                group = slice(0, 64) if h // G == 0 else slice(D - 64, D)
+                assert torch.isnan(o[0, h, -1, group]).all()
+            else:
+                assert torch.equal(o[0, h, -1], clean[0, h, -1])
+    # outside the window of the rows from position 110 on
     vv, kk = v.clone(), k.clone()
     vv[0, :, 10], kk[0, :, 10] = math.nan, math.inf
     gfa.kv4_append(cache, kk.to(DEV), vv.to(DEV), slots_of(table, [0], L, [L], page))
     o = gfa.attention_flash_gqa_kv4(q, cache, table, i32([L]), causal=True, slide_size=100)
-    assert torch.isfinite(o).all()
+    sees = max(0, 110 - (L - N))
+    assert torch.isnan(o[:, :, :sees]).all() and torch.isfinite(o[:, :, sees:]).all()
 
 
 def test_a_query_that_is_not_finite_spoils_its_row_only():
@@ -204,10 +209,10 @@ def test_requests_may_share_pages_and_tables_may_be_views():
     assert torch.equal(o, same)
 
 
-@pytest.mark.parametrize("N", [1, 130])
-def test_query_layouts(N):
+@pytest.mark.parametrize("Hq,N", [(4, 1), (32, 130)])  # in units of 8 rows, and dense
+def test_query_layouts(Hq, N):
     cache, table, held = small(L=300)
-    base = rand((2, N, 4, 128), 1, torch.bfloat16).to(DEV)
+    base = rand((2, N, Hq, 128), 1, torch.bfloat16).to(DEV)
     want = gfa.attention_flash_gqa_kv4(base.transpose(1, 2).contiguous(), cache, table, i32([300, 131]), causal=True)
     views = [base.transpose(1, 2), torch.cat([base, base], -1)[..., :128].transpose(1, 2),
              torch.nn.functional.pad(base, (4, 4))[..., 4:-4].transpose(1, 2)]
@@ -215,8 +220,8 @@ def test_query_layouts(N):
         o = gfa.attention_flash_gqa_kv4(q, cache, table, i32([300, 131]), causal=True)
         assert torch.equal(o, want)
     one = base[:, :, :1].transpose(1, 2)
-    o = gfa.attention_flash_gqa_kv4(one.expand(2, 4, N, 128), cache, table, i32([300, 131]), causal=True)
-    o2 = gfa.attention_flash_gqa_kv4(one.repeat(1, 4, 1, 1), cache, table, i32([300, 131]), causal=True)
+    o = gfa.attention_flash_gqa_kv4(one.expand(2, Hq, N, 128), cache, table, i32([300, 131]), causal=True)
+    o2 = gfa.attention_flash_gqa_kv4(one.repeat(1, Hq, 1, 1), cache, table, i32([300, 131]), causal=True)
     assert torch.equal(o, o2)
 
 
@@ -251,7 +256,7 @@ def test_calls_on_two_streams_at_once():
 
 def test_captured_calls_follow_lengths_that_change():
     cache, table, held = small(L=2000, D=64)
-    q1, q2 = (rand((2, 4, n, 64), n, torch.bfloat16).to(DEV) for n in (1, 160))
+    q1, q2 = (rand((2, h, n, 64), n, torch.bfloat16).to(DEV) for h, n in ((4, 1), (32, 160)))
     lens, new = i32([10, 10]), i32([1, 1])
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
@@ -285,7 +290,7 @@ def test_two_runs_give_the_same_bits():
 def test_a_chunk_and_its_tokens_alone_agree():
     """The dense path of a chunk and the 8-row units of its single tokens see the same cache."""
     cache, table, held = small(L=500)
-    q = rand((2, 4, 64, 128), 1, torch.bfloat16).to(DEV)
+    q = rand((2, 64, 64, 128), 1, torch.bfloat16).to(DEV)
     whole = gfa.attention_flash_gqa_kv4(q, cache, table, i32([500, 100]), causal=True)
     for at in (0, 17, 63):
         one = gfa.attention_flash_gqa_kv4(q[:, :, at:at + 1], cache, table, i32([500 - 63 + at, 100 - 63 + at]), causal=True)

@@ -242,7 +242,7 @@ def test_attention_over_a_long_ragged_batch(D, dtype):
     check(q, cache, table, held, lens, None, True, 3000, scale=0.01)
 
 
-# ------------------------------------------------------------------ many rows: the dense path
+# ------------------------------------------------------------------ many rows
 CHUNKS = [
     # B, Hq, Hkv, N, lens, q_lens, page, causal, window
     (1, 4, 1, 130, [130], None, 64, True, 0),                        # a prompt with nothing before it
@@ -266,3 +266,19 @@ def test_chunks_within_the_rounding_bound(D, dtype, shape):
     for b in range(B):
         n = N if q_lens is None else q_lens[b]
         assert (o[b, :, n:] == 0).all() and torch.isinf(lse[b, :, n:]).all()
+
+
+# enough rows for the dense path (keys and values written out, tcgen05 forward) at every head_dim
+DENSE = [
+    (3, 32, 4, 150, [1000, 150, 301], [150, 77, 0], 16, True, 0),
+    (3, 32, 4, 160, [700, 160, 0], None, 64, True, 200),             # window, an empty request
+    (2, 64, 4, 140, [90, 600], [140, 130], 32, False, 0),
+    (4, 32, 4, 131, [256, 257, 131, 60], None, 128, True, 0),        # more rows than keys in the last one
+]
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("shape", DENSE, ids=lambda s: "B{}_H{}-{}_N{}_L{}_q{}_p{}_c{}_w{}".format(*s).replace(" ", ""))
+def test_wide_chunks_within_the_rounding_bound(D, dtype, shape):
+    test_chunks_within_the_rounding_bound(D, dtype, shape)

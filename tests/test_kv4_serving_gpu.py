@@ -33,7 +33,7 @@ def ints(*v):
     return torch.tensor(v, dtype=torch.int32, device=DEV)
 
 
-# new tokens of four rows: prompts long (the dense path) and short, decoding, drafts, a row that finishes
+# new tokens of four rows: prompts long and short, decoding, drafts, a row that finishes
 # and one that takes its place, a request that the pool has no pages for
 SCHEDULE = [
     ((150, 7, 0, 33), 150),
