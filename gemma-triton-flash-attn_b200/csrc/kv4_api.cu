@@ -434,13 +434,13 @@ extern "C" int gqafa_kv4_attend(const void* q, const long long* q_strides, const
   const long long capacity = static_cast<long long>(cols) * page_size;
   if (max_kv_len < 0) return fail(GQAFA_ERR_INVALID, "max_kv_len must be >= 0");
   if (max_kv_len == 0 || max_kv_len > capacity) max_kv_len = static_cast<int>(capacity);
-  const int win = causal ? window : 0;
+  const int win = causal && window < capacity ? window : 0;  // a window over all keys cuts none
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if ((rc = bind_device(st))) return rc;
   const int sms = sm_count();
   if (sms <= 0) return fail(GQAFA_ERR_CUDA, "cannot read the device's multiprocessor count");
   const AttendShape s = attend_shape(batch, heads_q, heads_kv, seqlen_q, head_dim, max_kv_len, win, sms);
-  if (s.units * (capacity / 64 + 2) > INT_MAX)
+  if (!s.dense_batch && s.units * (capacity / 64 + 2) > INT_MAX)
     return fail(GQAFA_ERR_INVALID, "B * H_Q * N times the block table's capacity out of range");
   const long long need = attend_workspace(s);
   if (workspace == nullptr || workspace_bytes < need)

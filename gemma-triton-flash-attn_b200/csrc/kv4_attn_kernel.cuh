@@ -37,6 +37,11 @@
 // rows. All warps share one reference maximum per row; a warp that meets a
 // larger score publishes its own for this tile, and only then are P and the
 // accumulators rescaled.
+// The ninth warp costs registers (96 a thread, two CTAs per SM, instead of 128),
+// but warp 0 issuing the copies between its own tiles delays the other seven:
+// 130 us against 106 at head_dim 512, 16 requests of 8K keys, 54 against 38 at
+// head_dim 128. A producer warpgroup that gives its registers away (104 for the
+// others) changed the first by 1 % and the second by -5 %.
 //
 // Split. The tiles of all (request, row tile, KV head) units form one list,
 // cut into equal contiguous shares, one per CTA: ragged lengths and a single
@@ -341,7 +346,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
   uint8_t* sQ = reinterpret_cast<uint8_t*>(sM + 2 * 8 * ROWS);         // [ROWS] rows of Q_PITCH bytes
   int* sSum = reinterpret_cast<int*>(sQ + C::Q_BYTES);                 // [NG][ROWS] sum of the integer query
   int2* sMask = reinterpret_cast<int2*>(sSum + C::SUMQ_BYTES / 4);     // [ROWS]: first key, number of keys
-  float* sScale = reinterpret_cast<float*>(sMask + ROWS);              // [ROWS]: log2 units of score per unit of MMA result
+  float* sScale = reinterpret_cast<float*>(sMask + ROWS);              // [ROWS]: log2 units per unit of MMA result
   int* sMost = reinterpret_cast<int*>(sScale + ROWS);                  // [ROWS]: largest |q|, as bits
   uint64_t* bars = reinterpret_cast<uint64_t*>(sMost + ROWS);
   __shared__ int scratch[40];
@@ -584,7 +589,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
           const uint32_t base = ring + slot * C::STAGE_BYTES + (blk - half * SB) * BB;
           const uint32_t codes = base + lane * 16, metas = base + NG * KV4_CODE_BYTES + gid * 4;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[kb][e] = 0.f;
+          for (int e = 0; e < 4; ++e) s[kb][e] = 0.f;
 #pragma unroll 4
           for (int g = 0; g < NG; ++g) {
             const uint4 w = lds128(codes + g * KV4_CODE_BYTES);
@@ -664,10 +669,18 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
         const int blk = warp + 8 * kb;
         if (blk >= nv) continue;
         float* v = s[kb];
+        bool seen[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) seen[e] = v[e] != -INFINITY;
         v[0] = ex2(v[0] - f0);
         v[1] = ex2(v[1] - f1);
         v[2] = ex2(v[2] - f0);
         v[3] = ex2(v[3] - f1);
+        if (edge) {  // P = 0 marks a masked key: one that is seen has at least the least normal number
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (seen[e] && v[e] == 0.f) v[e] = 1.17549435e-38f;
+        }
         l_run[0] += v[0] + v[2];
         l_run[1] += v[1] + v[3];
         float* d = P + (blk * ROWS + 2 * tig) * PP + perm;
@@ -715,7 +728,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
       // ---------------- values ----------------
       float wz[4];  // -sum (F + z) P' of this tile
 #pragma unroll
-        for (int e = 0; e < 4; ++e) wz[e] = 0.f;
+      for (int e = 0; e < 4; ++e) wz[e] = 0.f;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         wait_full();
@@ -736,6 +749,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
                       s3 = meta_scale(mv.y);
           float4 pr = *reinterpret_cast<const float4*>(prow + sblk * ROWS * PP);
           if constexpr (SPECIAL) {
+            const bool off0 = edge && pr.x == 0.f, off1 = edge && pr.y == 0.f;  // masked
+            const bool off2 = edge && pr.z == 0.f, off3 = edge && pr.w == 0.f;
             if (rescale) {
               const int w = (half * SB + sblk) & 7;
               const float from = raised[buf][w] ? M[w * ROWS + gid] : vold;
@@ -746,10 +761,10 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
               pr.w *= f;
             }
             // a masked token's scale may be anything (a slot never written): its product must be 0
-            pr.x = pr.x == 0.f ? 0.f : pr.x * s0;
-            pr.y = pr.y == 0.f ? 0.f : pr.y * s1;
-            pr.z = pr.z == 0.f ? 0.f : pr.z * s2;
-            pr.w = pr.w == 0.f ? 0.f : pr.w * s3;
+            pr.x = off0 ? 0.f : pr.x * s0;
+            pr.y = off1 ? 0.f : pr.y * s1;
+            pr.z = off2 ? 0.f : pr.z * s2;
+            pr.w = off3 ? 0.f : pr.w * s3;
           } else {
             pr.x *= s0;
             pr.y *= s1;
@@ -777,9 +792,9 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
         release();
       }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[j][e] += wz[e];
+        for (int e = 0; e < 4; ++e) acc[j][e] += wz[e];
       buf ^= 1;
     }
 
@@ -795,8 +810,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
       l1 += __shfl_xor_sync(0xffffffffu, l1, o);
     }
     if (gid == 0) {
-      if (warp == 0)
-        *reinterpret_cast<float2*>(xM + 2 * tig) = make_float2(mref[0], mref[1]);
+      if (warp == 0) *reinterpret_cast<float2*>(xM + 2 * tig) = make_float2(mref[0], mref[1]);
       *reinterpret_cast<float2*>(xL + warp * ROWS + 2 * tig) = make_float2(l0, l1);
     }
     // value-side slices: halve their number until one is left
@@ -807,20 +821,20 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
         const int lane_at = ((dg * live + (ks % live)) * 32 + lane) * 4;
         if (ks >= live && ks < 2 * live) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              *reinterpret_cast<float4*>(X + j * (NG * live * 128) + lane_at) =
-                  make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<float4*>(X + j * (NG * live * 128) + lane_at) =
+                make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
         }
         compute_barrier();
         if (ks < live) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float4 v = *reinterpret_cast<const float4*>(X + j * (NG * live * 128) + lane_at);
-              acc[j][0] += v.x;
-              acc[j][1] += v.y;
-              acc[j][2] += v.z;
-              acc[j][3] += v.w;
-            }
+          for (int j = 0; j < 4; ++j) {
+            const float4 v = *reinterpret_cast<const float4*>(X + j * (NG * live * 128) + lane_at);
+            acc[j][0] += v.x;
+            acc[j][1] += v.y;
+            acc[j][2] += v.z;
+            acc[j][3] += v.w;
+          }
         }
         compute_barrier();
       }
@@ -854,10 +868,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
           }
         } else {
           float* d = p.part_o + (static_cast<long long>(part) * ROWS + i) * D + dg * 64 + gid * 8;
-          *reinterpret_cast<float4*>(d) =
-              make_float4(acc[0][e], acc[0][2 + e], acc[1][e], acc[1][2 + e]);
-          *reinterpret_cast<float4*>(d + 4) =
-              make_float4(acc[2][e], acc[2][2 + e], acc[3][e], acc[3][2 + e]);
+          *reinterpret_cast<float4*>(d) = make_float4(acc[0][e], acc[0][2 + e], acc[1][e], acc[1][2 + e]);
+          *reinterpret_cast<float4*>(d + 4) = make_float4(acc[2][e], acc[2][2 + e], acc[3][e], acc[3][2 + e]);
           if (dg == 0 && gid == 0) p.part_ml[static_cast<long long>(part) * ROWS + i] = make_float2(m, l);
         }
       }

@@ -193,8 +193,9 @@ def attention_flash_gqa_kv4(q, cache: KV4Cache, block_table, kv_lens, causal=Fal
 
     Returns O shaped and typed like q (and, with return_lse, the fp32 natural-log
     LSE (B, H_Q, N), -inf where no key is seen). max_kv_len: an upper bound of
-    kv_lens known to the host, which sizes the launch (default: the block
-    table's capacity; a bound that is too low costs speed, not results)."""
+    kv_lens known to the host, which sizes the launch and the workspace (default:
+    the block table's capacity). It has to hold: the rows of a longer request
+    may be wrong, and ``device_status`` then returns 18."""
     if not _all_cuda(q, block_table, kv_lens, q_lens):
         _refuse(q=q, block_table=block_table, kv_lens=kv_lens, q_lens=q_lens)
     if q.dim() != 4:

@@ -253,7 +253,8 @@ GQAFA_API int gqafa_kv4_read(const void* pages, long long num_pages, const int* 
  * q_lens[b] on, and rows that see no key, get zeros (lse -inf). lse may be
  * NULL, else fp32 [batch, heads_q, seqlen_q]. max_kv_len is an upper bound of
  * kv_lens that the host knows (0: the block table's capacity); it sizes the
- * launch and the workspace, longer lengths are still attended whole.
+ * launch and the workspace. Where a request is longer all the same, no access
+ * leaves the buffers, but its rows may be wrong, and then status 18 is recorded.
  * workspace: gqafa_kv4_attend_workspace_size bytes, 256-byte aligned, any
  * contents, not shared by calls that overlap on the GPU. */
 GQAFA_API long long gqafa_kv4_attend_workspace_size(int batch, int heads_q, int heads_kv, int seqlen_q, int head_dim,

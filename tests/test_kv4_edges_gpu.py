@@ -162,6 +162,49 @@ def test_non_finite_values_do_not_leave_the_rows_that_see_them(D, Hq, Hkv, N):
     assert torch.isnan(o[:, :, :sees]).all() and torch.isfinite(o[:, :, sees:]).all()
 
 
+@pytest.mark.parametrize("D,dtype", [(64, torch.float16), (128, torch.bfloat16), (256, torch.float16),
+                                     (512, torch.bfloat16)], ids=ids)
+@pytest.mark.parametrize("Hq,N", [(4, 2), (32, 240)])  # in units of 8 rows, and dense
+@pytest.mark.parametrize("at", [0, 150, 298])
+def test_a_nan_that_is_seen_with_hardly_any_weight_is_seen(D, dtype, Hq, N, at):
+    """exp(-2 * 16 * sqrt(D)) is 0 in fp32 (the least is exp(-103)), but not in the formula: NaN times it is NaN."""
+    Hkv, L = 4, 300
+    cache = gfa.kv4_alloc(-(-L // 16), Hkv, D, 16, dtype, DEV)
+    table = scattered_table(1, -(-L // 16), cache.num_pages, 1)
+    k = torch.full((1, Hkv, L, D), 4.0, dtype=dtype)
+    v = rand((1, Hkv, L, D), 2, dtype)
+    k[:, :, at], v[:, :, at, 3] = -4.0, math.nan
+    gfa.kv4_append(cache, k.to(DEV), v.to(DEV), slots_of(table, [0], L, [L], 16))
+    q = torch.full((1, Hq, N, D), 4.0, dtype=dtype, device=DEV)
+    o = gfa.attention_flash_gqa_kv4(q, cache, table, i32([L]), causal=True)
+    sees = torch.arange(L - N, L) >= at
+    assert torch.isnan(o[0, :, sees, 3]).all()
+    assert torch.isfinite(o[0, :, ~sees]).all()
+
+
+@pytest.mark.parametrize("Hq", [4, 64])  # in units of 8 rows, and dense
+def test_a_window_of_any_length(Hq):
+    """Windows as long as the table and longer are none, also where rows lie before the first key."""
+    cache, table, _ = small(L=200)
+    lens, ql = i32([4, 200]), i32([40, 40])
+    q = rand((2, Hq, 40, 128), 1, torch.bfloat16).to(DEV)
+    want = gfa.attention_flash_gqa_kv4(q, cache, table, lens, causal=True, q_lens=ql)
+    for window in (table.shape[1] * 16, 2 ** 31 - 1):
+        assert torch.equal(gfa.attention_flash_gqa_kv4(q, cache, table, lens, causal=True, slide_size=window,
+                                                       q_lens=ql), want)
+    assert (want[0, :, :36] == 0).all() and (want[0, :, 36:] != 0).any()
+
+
+@pytest.mark.parametrize("Hq,N", [(4, 1), (32, 150)])  # in units of 8 rows, and dense
+def test_a_bound_that_does_not_hold_touches_one_request(Hq, N):
+    cache, table, _ = small(L=200)
+    q = rand((2, Hq, N, 128), 1, torch.bfloat16).to(DEV)
+    good = gfa.attention_flash_gqa_kv4(q, cache, table, i32([200, 160]), causal=True)
+    o = gfa.attention_flash_gqa_kv4(q, cache, table, i32([200, 160]), causal=True, max_kv_len=160)
+    assert torch.equal(o[1], good[1])
+    assert status() == LENGTH or torch.equal(o, good)
+
+
 def test_a_query_that_is_not_finite_spoils_its_row_only():
     cache, table, held = small(L=300)
     q = rand((2, 4, 3, 128), 1, torch.bfloat16).to(DEV)
