@@ -264,6 +264,8 @@ extern "C" int gqafa_kv4_plan(const int* kv_lens, const int* new_lens, const int
   if (batch <= 0 || max_new <= 0)
     return fail(GQAFA_ERR_INVALID, "sizes must be positive (B=%d max_new=%d)", batch, max_new);
   if ((rc = check_table(block_table, table_stride, cols, page_size))) return rc;
+  if (static_cast<long long>(batch) * cols > INT_MAX)
+    return fail(GQAFA_ERR_INVALID, "block_table: %d rows of %d columns out of range", batch, cols);
   if (num_free <= 0 || static_cast<long long>(num_free) * page_size > INT_MAX)
     return fail(GQAFA_ERR_INVALID, "free_pages: %d entries out of range (entries * page_size must be in 1..2^31-1)",
                 num_free);
@@ -336,8 +338,9 @@ extern "C" int gqafa_kv4_append(const void* k, const long long* k_strides, const
   const bool tiled = seqlen >= 16;
   // tokens, or the 16-token tiles that can hold them from any first slot
   const long long units = (tiled ? (seqlen + 30LL) / 16 * 16 : seqlen) * (head_dim / KV4_GROUP);
-  if (heads_kv > 65535 || batch > 65535 || (units + 63) / 64 > INT_MAX)
-    return fail(GQAFA_ERR_INVALID, "B (%d) and heads_kv (%d) must be at most 65535", batch, heads_kv);
+  if (heads_kv > 65535 || batch > 65535 || units > INT_MAX)
+    return fail(GQAFA_ERR_INVALID, "B (%d), heads_kv (%d) and tokens (%d) out of range (65535, 65535, 2^28)", batch,
+                heads_kv, seqlen);
   const dim3 grid(static_cast<unsigned>((units + 63) / 64), heads_kv, batch);
   const bool bf16 = dtype == GQAFA_DTYPE_BF16;
 #define GQAFA_LAUNCH(DIM)                                                                      \

@@ -39,7 +39,7 @@
 // accumulators rescaled.
 // The ninth warp costs registers (96 a thread, two CTAs per SM, instead of 128),
 // but warp 0 issuing the copies between its own tiles delays the other seven:
-// 130 us against 106 at head_dim 512, 16 requests of 8K keys, 54 against 38 at
+// 130 us against 106 at head_dim 512, 16 requests of 8K to 16K keys, 54 against 38 at
 // head_dim 128. A producer warpgroup that gives its registers away (104 for the
 // others) changed the first by 1 % and the second by -5 %.
 //

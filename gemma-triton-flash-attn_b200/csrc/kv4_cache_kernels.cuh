@@ -45,8 +45,12 @@ __device__ __forceinline__ Kv4Request kv4_request(const Kv4PlanParams& p, int b)
 
 // One CTA per request. Each CTA scans the page counts of all requests (a few
 // hundred integers from L2) instead of waiting for another CTA's prefix, so
-// the plan is a single launch without communication. Requests take free pages
-// in request order; one whose running total passes the free count is refused.
+// the plan is a single launch without communication: 2.6 us for 8 requests, 3.4
+// us for 256 with chunks of up to 512 tokens, the time of a launch and three
+// dependent loads (the tables' bytes take 0.3 us). The scans grow with the
+// square of the requests; 600 are read in three rounds of loads. Requests take
+// free pages in request order; one whose running total passes the free count is
+// refused.
 __global__ void __launch_bounds__(256) kv4_plan_kernel(const Kv4PlanParams p) {
   __shared__ long long warp_sum[8];
   __shared__ long long mine;  // (pages needed, pages given back) before this request
@@ -250,9 +254,10 @@ __device__ __forceinline__ uint32_t kv4_key_values(uint32_t c) {
 // Four lanes (a quad) hold one group of a token, 32 bytes of keys and 32 of
 // values each: the group's extremes are a shuffle reduction over packed pairs,
 // and nothing else is shared. The rows are loaded beside the slot, not behind
-// it. Bound by instructions (with eight lanes a group, the scale's arithmetic and
-// an index computed with divisions took 28 instructions a value, 65 us for 16384
-// tokens at head_dim 256). blockIdx: 64 (token, group) pairs, head, request.
+// it. Bound by instructions: 16384 tokens of 8 heads at head_dim 256 take 40 us,
+// 4.2 TB/s (with eight lanes a group, the scale's arithmetic and an index
+// computed with divisions took 28 instructions a value and 65 us). blockIdx: 64
+// (token, group) pairs, head, request.
 //
 // TILED (16 tokens or more): neighbouring quads take tokens whose slots end in
 // 2t, 2t+1, 2t+8, 2t+9 if the slots run on from the row's first one, so a warp's
@@ -355,7 +360,9 @@ __device__ __forceinline__ uint4 kv4_values(uint32_t codes, uint32_t meta) {
 // group, as stored; all loads in flight together) and writes 16 tokens x 64
 // values of each: 128 contiguous bytes per token. blockIdx.x: request, head and
 // 8 * UNITS (block, group) pairs; blockIdx.y: keys / values. Rows behind a
-// request's last token become zeros.
+// request's last token become zeros. Bound by the writes, 79 % of the bytes:
+// 16384 tokens of 8 heads at head_dim 256 take 36 us, 4.7 TB/s (key stores of 16
+// bytes, half a sector each: 42 us).
 //
 // For the ragged forward, whose MMAs also multiply masked keys' values by P = 0,
 // a token with a NaN among its values goes out with NaN keys and zero values:

@@ -130,6 +130,7 @@ def test_page_bytes(heads, dim, page, want):
 @pytest.mark.parametrize("over,code,msg", [
     (dict(B=0), _lib.GQAFA_ERR_INVALID, "positive"), (dict(max_new=0), _lib.GQAFA_ERR_INVALID, "positive"),
     (dict(page=40), _lib.GQAFA_ERR_UNSUPPORTED, "page_size"), (dict(cols=0), _lib.GQAFA_ERR_INVALID, "columns"),
+    (dict(B=2 ** 16, cols=2 ** 16), _lib.GQAFA_ERR_INVALID, "out of range"),
     (dict(F=0), _lib.GQAFA_ERR_INVALID, "free_pages"), (dict(F=2 ** 30), _lib.GQAFA_ERR_INVALID, "free_pages"),
     (dict(lens=None), _lib.GQAFA_ERR_INVALID, "kv_lens"), (dict(slots=FAKE + 2), _lib.GQAFA_ERR_INVALID, "slot_map"),
     (dict(stride=-1), _lib.GQAFA_ERR_INVALID, "stride")])
