@@ -252,6 +252,24 @@ def test_requests_may_share_pages_and_tables_may_be_views():
     assert torch.equal(o, same)
 
 
+def test_pages_behind_the_first_4_gib():
+    """The same tokens in a small cache and in the last pages of one of 8.5 GiB."""
+    Hkv, D, page, L, dtype = 4, 512, 256, 300, torch.bfloat16
+    k, v = (rand((1, Hkv, L, D), s, dtype).to(DEV) for s in (1, 2))
+    q = rand((1, 32, 130, D), 3, dtype).to(DEV)
+    got = []
+    for total, pages in ((2, [1, 0]), (16384, [16383, 8192])):
+        cache = gfa.kv4_alloc(total, Hkv, D, page, dtype, DEV)
+        table = i32([pages])
+        gfa.kv4_append(cache, k, v, slots_of(table, [0], L, [L], page))
+        got.append([*gfa.kv4_read(cache, table, i32([L]), L),
+                    gfa.attention_flash_gqa_kv4(q, cache, table, i32([L]), causal=True),
+                    gfa.attention_flash_gqa_kv4(q[:, :, :1], cache, table, i32([L]), causal=True)])
+    assert cache.pages.numel() > 2 ** 33
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("Hq,N", [(4, 1), (32, 130)])  # in units of 8 rows, and dense
 def test_query_layouts(Hq, N):
     cache, table, held = small(L=300)
