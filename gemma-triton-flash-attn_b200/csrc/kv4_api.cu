@@ -341,7 +341,7 @@ extern "C" int gqafa_kv4_append(const void* k, const long long* k_strides, const
   if (heads_kv > 65535 || batch > 65535 || units > INT_MAX)
     return fail(GQAFA_ERR_INVALID, "B (%d), heads_kv (%d) and tokens (%d) out of range (65535, 65535, 2^28)", batch,
                 heads_kv, seqlen);
-  const dim3 grid(static_cast<unsigned>((units + 63) / 64), heads_kv, batch);
+  const dim3 grid(static_cast<unsigned>((units + 127) / 128), heads_kv, batch);
   const bool bf16 = dtype == GQAFA_DTYPE_BF16;
 #define GQAFA_LAUNCH(DIM)                                                                      \
   if (tiled) {                                                                                 \

@@ -159,7 +159,7 @@ __device__ __forceinline__ constexpr float kv4_max_finite() {
   return BF16 ? 3.3895313892515355e38f : 65504.f;
 }
 
-// Pairwise maximum of 16-bit values that keeps NaNs.
+// Pairwise maximum and minimum of 16-bit values that keep NaNs.
 template <bool BF16>
 __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -169,29 +169,44 @@ __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
     asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-
-// Quantise this lane's two words (16 values) of a group whose other words are
-// held by the quad's three other lanes: the words as the cache holds them (keys
-// or values) and the group's meta word.
 template <bool BF16>
-__device__ __forceinline__ uint2 kv4_quantise(const uint4 raw0, const uint4 raw1, bool keys, uint32_t& meta) {
-  const uint32_t w[8] = {raw0.x, raw0.y, raw0.z, raw0.w, raw1.x, raw1.y, raw1.z, raw1.w};
-  // largest x and largest -x, in the halves of one word
-  constexpr uint32_t SIGNS = 0x80008000u;
-  uint32_t up = w[0], dn = w[0] ^ SIGNS;
+__device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (BF16)
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Quantise this lane's four words (32 values) of a group whose other words are
+// held by the neighbouring lane: the words as the cache holds them (keys or
+// values) and the group's meta word.
+template <bool BF16>
+__device__ __forceinline__ uint4 kv4_quantise(const uint4 (&raw)[4], bool keys, uint32_t& meta) {
+  uint32_t w[16];
 #pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    up = max2_nan<BF16>(up, w[i]);
-    dn = max2_nan<BF16>(dn, w[i] ^ SIGNS);
+  for (int i = 0; i < 4; ++i) {
+    w[4 * i] = raw[i].x;
+    w[4 * i + 1] = raw[i].y;
+    w[4 * i + 2] = raw[i].z;
+    w[4 * i + 3] = raw[i].w;
   }
-  uint32_t top = max2_nan<BF16>(__byte_perm(up, dn, 0x5410), __byte_perm(up, dn, 0x7632));
+  uint32_t up = w[0], dn = w[0];
 #pragma unroll
-  for (int o = 1; o < 4; o <<= 1) top = max2_nan<BF16>(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int i = 1; i < 16; ++i) {
+    up = max2_nan<BF16>(up, w[i]);
+    dn = min2_nan<BF16>(dn, w[i]);
+  }
+  // largest x and largest -x, in the halves of one word
+  dn ^= 0x80008000u;
+  uint32_t top = max2_nan<BF16>(__byte_perm(up, dn, 0x5410), __byte_perm(up, dn, 0x7632));
+  top = max2_nan<BF16>(top, __shfl_xor_sync(0xffffffffu, top, 1));
   const float most = kv4_max_finite<BF16>();
   float hi = unpack_lo<BF16>(top), lo = -unpack_hi<BF16>(top);
   if (!(hi <= most && lo >= -most && lo <= most && hi >= -most)) {  // an infinity or a NaN in the group
     meta = KV4_META_NAN;
-    return make_uint2(0, 0);
+    return make_uint4(0, 0, 0, 0);
   }
   hi = fmaxf(hi, 0.f);
   lo = fminf(lo, 0.f);
@@ -213,15 +228,21 @@ __device__ __forceinline__ uint2 kv4_quantise(const uint4 raw0, const uint4 raw1
   const float zf = static_cast<float>(z), zb = zf + EPS;
   meta = (__float_as_uint(s) >> 16) | z;
   const bool far = fmaxf(hi, -lo) > most - s;  // a code may pass the largest number
-  uint32_t word[2];
+  // hi's code is 16 where both ends of the range are ties: codes grow with x, so no other group has one
+  const bool over = fmaf(hi, inv, zb) + MAGIC > MAGIC + 15.f;
+  uint32_t word[4];
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  for (int u = 0; u < 4; ++u) {
     uint32_t c[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t v = w[4 * u + (i >> 1)];
       const float x = (i & 1) ? unpack_hi<BF16>(v) : unpack_lo<BF16>(v);
-      c[i] = __float_as_uint(fminf(fmaf(x, inv, zb) + MAGIC, MAGIC + 15.f));
+      c[i] = __float_as_uint(fmaf(x, inv, zb) + MAGIC);
+    }
+    if (over) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = __float_as_uint(fminf(__uint_as_float(c[i]), MAGIC + 15.f));
     }
     if (far) {
 #pragma unroll
@@ -239,7 +260,7 @@ __device__ __forceinline__ uint2 kv4_quantise(const uint4 raw0, const uint4 raw1
     const uint32_t odd = keys ? bytes(c[2], c[6], c[3], c[7]) : bytes(c[1], c[3], c[5], c[7]);
     word[u] = even | (odd << 4);
   }
-  return make_uint2(word[0], word[1]);
+  return make_uint4(word[0], word[1], word[2], word[3]);
 }
 
 // Key word order (nibble i: dim 2i, nibble 4+i: dim 2i+1) -> value order.
@@ -251,24 +272,21 @@ __device__ __forceinline__ uint32_t kv4_key_values(uint32_t c) {
   return c;
 }
 
-// Four lanes (a quad) hold one group of a token, 32 bytes of keys and 32 of
-// values each: the group's extremes are a shuffle reduction over packed pairs,
-// and nothing else is shared. The rows are loaded beside the slot, not behind
-// it. Bound by instructions: 16384 tokens of 8 heads at head_dim 256 take 40 us,
-// 4.2 TB/s (with eight lanes a group, the scale's arithmetic and an index
-// computed with divisions took 28 instructions a value and 65 us). blockIdx: 64
-// (token, group) pairs, head, request.
+// Two lanes hold one group of a token, two pieces of 32 bytes of the keys and of
+// the values each (words 2t, 2t+1 and 2t+4, 2t+5): the group's extremes are one
+// shuffle, and nothing else is shared. The rows are loaded beside the slot, not
+// behind it. blockIdx: 128 (token, group) pairs, head, request.
 //
-// TILED (16 tokens or more): neighbouring quads take tokens whose slots end in
-// 2t, 2t+1, 2t+8, 2t+9 if the slots run on from the row's first one, so a warp's
-// stores fill whole sectors.
+// TILED (16 tokens or more): a warp takes one group of 16 tokens, neighbouring
+// lane pairs those whose slots end in 2t, 2t+1, 2t+8, 2t+9 if the slots run on
+// from the row's first one, so a warp's stores fill whole sectors.
 template <int D, bool BF16, bool TILED>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p) {
   constexpr int NG = D / KV4_GROUP;
-  const int t = threadIdx.x & 3;
+  const int t = threadIdx.x & 1;
   const int blocks_shift = p.page_shift - 4;
   const int h = blockIdx.y, b = blockIdx.z;
-  unsigned rest = blockIdx.x * 64u + (threadIdx.x >> 2);
+  unsigned rest = blockIdx.x * 128u + (threadIdx.x >> 1);
   int n = 0;
   if constexpr (TILED) {
     const unsigned q = rest & 3, pair = (rest >> 2) & 3;
@@ -282,7 +300,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p
   } else {
     n = rest / NG;
   }
-  uint4 raw[2][2] = {};
+  uint4 raw[2][4] = {};
   int slot = -1;
   if (n >= 0 && n < p.N) {  // the shuffles need all lanes
     slot = p.slots[b * p.slots_stride + n];
@@ -292,6 +310,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p
                                                         g * KV4_GROUP + t * 16);
       raw[kind][0] = __ldcs(src);
       raw[kind][1] = __ldcs(src + 1);
+      raw[kind][2] = __ldcs(src + 4);
+      raw[kind][3] = __ldcs(src + 5);
     }
   }
   if (slot >= p.num_slots || slot < -1) {
@@ -305,14 +325,17 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p
 #pragma unroll
   for (int kind = 0; kind < 2; ++kind) {
     uint32_t meta;
-    const uint2 codes = kv4_quantise<BF16>(raw[kind][0], raw[kind][1], kind == 0, meta);
+    const uint4 codes = kv4_quantise<BF16>(raw[kind], kind == 0, meta);
     if (slot >= 0) {
       uint8_t* dst = page + (kind == 0 ? 0 : (static_cast<long long>(p.Hkv) << blocks_shift) * kv4_block_bytes(D));
       if (kind == 0) {
-        *reinterpret_cast<uint2*>(dst + g * KV4_CODE_BYTES + kv4_key_word(r, 2 * t)) = codes;
+        *reinterpret_cast<uint2*>(dst + g * KV4_CODE_BYTES + kv4_key_word(r, 2 * t)) = make_uint2(codes.x, codes.y);
+        *reinterpret_cast<uint2*>(dst + g * KV4_CODE_BYTES + kv4_key_word(r, 2 * t + 4)) = make_uint2(codes.z, codes.w);
       } else {
         *reinterpret_cast<uint32_t*>(dst + g * KV4_CODE_BYTES + kv4_value_word(r, 2 * t)) = codes.x;
         *reinterpret_cast<uint32_t*>(dst + g * KV4_CODE_BYTES + kv4_value_word(r, 2 * t + 1)) = codes.y;
+        *reinterpret_cast<uint32_t*>(dst + g * KV4_CODE_BYTES + kv4_value_word(r, 2 * t + 4)) = codes.z;
+        *reinterpret_cast<uint32_t*>(dst + g * KV4_CODE_BYTES + kv4_value_word(r, 2 * t + 5)) = codes.w;
       }
       if (t == 0)
         reinterpret_cast<uint16_t*>(dst + NG * KV4_CODE_BYTES + g * KV4_META_BYTES)[kind == 0 ? kv4_key_meta(r)
@@ -361,8 +384,11 @@ __device__ __forceinline__ uint4 kv4_values(uint32_t codes, uint32_t meta) {
 // values of each: 128 contiguous bytes per token. blockIdx.x: request, head and
 // 8 * UNITS (block, group) pairs; blockIdx.y: keys / values. Rows behind a
 // request's last token become zeros. Bound by the writes, 79 % of the bytes:
-// 16384 tokens of 8 heads at head_dim 256 take 36 us, 4.7 TB/s (key stores of 16
-// bytes, half a sector each: 42 us).
+// 16384 tokens of 8 heads at head_dim 256 take 36 us, 4.7 TB/s; a plain fill of as
+// many bytes as are written takes 38. (Key stores of 16 bytes, half a sector each:
+// 42 us. Two or eight groups a warp instead of four: 7 and 3 % more over five
+// ragged caches of up to 16384 tokens, 8 heads at head_dim 128.) Stores that the
+// L2 drops first took 72 us there instead of 75.
 //
 // For the ragged forward, whose MMAs also multiply masked keys' values by P = 0,
 // a token with a NaN among its values goes out with NaN keys and zero values:
@@ -442,15 +468,25 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
     };
     auto store = [&](int r, int j, uint32_t c, uint32_t m) {
       const long long i = pos0 + r - start;
-      if (i >= 0 && i < n) *reinterpret_cast<uint4*>(out + i * D + j * 8) = value(r, c, m);
+      if (i < 0 || i >= n) return;
+      uint4* at = reinterpret_cast<uint4*>(out + i * D + j * 8);
+      if constexpr (RAGGED)
+        *at = value(r, c, m);
+      else
+        __stcs(at, value(r, c, m));
     };
     auto store_pair = [&](int r, int t, uint32_t c0, uint32_t c1, uint32_t m) {
       const long long i = pos0 + r - start;
       if (i < 0 || i >= n) return;
       const uint4 v = value(r, c0, m), w = value(r, c1, m);
-      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + i * D + t * 16), "r"(v.x),
-                   "r"(v.y), "r"(v.z), "r"(v.w), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
-                   : "memory");
+      if constexpr (RAGGED)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + i * D + t * 16), "r"(v.x),
+                     "r"(v.y), "r"(v.z), "r"(v.w), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                     : "memory");
+      else
+        asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + i * D + t * 16),
+                     "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                     : "memory");
     };
     const uint2 m = metas[k];
     if (kind == 0) {
