@@ -341,7 +341,8 @@ extern "C" int gqafa_kv4_append(const void* k, const long long* k_strides, const
   if (heads_kv > 65535 || batch > 65535 || units > INT_MAX)
     return fail(GQAFA_ERR_INVALID, "B (%d), heads_kv (%d) and tokens (%d) out of range (65535, 65535, 2^28)", batch,
                 heads_kv, seqlen);
-  const dim3 grid(static_cast<unsigned>((units + 127) / 128), heads_kv, batch);
+  const int pairs = 256 / kv4_append_lanes(tiled);  // (token, group) pairs of a CTA
+  const dim3 grid(static_cast<unsigned>((units + pairs - 1) / pairs), heads_kv, batch);
   const bool bf16 = dtype == GQAFA_DTYPE_BF16;
 #define GQAFA_LAUNCH(DIM)                                                                      \
   if (tiled) {                                                                                 \

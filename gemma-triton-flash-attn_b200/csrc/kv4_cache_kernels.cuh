@@ -179,14 +179,15 @@ __device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
   return r;
 }
 
-// Quantise this lane's four words (32 values) of a group whose other words are
-// held by the neighbouring lane: the words as the cache holds them (keys or
-// values) and the group's meta word.
-template <bool BF16>
-__device__ __forceinline__ uint4 kv4_quantise(const uint4 (&raw)[4], bool keys, uint32_t& meta) {
-  uint32_t w[16];
+// Quantise this lane's W words (8 values each) of a group whose other words are
+// held by the 8 / W - 1 lanes beside it: the words as the cache holds them (keys
+// or values) and the group's meta word.
+template <bool BF16, int W>
+__device__ __forceinline__ void kv4_quantise(const uint4 (&raw)[W], bool keys, uint32_t (&word)[W], uint32_t& meta) {
+  uint32_t w[4 * W];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < W; ++i) {
+    word[i] = 0;
     w[4 * i] = raw[i].x;
     w[4 * i + 1] = raw[i].y;
     w[4 * i + 2] = raw[i].z;
@@ -194,19 +195,20 @@ __device__ __forceinline__ uint4 kv4_quantise(const uint4 (&raw)[4], bool keys, 
   }
   uint32_t up = w[0], dn = w[0];
 #pragma unroll
-  for (int i = 1; i < 16; ++i) {
+  for (int i = 1; i < 4 * W; ++i) {
     up = max2_nan<BF16>(up, w[i]);
     dn = min2_nan<BF16>(dn, w[i]);
   }
   // largest x and largest -x, in the halves of one word
   dn ^= 0x80008000u;
   uint32_t top = max2_nan<BF16>(__byte_perm(up, dn, 0x5410), __byte_perm(up, dn, 0x7632));
-  top = max2_nan<BF16>(top, __shfl_xor_sync(0xffffffffu, top, 1));
+#pragma unroll
+  for (int o = 1; o < 8 / W; o <<= 1) top = max2_nan<BF16>(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float most = kv4_max_finite<BF16>();
   float hi = unpack_lo<BF16>(top), lo = -unpack_hi<BF16>(top);
   if (!(hi <= most && lo >= -most && lo <= most && hi >= -most)) {  // an infinity or a NaN in the group
     meta = KV4_META_NAN;
-    return make_uint4(0, 0, 0, 0);
+    return;
   }
   hi = fmaxf(hi, 0.f);
   lo = fminf(lo, 0.f);
@@ -230,9 +232,8 @@ __device__ __forceinline__ uint4 kv4_quantise(const uint4 (&raw)[4], bool keys, 
   const bool far = fmaxf(hi, -lo) > most - s;  // a code may pass the largest number
   // hi's code is 16 where both ends of the range are ties: codes grow with x, so no other group has one
   const bool over = fmaf(hi, inv, zb) + MAGIC > MAGIC + 15.f;
-  uint32_t word[4];
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
+  for (int u = 0; u < W; ++u) {
     uint32_t c[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -260,7 +261,6 @@ __device__ __forceinline__ uint4 kv4_quantise(const uint4 (&raw)[4], bool keys, 
     const uint32_t odd = keys ? bytes(c[2], c[6], c[3], c[7]) : bytes(c[1], c[3], c[5], c[7]);
     word[u] = even | (odd << 4);
   }
-  return make_uint4(word[0], word[1], word[2], word[3]);
 }
 
 // Key word order (nibble i: dim 2i, nibble 4+i: dim 2i+1) -> value order.
@@ -272,21 +272,30 @@ __device__ __forceinline__ uint32_t kv4_key_values(uint32_t c) {
   return c;
 }
 
-// Two lanes hold one group of a token, two pieces of 32 bytes of the keys and of
-// the values each (words 2t, 2t+1 and 2t+4, 2t+5): the group's extremes are one
-// shuffle, and nothing else is shared. The rows are loaded beside the slot, not
-// behind it. blockIdx: 128 (token, group) pairs, head, request.
+__host__ __device__ constexpr int kv4_append_lanes(bool tiled) { return tiled ? 2 : 4; }
+
+// LANES neighbouring lanes hold one group of a token, lane t the words 2t, 2t+1
+// (and 2t+4, 2t+5 where there are two) of its keys and values: the group's
+// extremes are a shuffle reduction over packed pairs, and nothing else is shared.
+// The rows are loaded beside the slot, not behind it. blockIdx: 256 / LANES
+// (token, group) pairs, head, request.
 //
-// TILED (16 tokens or more): a warp takes one group of 16 tokens, neighbouring
-// lane pairs those whose slots end in 2t, 2t+1, 2t+8, 2t+9 if the slots run on
-// from the row's first one, so a warp's stores fill whole sectors.
+// TILED (16 tokens or more): two lanes, a warp takes one group of 16 tokens,
+// neighbouring pairs those whose slots end in 2t, 2t+1, 2t+8, 2t+9 if the slots run
+// on from the row's first one, so a warp's stores fill whole sectors. 16384 tokens
+// of 8 heads at head_dim 256 take 32.6 us, 5.2 TB/s; the scale's arithmetic and the
+// addresses, once a lane, made it bound by ALU instructions before: 40 us with four
+// lanes a group, 65 with eight and divisions. Fewer tokens take four lanes: 64
+// requests of one token, 4 heads at head_dim 512, 2.3 us, a launch and two
+// dependent loads, against 2.75 with two.
 template <int D, bool BF16, bool TILED>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p) {
   constexpr int NG = D / KV4_GROUP;
-  const int t = threadIdx.x & 1;
+  constexpr int LANES = kv4_append_lanes(TILED), W = 8 / LANES;
+  const int t = threadIdx.x % LANES;
   const int blocks_shift = p.page_shift - 4;
   const int h = blockIdx.y, b = blockIdx.z;
-  unsigned rest = blockIdx.x * 128u + (threadIdx.x >> 1);
+  unsigned rest = blockIdx.x * (256u / LANES) + threadIdx.x / LANES;
   int n = 0;
   if constexpr (TILED) {
     const unsigned q = rest & 3, pair = (rest >> 2) & 3;
@@ -300,7 +309,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p
   } else {
     n = rest / NG;
   }
-  uint4 raw[2][4] = {};
+  uint4 raw[2][W] = {};
   int slot = -1;
   if (n >= 0 && n < p.N) {  // the shuffles need all lanes
     slot = p.slots[b * p.slots_stride + n];
@@ -308,10 +317,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p
     for (int kind = 0; kind < 2; ++kind) {
       const uint4* src = reinterpret_cast<const uint4*>(p.x[kind] + b * p.sb[kind] + h * p.sh[kind] + n * p.sn[kind] +
                                                         g * KV4_GROUP + t * 16);
-      raw[kind][0] = __ldcs(src);
-      raw[kind][1] = __ldcs(src + 1);
-      raw[kind][2] = __ldcs(src + 4);
-      raw[kind][3] = __ldcs(src + 5);
+#pragma unroll
+      for (int i = 0; i < W; ++i) raw[kind][i] = __ldcs(src + (i & 1) + (i >> 1) * 4);
     }
   }
   if (slot >= p.num_slots || slot < -1) {
@@ -325,17 +332,20 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p
 #pragma unroll
   for (int kind = 0; kind < 2; ++kind) {
     uint32_t meta;
-    const uint4 codes = kv4_quantise<BF16>(raw[kind], kind == 0, meta);
+    uint32_t word[W];
+    kv4_quantise<BF16, W>(raw[kind], kind == 0, word, meta);
     if (slot >= 0) {
       uint8_t* dst = page + (kind == 0 ? 0 : (static_cast<long long>(p.Hkv) << blocks_shift) * kv4_block_bytes(D));
-      if (kind == 0) {
-        *reinterpret_cast<uint2*>(dst + g * KV4_CODE_BYTES + kv4_key_word(r, 2 * t)) = make_uint2(codes.x, codes.y);
-        *reinterpret_cast<uint2*>(dst + g * KV4_CODE_BYTES + kv4_key_word(r, 2 * t + 4)) = make_uint2(codes.z, codes.w);
-      } else {
-        *reinterpret_cast<uint32_t*>(dst + g * KV4_CODE_BYTES + kv4_value_word(r, 2 * t)) = codes.x;
-        *reinterpret_cast<uint32_t*>(dst + g * KV4_CODE_BYTES + kv4_value_word(r, 2 * t + 1)) = codes.y;
-        *reinterpret_cast<uint32_t*>(dst + g * KV4_CODE_BYTES + kv4_value_word(r, 2 * t + 4)) = codes.z;
-        *reinterpret_cast<uint32_t*>(dst + g * KV4_CODE_BYTES + kv4_value_word(r, 2 * t + 5)) = codes.w;
+      uint8_t* codes = dst + g * KV4_CODE_BYTES;
+#pragma unroll
+      for (int i = 0; i < W; i += 2) {
+        const int j = 2 * t + 2 * i;
+        if (kind == 0) {
+          *reinterpret_cast<uint2*>(codes + kv4_key_word(r, j)) = make_uint2(word[i], word[i + 1]);
+        } else {
+          *reinterpret_cast<uint32_t*>(codes + kv4_value_word(r, j)) = word[i];
+          *reinterpret_cast<uint32_t*>(codes + kv4_value_word(r, j + 1)) = word[i + 1];
+        }
       }
       if (t == 0)
         reinterpret_cast<uint16_t*>(dst + NG * KV4_CODE_BYTES + g * KV4_META_BYTES)[kind == 0 ? kv4_key_meta(r)
