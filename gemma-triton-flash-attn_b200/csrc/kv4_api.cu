@@ -205,20 +205,21 @@ int attend_dim(int D, const Kv4Params& p, cudaStream_t st) {
   }
 }
 
-template <bool RAGGED>
+// UNITS: (block, group) pairs a warp reads.
+template <bool RAGGED, int UNITS>
 int launch_read(Kv4ReadParams p, int head_dim, bool bf16, cudaStream_t st) {
   const int NG = head_dim / KV4_GROUP;
   // n tokens from any start touch at most (n + 15 + 15) / 16 blocks
   const long long items = ((p.n + 30LL) / 16) * NG;
-  const long long xblocks = (items + 8 * KV4_READ_UNITS - 1) / (8 * KV4_READ_UNITS), blocks = xblocks * p.B * p.Hkv;
+  const long long xblocks = (items + 8 * UNITS - 1) / (8 * UNITS), blocks = xblocks * p.B * p.Hkv;
   if (blocks > INT_MAX) return fail(GQAFA_ERR_INVALID, "grid size %lld out of range", blocks);
   p.xblocks = static_cast<int>(xblocks);
   const dim3 grid(static_cast<unsigned>(blocks), 2);
-#define GQAFA_LAUNCH(DIM)                                         \
-  if (bf16)                                                       \
-    kv4_read_kernel<DIM, true, RAGGED><<<grid, 256, 0, st>>>(p);  \
-  else                                                            \
-    kv4_read_kernel<DIM, false, RAGGED><<<grid, 256, 0, st>>>(p); \
+#define GQAFA_LAUNCH(DIM)                                                \
+  if (bf16)                                                              \
+    kv4_read_kernel<DIM, true, RAGGED, UNITS><<<grid, 256, 0, st>>>(p);  \
+  else                                                                   \
+    kv4_read_kernel<DIM, false, RAGGED, UNITS><<<grid, 256, 0, st>>>(p); \
   break
   switch (head_dim) {
     case 64: GQAFA_LAUNCH(64);
@@ -237,7 +238,8 @@ int check_attend(int batch, int heads_q, int heads_kv, int seqlen_q, int head_di
     return fail(GQAFA_ERR_INVALID, "sizes must be positive (B=%d H_Q=%d N=%d)", batch, heads_q, seqlen_q);
   if (heads_q % heads_kv != 0)
     return fail(GQAFA_ERR_INVALID, "H_Q (%d) must be a multiple of H_KV (%d)", heads_q, heads_kv);
-  if (static_cast<long long>(batch) * heads_q * seqlen_q > INT_MAX / 2)
+  if (static_cast<long long>(batch) * heads_q > INT_MAX ||
+      static_cast<long long>(batch) * heads_q * seqlen_q > INT_MAX / 2)
     return fail(GQAFA_ERR_INVALID, "B * H_Q * N out of range");
   return GQAFA_OK;
 }
@@ -370,6 +372,9 @@ extern "C" int gqafa_kv4_read(const void* pages, long long num_pages, const int*
   int rc;
   if ((rc = check_cache(heads_kv, head_dim, page_size, dtype))) return rc;
   if (batch <= 0 || seqlen <= 0) return fail(GQAFA_ERR_INVALID, "sizes must be positive (B=%d n=%d)", batch, seqlen);
+  if (static_cast<long long>(batch) * heads_kv > INT_MAX ||
+      static_cast<long long>(batch) * heads_kv * seqlen > (1LL << 40))
+    return fail(GQAFA_ERR_INVALID, "B * H_KV * n out of range");
   if ((rc = check_pages(pages, num_pages, page_size))) return rc;
   if ((rc = check_table(block_table, table_stride, cols, page_size))) return rc;
   if ((rc = check_ints("kv_lens", kv_lens))) return rc;
@@ -396,7 +401,16 @@ extern "C" int gqafa_kv4_read(const void* pages, long long num_pages, const int*
   p.num_pages = static_cast<int>(num_pages);
   p.status = status_ptr();
   if (!p.status) return fail(GQAFA_ERR_CUDA, "cannot resolve the device status word");
-  return launch_read<false>(p, head_dim, dtype == GQAFA_DTYPE_BF16, st);
+  // Few values: one group a warp, whose code is a quarter as long and comes in
+  // sooner (512 tokens, 4 heads, head_dim 512: 3.6 us against 4.6; one token of 64
+  // requests: 4.8 and 5.9). Many: more loads in flight per warp (1024 tokens: 5.0
+  // us against 5.3, 2048: 7.0 and 8.2).
+  const int sms = sm_count();
+  if (sms <= 0) return fail(GQAFA_ERR_CUDA, "cannot read the device's multiprocessor count");
+  const long long groups = 2LL * batch * heads_kv * seqlen * (head_dim / KV4_GROUP);  // of tokens
+  const bool bf16 = dtype == GQAFA_DTYPE_BF16;
+  return groups <= 256LL * sms ? launch_read<false, 1>(p, head_dim, bf16, st)
+                              : launch_read<false, KV4_READ_UNITS>(p, head_dim, bf16, st);
 }
 
 extern "C" long long gqafa_kv4_attend_workspace_size(int batch, int heads_q, int heads_kv, int seqlen_q, int head_dim,
@@ -476,7 +490,7 @@ extern "C" int gqafa_kv4_attend(const void* q, const long long* q_strides, const
       rd.q_lens = q_lens ? q_lens + b : nullptr;
       rd.out[0] = k;
       rd.out[1] = v;
-      if ((rc = launch_read<true>(rd, head_dim, bf16, st))) return rc;
+      if ((rc = launch_read<true, KV4_READ_UNITS>(rd, head_dim, bf16, st))) return rc;
       RaggedForward f{};
       f.q = static_cast<const uint16_t*>(q) + b * qs[0];
       f.q_strides = q_strides;

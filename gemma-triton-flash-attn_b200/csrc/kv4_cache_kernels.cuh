@@ -372,7 +372,7 @@ struct Kv4ReadParams {
   const int* q_lens;
 };
 
-constexpr int KV4_READ_UNITS = 4;  // groups of a block a warp reads
+constexpr int KV4_READ_UNITS = 4;  // groups of a block a warp reads, many of them
 
 // Eight values of a word as 16 bytes of 16-bit values, exactly s * (c - z).
 template <bool BF16>
@@ -403,7 +403,7 @@ __device__ __forceinline__ uint4 kv4_values(uint32_t codes, uint32_t meta) {
 // For the ragged forward, whose MMAs also multiply masked keys' values by P = 0,
 // a token with a NaN among its values goes out with NaN keys and zero values:
 // rows that see it become NaN, the others stay clean.
-template <int D, bool BF16, bool RAGGED>
+template <int D, bool BF16, bool RAGGED, int UNITS>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
   constexpr int NG = D / KV4_GROUP;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -423,14 +423,14 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
     if (r.Nk > p.n && threadIdx.x == 0) atomicCAS(p.status, 0, ST_KV4_LENGTH);  // beyond the given bound
     n = min(p.n, (r.Nk + 255) & ~255);
   }
-  const int item0 = ((blockIdx.x - bh * p.xblocks) * 8 + warp) * KV4_READ_UNITS;
+  const int item0 = ((blockIdx.x - bh * p.xblocks) * 8 + warp) * UNITS;
   const int blocks_shift = p.page_shift - 4;
   const long long end = static_cast<long long>(start) + n;
-  uint4 codes[KV4_READ_UNITS];
-  uint2 metas[KV4_READ_UNITS];
-  uint32_t bad[KV4_READ_UNITS];  // tokens with a NaN among their values
+  uint4 codes[UNITS];
+  uint2 metas[UNITS];
+  uint32_t bad[UNITS];  // tokens with a NaN among their values
 #pragma unroll
-  for (int k = 0; k < KV4_READ_UNITS; ++k) {
+  for (int k = 0; k < UNITS; ++k) {
     const int g = (item0 + k) % NG;
     const long long pos0 = (static_cast<long long>(start) / 16 + (item0 + k) / NG) * 16;  // first token of the block
     codes[k] = make_uint4(0, 0, 0, 0);
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
     }
   }
 #pragma unroll
-  for (int k = 0; k < KV4_READ_UNITS; ++k) {
+  for (int k = 0; k < UNITS; ++k) {
     const int g = (item0 + k) % NG;
     const long long pos0 = (static_cast<long long>(start) / 16 + (item0 + k) / NG) * 16;
     if (pos0 >= end) return;

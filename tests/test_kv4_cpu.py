@@ -161,18 +161,20 @@ def test_append_validation(over, code, msg):
 
 
 @pytest.mark.parametrize("over,code,msg", [
-    (dict(n=0), _lib.GQAFA_ERR_INVALID, "positive"), (dict(lens=None), _lib.GQAFA_ERR_INVALID, "kv_lens"),
+    (dict(n=0), _lib.GQAFA_ERR_INVALID, "positive"), (dict(B=2 ** 31 - 1, n=2 ** 31 - 1), _lib.GQAFA_ERR_INVALID, "range"),
+    (dict(lens=None), _lib.GQAFA_ERR_INVALID, "kv_lens"),
     (dict(k=FAKE + 16), _lib.GQAFA_ERR_INVALID, "32-byte"), (dict(v=None), _lib.GQAFA_ERR_INVALID, "outputs"),
     (dict(cols=2 ** 27), _lib.GQAFA_ERR_INVALID, "columns"), (dict(starts=FAKE + 1), _lib.GQAFA_ERR_INVALID, "starts")])
 def test_read_validation(over, code, msg):
-    a = dict(lens=FAKE, starts=None, k=FAKE, v=FAKE, cols=4, n=8) | over
-    rc = _lib.load().gqafa_kv4_read(FAKE, 9, FAKE, 4, a["cols"], a["lens"], a["starts"], a["k"], a["v"], 2, 2, a["n"], 64, 64,
-                                    1, None)
+    a = dict(lens=FAKE, starts=None, k=FAKE, v=FAKE, cols=4, n=8, B=2) | over
+    rc = _lib.load().gqafa_kv4_read(FAKE, 9, FAKE, 4, a["cols"], a["lens"], a["starts"], a["k"], a["v"], a["B"], 2, a["n"],
+                                    64, 64, 1, None)
     assert rc == code and msg in _message()
 
 
 @pytest.mark.parametrize("over,code,msg", [
-    (dict(Hq=5), _lib.GQAFA_ERR_INVALID, "multiple"), (dict(N=0), _lib.GQAFA_ERR_INVALID, "positive"),
+    (dict(Hq=5), _lib.GQAFA_ERR_INVALID, "multiple"), (dict(Hq=2 ** 31 - 2, N=2 ** 31 - 1), _lib.GQAFA_ERR_INVALID, "range"),
+    (dict(N=0), _lib.GQAFA_ERR_INVALID, "positive"),
     (dict(D=32), _lib.GQAFA_ERR_UNSUPPORTED, "head_dim"), (dict(page=17), _lib.GQAFA_ERR_UNSUPPORTED, "page_size"),
     (dict(scale=0.0), _lib.GQAFA_ERR_INVALID, "softmax_scale"), (dict(scale=math.nan), _lib.GQAFA_ERR_INVALID, "softmax_scale"),
     (dict(window=-1), _lib.GQAFA_ERR_INVALID, "window"), (dict(max_len=-1), _lib.GQAFA_ERR_INVALID, "max_kv_len"),
