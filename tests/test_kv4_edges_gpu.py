@@ -286,6 +286,36 @@ def test_query_layouts(Hq, N):
     assert torch.equal(o, o2)
 
 
+def test_the_cache_is_outside_autograd():
+    cache, table, _ = small(L=100)
+    k = rand((2, 2, 3, 128), 1, torch.bfloat16).to(DEV)
+    slots = i32([[0, 1, 2], [3, 4, -1]])
+    gfa.kv4_append(cache, k, k, slots)
+    want = cache.pages.clone()
+    gfa.kv4_append(cache, torch.zeros_like(k), torch.zeros_like(k), slots)
+    leaf = k.clone().requires_grad_()
+    gfa.kv4_append(cache, leaf * 1, leaf, slots)
+    assert torch.equal(cache.pages, want) and not cache.pages.requires_grad
+    for t in gfa.kv4_read(cache, table, i32([100, 50]), 100):
+        assert not t.requires_grad
+    with pytest.raises(NotImplementedError, match="backward"):
+        gfa.attention_flash_gqa_kv4(leaf, cache, table, i32([100, 50]))
+
+
+@pytest.mark.parametrize("n", [1, 5, 100, 1000])  # one group a warp, and four
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_read_of_few_and_many_rows(D, n):
+    B, H, L = 3, 7, 1000
+    cache, table, held = filled(B, H, D, L, 64, torch.bfloat16, 9)
+    lens, start = [L, 0, 37], [L - n, 0, 30]
+    for i, t in enumerate(gfa.kv4_read(cache, table, i32(lens), n, starts=i32(start))):
+        for b in range(B):
+            want = torch.zeros(H, n, D, dtype=torch.float64, device=DEV)
+            m = max(0, min(n, lens[b] - start[b]))
+            want[:, :m] = held[i][b, :, start[b]:start[b] + m]
+            assert torch.equal(t[b].double(), want)
+
+
 def test_read_from_any_start():
     cache, table, held = small(L=200, B=3)
     lens, starts = [200, 64, 5], [33, 64, 0]
