@@ -96,8 +96,12 @@ struct Kv4Params {
   int no_loads;
 };
 
-// Blocks per warp and tile: enough work between barriers at small head_dim.
-__host__ __device__ constexpr int kv4_warp_blocks(int D) { return D >= 256 ? 1 : (D == 128 ? 2 : 4); }
+// Blocks per warp and tile: enough work between barriers at small head_dim. 16
+// requests of 8K to 16K keys, 32/4 heads: 43.5 us with four at head_dim 128 (two:
+// 45.8, one: 49.6), 32.8 with four at 64 (two: 34.3; a tile has at most 32 blocks,
+// a lane of the producer each), 105.7 with one at 512 (two: 114.8); one token
+// over a window of 512 at 256: 10.3 with one (two: 11.5).
+__host__ __device__ constexpr int kv4_warp_blocks(int D) { return D >= 256 ? 1 : 4; }
 
 template <int D_, bool BF16_>
 struct Kv4Cfg {
