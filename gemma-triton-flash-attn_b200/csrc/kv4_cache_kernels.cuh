@@ -272,46 +272,30 @@ __device__ __forceinline__ uint32_t kv4_key_values(uint32_t c) {
   return c;
 }
 
-__host__ __device__ constexpr int kv4_append_lanes(bool tiled) { return tiled ? 2 : 4; }
-
 // LANES neighbouring lanes hold one group of a token, lane t the words 2t, 2t+1
-// (and 2t+4, 2t+5 where there are two) of its keys and values: the group's
+// (and 2t+4, 2t+5 where there are two lanes) of its keys and values: the group's
 // extremes are a shuffle reduction over packed pairs, and nothing else is shared.
 // The rows are loaded beside the slot, not behind it. blockIdx: 256 / LANES
 // (token, group) pairs, head, request.
 //
-// TILED (16 tokens or more): two lanes, a warp takes one group of 16 tokens,
-// neighbouring pairs those whose slots end in 2t, 2t+1, 2t+8, 2t+9 if the slots run
-// on from the row's first one, so a warp's stores fill whole sectors. 16384 tokens
-// of 8 heads at head_dim 256 take 32.6 us, 5.2 TB/s; the scale's arithmetic and the
-// addresses, once a lane, made it bound by ALU instructions before: 40 us with four
-// lanes a group, 65 with eight and divisions. Fewer tokens take four lanes: 64
-// requests of one token, 4 heads at head_dim 512, 2.3 us, a launch and two
-// dependent loads, against 2.75 with two.
-template <int D, bool BF16, bool TILED>
+// 16384 tokens of 8 heads at head_dim 256 take 31.2 us with two lanes, 5.4 TB/s;
+// the scale's arithmetic and the addresses, once per lane, made it bound by ALU
+// instructions before: 36 us with four lanes a group, 65 with eight and divisions.
+// (An order in which a warp takes the 16 tokens of a block, for stores of whole
+// sectors, waits for the row's first slot: 32.5.) Few tokens take four lanes, see
+// the launch.
+template <int D, bool BF16, int LANES>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p) {
   constexpr int NG = D / KV4_GROUP;
-  constexpr int LANES = kv4_append_lanes(TILED), W = 8 / LANES;
+  constexpr int W = 8 / LANES;
   const int t = threadIdx.x % LANES;
   const int blocks_shift = p.page_shift - 4;
   const int h = blockIdx.y, b = blockIdx.z;
-  unsigned rest = blockIdx.x * (256u / LANES) + threadIdx.x / LANES;
-  int n = 0;
-  if constexpr (TILED) {
-    const unsigned q = rest & 3, pair = (rest >> 2) & 3;
-    n = static_cast<int>(2 * pair + (q & 1) + 8 * (q >> 1));
-    rest >>= 4;
-  }
-  const int g = rest % NG;
-  if constexpr (TILED) {
-    const int first = p.slots[b * p.slots_stride];
-    n += static_cast<int>(rest / NG) * 16 - (first >= 0 ? first & 15 : 0);
-  } else {
-    n = rest / NG;
-  }
+  const unsigned pair = blockIdx.x * (256u / LANES) + threadIdx.x / LANES;
+  const int g = pair % NG, n = pair / NG;
   uint4 raw[2][W] = {};
   int slot = -1;
-  if (n >= 0 && n < p.N) {  // the shuffles need all lanes
+  if (n < p.N) {  // the shuffles need all lanes
     slot = p.slots[b * p.slots_stride + n];
 #pragma unroll
     for (int kind = 0; kind < 2; ++kind) {

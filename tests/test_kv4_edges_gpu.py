@@ -286,6 +286,37 @@ def test_query_layouts(Hq, N):
     assert torch.equal(o, o2)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=ids)
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_many_tokens_at_once_write_what_a_few_at_a_time_do(D, dtype):
+    """Two lanes a group against four: groups of all magnitudes, ties at both ends, infinities and NaNs."""
+    H, page = 8, 16
+    N = 64000 * 64 // (H * D) + 37
+    cols = -(-N // page)
+    table = scattered_table(1, cols, cols, 5)
+    slots = slots_of(table, [0], N, [N - 5], page)
+    k, v = (rand((1, H, N, D), s, torch.float32) for s in (1, 2))
+    top = 15 if dtype == torch.float16 else 126
+    k = k * torch.exp2(torch.randint(-top, top, (1, 1, N, D // 64), generator=torch.Generator().manual_seed(3))
+                       .float()).repeat_interleave(64, -1)
+    v[:, :, ::3] = (v[:, :, ::3] * 4).round().clamp(-15, 15) / 2  # many ties
+    v[:, :, ::7] = torch.where(v[:, :, ::7] > 0, 7.5, -7.5)       # both ends of the range
+    k, v = k.to(dtype), v.to(dtype)
+    v[0, 0, 11, 3], v[0, 1, 12, D - 1], k[0, 2, 13, D // 2] = math.nan, math.inf, -math.inf
+    k, v = k.to(DEV), v.to(DEV)
+    caches = [gfa.kv4_alloc(cols, H, D, page, dtype, DEV) for _ in range(2)]
+    for c in caches:
+        c.pages.fill_(0xA5)
+    gfa.kv4_append(caches[0], k, v, slots)
+    for i in range(0, N, 500):
+        gfa.kv4_append(caches[1], k[:, :, i:i + 500], v[:, :, i:i + 500], slots[:, i:i + 500])
+    assert torch.equal(caches[0].pages, caches[1].pages)
+    got = gfa.kv4_read(caches[0], table, i32([N - 5]), 200)
+    for x, y in zip(got, (k, v)):
+        want = kv4_ref.values(*kv4_ref.quantise(y[:, :, :200]))
+        assert torch.equal(torch.nan_to_num(x.double(), nan=1e300), torch.nan_to_num(want, nan=1e300))
+
+
 def test_the_cache_is_outside_autograd():
     cache, table, _ = small(L=100)
     k = rand((2, 2, 3, 128), 1, torch.bfloat16).to(DEV)
