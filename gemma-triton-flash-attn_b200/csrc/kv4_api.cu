@@ -40,7 +40,8 @@ int check_pages(const void* pages, long long num_pages, int page_size) {
   if (reinterpret_cast<uintptr_t>(pages) % 16 != 0)
     return fail(GQAFA_ERR_INVALID, "pages: data pointer must be 16-byte aligned");
   if (num_pages <= 0 || num_pages * page_size > INT_MAX)
-    return fail(GQAFA_ERR_INVALID, "num_pages %lld out of range (num_pages * page_size must be in 1..2^31-1)", num_pages);
+    return fail(GQAFA_ERR_INVALID, "num_pages %lld out of range (num_pages * page_size must be in 1..2^31-1)",
+                num_pages);
   return GQAFA_OK;
 }
 
@@ -70,8 +71,9 @@ int check_rows(const char* name, const void* ptr, const long long* st, int B, in
   for (int i = 0; i < 3; ++i) {
     out[i] = size[i] == 1 ? 0 : st[i];
     if ((size[i] > 1 && out[i] <= 0) || out[i] % 8 != 0)
-      return fail(GQAFA_ERR_INVALID, "%s: strides must be positive multiples of 8 elements (16 bytes), got (%lld, %lld, %lld, %lld)",
-                  name, st[0], st[1], st[2], st[3]);
+      return fail(GQAFA_ERR_INVALID,
+                  "%s: strides must be positive multiples of 8 elements (16 bytes), got (%lld, %lld, %lld, %lld)", name,
+                  st[0], st[1], st[2], st[3]);
   }
   return GQAFA_OK;
 }
@@ -97,6 +99,7 @@ int launch_status(const char* what) {
 struct AttendShape {
   int B, Hq, Hkv, N, D, G;
   int row_tiles, ctas, join_blocks;
+  bool wide;  // tiles of more blocks (kv4_warp_blocks)
   long long units;
   // Dense path (0 requests: not taken): rows of K and V, requests at a time.
   int dense_rows, dense_batch;
@@ -111,8 +114,8 @@ constexpr long long kDenseBytes = 2LL << 30;
 // forward of dense caches runs over them, with the lengths of each request. Its
 // CTAs (pairs at head_dim 512) take 128 tokens of one query head over all keys;
 // the MMAs above take 8 rows of all heads of a group and split the keys. Both
-// times grow with the keys: per key a unit of 8 rows costs the whole GPU 82, 52,
-// 30, 21 ps at head_dim 512, 256, 128, 64, a wave of 128-row tiles 20.6, 18.7,
+// times grow with the keys: per key a unit of 8 rows costs the whole GPU 82, 46,
+// 29, 21 ps at head_dim 512, 256, 128, 64, a wave of 128-row tiles 20.6, 18.7,
 // 16.4, 18.0 ns. Measured on both sides of the rule, 2 requests of 7K keys, 32/4
 // heads, head_dim 512: 24 tokens 141 us in units and 171 us dense, 48 tokens 240
 // and 172 us; 8 requests, 16/4 heads, head_dim 64: 48 tokens 120 and 147 us, 100
@@ -120,7 +123,7 @@ constexpr long long kDenseBytes = 2LL << 30;
 bool dense_path(int B, int Hq, int Hkv, int N, int D, int sms) {
   const long long units = static_cast<long long>(B) * Hkv * ((static_cast<long long>(Hq / Hkv) * N + 7) / 8);
   const long long tiles = static_cast<long long>(B) * Hq * ((N + 127) / 128) * (D == 512 ? 2 : 1);
-  const int ratio = D == 512 ? 250 : (D == 256 ? 360 : (D == 128 ? 550 : 860));
+  const int ratio = D == 512 ? 250 : (D == 256 ? 400 : (D == 128 ? 560 : 860));
   return units > ratio * ((tiles + sms - 1) / sms);
 }
 
@@ -136,12 +139,21 @@ AttendShape attend_shape(int B, int Hq, int Hkv, int N, int D, int max_len, int 
   s.G = Hq / Hkv;
   const long long rows = static_cast<long long>(s.G) * N;
   s.row_tiles = static_cast<int>((rows + 7) / 8);
-  const int tile_tokens = 8 * 16 * kv4_warp_blocks(D);
   long long span = max_len;
   if (window > 0) span = std::min<long long>(span, static_cast<long long>(window) + 8 / s.G + 1);
-  const long long tiles = (span + 15 + tile_tokens - 1) / tile_tokens + 1;
   s.units = static_cast<long long>(B) * s.row_tiles * Hkv;
-  s.ctas = static_cast<int>(std::min<long long>(2LL * sms, s.units * tiles));
+  auto tiles = [&](bool wide) {
+    const int tile_tokens = 8 * 16 * kv4_warp_blocks(D, wide);
+    return s.units * ((span + 15 + tile_tokens - 1) / tile_tokens + 1);
+  };
+  // Short tiles where each gets a CTA of its own: one token over a window of 512,
+  // 16/8 heads, 4 requests at head_dim 256 12.6 us against 13.7, at 128 11.6 and
+  // 12.8, at 64 10.4 and 11.4. Else long ones, fewer barriers: 8 requests at 256
+  // 15.2 us against 16.8, at 128 13.7 and 14.8; 16 requests of 8K to 16K keys, 32/4
+  // heads, at 256 65.3 and 69.7, at 128 43.5 and 49.6, at 64 32.8 and 34.3. At 512
+  // one block a warp is the best of both: with two, 114.8 us against 105.8.
+  s.wide = D != 512 && tiles(false) > 2LL * sms;
+  s.ctas = static_cast<int>(std::min<long long>(2LL * sms, tiles(s.wide)));
   // the join: at most two CTAs per SM, all of them where few units are cut into many parts
   s.join_blocks = 1;
   if (dense_path(B, Hq, Hkv, N, D, sms)) {
@@ -196,12 +208,14 @@ int launch_attend(Kv4Params p, cudaStream_t st) {
 }
 
 template <bool BF16>
-int attend_dim(int D, const Kv4Params& p, cudaStream_t st) {
+int attend_dim(int D, bool wide, const Kv4Params& p, cudaStream_t st) {
   switch (D) {
-    case 64: return launch_attend<Kv4Cfg<64, BF16>>(p, st);
-    case 128: return launch_attend<Kv4Cfg<128, BF16>>(p, st);
-    case 256: return launch_attend<Kv4Cfg<256, BF16>>(p, st);
-    default: return launch_attend<Kv4Cfg<512, BF16>>(p, st);
+    case 64: return wide ? launch_attend<Kv4Cfg<64, BF16, true>>(p, st) : launch_attend<Kv4Cfg<64, BF16, false>>(p, st);
+    case 128:
+      return wide ? launch_attend<Kv4Cfg<128, BF16, true>>(p, st) : launch_attend<Kv4Cfg<128, BF16, false>>(p, st);
+    case 256:
+      return wide ? launch_attend<Kv4Cfg<256, BF16, true>>(p, st) : launch_attend<Kv4Cfg<256, BF16, false>>(p, st);
+    default: return launch_attend<Kv4Cfg<512, BF16, false>>(p, st);
   }
 }
 
@@ -556,6 +570,6 @@ extern "C" int gqafa_kv4_attend(const void* q, const long long* q_strides, const
   if (!p.status) return fail(GQAFA_ERR_CUDA, "cannot resolve the device status word");
   p.wait_limit = wait_limit_setting();
   p.no_loads = no_loads_setting();
-  return dtype == GQAFA_DTYPE_BF16 ? attend_dim<true>(head_dim, p, st)
-                                   : attend_dim<false>(head_dim, p, st);
+  return dtype == GQAFA_DTYPE_BF16 ? attend_dim<true>(head_dim, s.wide, p, st)
+                                   : attend_dim<false>(head_dim, s.wide, p, st);
 }

@@ -39,9 +39,15 @@
 // accumulators rescaled.
 // The ninth warp costs registers (96 a thread, two CTAs per SM, instead of 128),
 // but warp 0 issuing the copies between its own tiles delays the other seven:
-// 130 us against 106 at head_dim 512, 16 requests of 8K to 16K keys, 54 against 38 at
-// head_dim 128. A producer warpgroup that gives its registers away (104 for the
-// others) changed the first by 1 % and the second by -5 %.
+// 130 us against 106 at head_dim 512, 16 requests of 8K to 16K keys, 54 against
+// 38 at head_dim 128. A producer warpgroup that gives its registers away (104 for the
+// others) made the first 1 % faster and the second 5 % slower.
+//
+// Measured: 16 requests of 8K to 16K keys, 32/4 heads, head_dim 512: 106 us for 430
+// MB of codes, 4.0 TB/s; 131072 keys of one request, 16/2 heads: 44.5 us, 3.2 TB/s.
+// Bound by neither alone: 58 % of the issue slots, 56 % of the ALU; without the
+// products the first takes 83 us. 20 rows at head_dim 128 (three units): 38 us,
+// bound by instructions.
 //
 // Split. The tiles of all (request, row tile, KV head) units form one list,
 // cut into equal contiguous shares, one per CTA: ragged lengths and a single
@@ -96,21 +102,20 @@ struct Kv4Params {
   int no_loads;
 };
 
-// Blocks per warp and tile: enough work between barriers at small head_dim. 16
-// requests of 8K to 16K keys, 32/4 heads: 43.5 us with four at head_dim 128 (two:
-// 45.8, one: 49.6), 32.8 with four at 64 (two: 34.3; a tile has at most 32 blocks,
-// a lane of the producer each), 105.7 with one at 512 (two: 114.8); one token
-// over a window of 512 at 256: 10.3 with one (two: 11.5).
-__host__ __device__ constexpr int kv4_warp_blocks(int D) { return D >= 256 ? 1 : 4; }
+// Blocks per warp and tile: enough work between barriers, or (wide false) tiles
+// that spread a few keys over more CTAs.
+__host__ __device__ constexpr int kv4_warp_blocks(int D, bool wide) {
+  return D == 512 ? 1 : (D == 256 ? (wide ? 2 : 1) : (D == 128 ? (wide ? 4 : 1) : (wide ? 4 : 2)));
+}
 
-template <int D_, bool BF16_>
+template <int D_, bool BF16_, bool WIDE_>
 struct Kv4Cfg {
   static constexpr int D = D_;
   static constexpr bool BF16 = BF16_;
   static constexpr int ROWS = 8;              // query rows of a unit
   static constexpr int NG = D / KV4_GROUP;    // groups of a token
   static constexpr int KS = 8 / NG;           // value-side slices of a tile's blocks
-  static constexpr int KB = kv4_warp_blocks(D);
+  static constexpr int KB = kv4_warp_blocks(D, WIDE_);
   static constexpr int TB = 8 * KB;           // blocks per tile
   static constexpr int SB = TB / 2;           // blocks per stage
   static constexpr int BLOCK_BYTES = kv4_block_bytes(D);

@@ -232,6 +232,20 @@ def test_attention_within_the_rounding_bound(D, dtype, shape):
         assert (o[b, :, n:] == 0).all() and torch.isinf(lse[b, :, n:]).all()
 
 
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("N,capacity", [(3, 704), (3, 65536), (40, 704)])  # short tiles, and long ones twice
+@pytest.mark.parametrize("window", [0, 300])
+def test_tiles_of_few_and_of_many_blocks(D, dtype, N, capacity, window):
+    """The length of a tile goes by the table's capacity and the rows: partial tiles at either end of both."""
+    B, Hkv, page = 5, 4, 16
+    cache, table, held = filled(B, Hkv, D, 700, page, dtype, 21)
+    wide = torch.full((B, capacity // page), -1, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    q = rand((B, 8, N, D), 7, dtype).to(DEV)
+    check(q, cache, wide, held, [700, 513, 1, 128, 0], [N, 1, N, 2, N], True, window)
+
+
 @pytest.mark.parametrize("D,dtype", [(64, torch.float16), (128, torch.bfloat16), (256, torch.float16),
                                      (512, torch.bfloat16)], ids=ids)
 def test_attention_over_a_long_ragged_batch(D, dtype):
