@@ -383,7 +383,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
   const int first_tile = static_cast<int>(begin);
   const int last_tile = min(share.total, first_tile + per);
 
-  // Walk the pieces of the share: f(unit, head, tile range inside the unit). Producer and compute warps walk the same way.
+  // Walk the pieces of the share: f(unit, head, tile range inside the unit).
+  // Producer and compute warps walk the same way.
   auto pieces = [&](auto&& f) {
     int entry = share.entry, base = share.base, at = first_tile;
     while (at < last_tile) {
@@ -507,8 +508,10 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
       }
     }
     auto load8 = [](const uint4& v, float (&x)[8]) {
-      x[0] = unpack_lo<BF16>(v.x), x[1] = unpack_hi<BF16>(v.x), x[2] = unpack_lo<BF16>(v.y), x[3] = unpack_hi<BF16>(v.y);
-      x[4] = unpack_lo<BF16>(v.z), x[5] = unpack_hi<BF16>(v.z), x[6] = unpack_lo<BF16>(v.w), x[7] = unpack_hi<BF16>(v.w);
+      x[0] = unpack_lo<BF16>(v.x), x[1] = unpack_hi<BF16>(v.x);
+      x[2] = unpack_lo<BF16>(v.y), x[3] = unpack_hi<BF16>(v.y);
+      x[4] = unpack_lo<BF16>(v.z), x[5] = unpack_hi<BF16>(v.z);
+      x[6] = unpack_lo<BF16>(v.w), x[7] = unpack_hi<BF16>(v.w);
     };
 #pragma unroll
     for (int k = 0; k < RN; ++k) {
