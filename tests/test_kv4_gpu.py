@@ -296,3 +296,14 @@ DENSE = [
 @pytest.mark.parametrize("shape", DENSE, ids=lambda s: "B{}_H{}-{}_N{}_L{}_q{}_p{}_c{}_w{}".format(*s).replace(" ", ""))
 def test_wide_chunks_within_the_rounding_bound(D, dtype, shape):
     test_chunks_within_the_rounding_bound(D, dtype, shape)
+
+
+@pytest.mark.parametrize("window", [0, 300])
+def test_chunks_of_more_requests_than_are_written_out_at_once(window):
+    """Keys and values of two requests of 131072 tokens' room fill 2 GiB: five requests take three turns."""
+    B, Hkv, D, page, N, capacity, dtype = 5, 4, 512, 256, 240, 131072, torch.bfloat16
+    cache, table, held = filled(B, Hkv, D, 600, page, dtype, 31)
+    wide = torch.full((B, capacity // page), -1, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    q = rand((B, 32, N, D), 8, dtype).to(DEV)
+    check(q, cache, wide, held, [600, 240, 513, 0, 257], [N, N, 7, 3, 130], True, window)
