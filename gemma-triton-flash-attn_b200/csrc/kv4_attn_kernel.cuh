@@ -21,6 +21,20 @@
 // are joined after every tile: F * sum(P') would otherwise outgrow the result
 // over a long cache and cost it its low bits.
 //
+// fp16 has not the exponents for s * P: with s = 3e-4 (values of 1e-3) and P =
+// 2^-3 it would begin among the subnormals and lose every weight below 2^-10 of
+// the largest. So P carries a power of two that brings the largest scale met so
+// far (of all groups) to the exponent of TOP, and the accumulators give it back
+// at the end: P' of the largest key is then at least 2^10 for the largest scale,
+// 24 powers of two above the least normal number, whatever the values' size.
+// (16384 keys of values near 0.02 with one score 9.7 above the others: 16 % of
+// the result were lost without it.) The warps look at the value blocks' scales
+// before a tile's barrier, a word per thread; a larger one is published as a
+// raised maximum is. That costs 109 us against 104 at head_dim 512, 16 requests of
+// 8K to 16K keys, 46.5 against 42.6 at 128 (each warp looking after its own groups
+// in the value loop, with a power for each: 113 and 49.5).
+// bf16 needs none of it.
+//
 // Shape. A decode step has G = H_Q / H_KV query rows per KV head, far below
 // the 128 rows of a tcgen05 tile, and reads each cached byte once: it is bound
 // by HBM. The products therefore run transposed on m16n8 MMAs with the
@@ -135,10 +149,15 @@ struct Kv4Cfg {
   // Reference of a row's softmax: its largest score so far plus RAISE when it
   // was last raised, and it is raised again when a score passes it by more than
   // SLACK (log2 units), so P stays within 2^SLACK. bf16 P' has the range for
-  // that; fp16 P' = s * P must stay below 65504 (s is at most 8736) and loses
-  // low bits below 2^-14.
+  // that; fp16 P' = s * P must stay below 65504, with s brought to at most
+  // 1.875 * 2^13 (TOP).
   static constexpr float RAISE = BF16 ? 8.f : 3.f;
-  static constexpr float SLACK = BF16 ? 8.f : 2.f;
+  static constexpr int SLACK2 = BF16 ? 8 : 2;
+  static constexpr float SLACK = SLACK2;
+  // fp16: exponent fields of the format's smallest and largest scales (2^-21 and
+  // 9216, the 4-bit number above 2 * 65504 / 15).
+  static constexpr int BOTTOM = 127 - 21, TOP = 127 + 13;
+  static_assert(BF16 || 1.875 * (1 << (TOP - 127)) * (1 << SLACK2) <= 65504 * 0.99, "P' stays finite");
   static_assert(NST >= 4, "two stages of keys and two of values");
   // the slices' sums are joined through the P buffers
   static_assert(KS == 1 || (KS / 2) * ROWS * D * 4 <= 2 * P_BYTES, "slice exchange");
@@ -312,6 +331,11 @@ template <bool BF16>
 __device__ __forceinline__ uint32_t minus_zero_odd(uint32_t w, const Kv4Tops& f) {
   return BF16 ? and_or(w, 0x000F000Fu, f.minus_even) : and_or(w << 6, 0x03C003C0u, f.minus_odd);
 }
+__device__ __forceinline__ uint32_t max2_u16(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 // Scale of the meta word in w's upper half.
 __device__ __forceinline__ float meta_scale(uint32_t w) { return __uint_as_float(w & 0xFFF00000u); }
 
@@ -473,10 +497,11 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
   const uint32_t qbase = smem_u32(sQ + gid * C::Q_PITCH + tig * 32);
   int slot = 0, buf = 0;  // next ring stage, P buffer
   uint32_t phase = 0;
-  auto wait_full = [&]() {
-    if (!mbar_try_wait(FULL(slot), phase)) kv4_wait_slow(FULL(slot), phase, abort_flag, p.status, p.wait_limit);
+  auto wait_at = [&](int s, uint32_t ph) {
+    if (!mbar_try_wait(FULL(s), ph)) kv4_wait_slow(FULL(s), ph, abort_flag, p.status, p.wait_limit);
     __syncwarp();
   };
+  auto wait_full = [&]() { wait_at(slot, phase); };
   // Gives the stage back and moves on. A warp that has nothing to read in a
   // key stage gives it back unseen: it cannot come round to the same stage
   // again before the others, there is a barrier in every tile and a tile is
@@ -570,6 +595,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
     compute_barrier();
     // keys that every row of the unit sees: [all_lo, all_hi) (what its padding rows see is not used)
     const int nlast = (min(r0 + ROWS, rows) - 1) / p.G;
+    const int any_hi = p.causal ? min(u.len, off + nlast + 1) : u.len;  // and keys that some row sees
+    const int any_lo = (p.causal && p.window > 0) ? max(0, off + r0 / p.G - p.window + 1) : 0;
     const int all_hi = p.causal ? min(u.len, off + r0 / p.G + 1) : u.len;
     const int all_lo = (p.causal && p.window > 0) ? max(0, off + nlast - p.window + 1) : 0;
 
@@ -583,6 +610,10 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
       for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
     mref[0] = mref[1] = -INFINITY;
     l_run[0] = l_run[1] = 0.f;
+    // fp16: exponent field of the largest scale so far; P and the accumulators
+    // hold 2^(TOP - top) times their values.
+    int top = C::BOTTOM;
+    auto power = [](int e) { return __int_as_float((127 + e) << 23); };
 
     for (int tile = t0; tile < t1; ++tile) {
       const int nv = min(TB, u.nblk - tile * TB);
@@ -630,6 +661,21 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
         release();
       }
 
+      // fp16: this thread's word (four tokens) of the tile's value scales; the
+      // loads are under way during the softmax
+      const int scale_blk = threadIdx.x / (NG * 4);
+      const uint32_t limit = top * 0x00800080u + 0x007F007Fu;
+      uint2 mv = make_uint2(0, 0);
+      if constexpr (!BF16) {
+        static_assert(TB * NG * 4 <= 256, "a word per thread");
+        const int slot1 = slot + 1 == NST ? 0 : slot + 1;
+        wait_full();
+        wait_at(slot1, slot1 == 0 ? phase ^ 1 : phase);
+        if (scale_blk < nv)
+          mv = lds64(ring + (scale_blk < SB ? slot : slot1) * C::STAGE_BYTES + scale_blk % SB * BB +
+                     NG * KV4_CODE_BYTES + threadIdx.x % (NG * 4) * 8);
+      }
+
       // ---------------- softmax over this warp's blocks ----------------
       float* P = sP + buf * (C::P_BYTES / 4);
       float* M = sM + buf * 8 * ROWS;
@@ -654,8 +700,29 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
         }
         above |= fmaxf(v[0], v[2]) > mref[0] + C::SLACK || fmaxf(v[1], v[3]) > mref[1] + C::SLACK;
       }
-      const bool raise = __any_sync(0xffffffffu, above);
-      if (lane == 0) raised[buf][warp] = raise;
+      bool raise, larger = false;
+      int mytop = top;
+      if constexpr (BF16) {
+        raise = __any_sync(0xffffffffu, above);
+      } else {
+        raise = __any_sync(0xffffffffu, above || max2_u16(max2_u16(mv.x, mv.y), limit) != limit);
+        if (raise) {
+          raise = __any_sync(0xffffffffu, above);
+          const uint32_t word[4] = {mv.x & 0xFFFFu, mv.x >> 16, mv.y & 0xFFFFu, mv.y >> 16};
+          const int key0 = key_tile + scale_blk * 16 + (threadIdx.x & 3) * 2;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = key0 + (j & 1) + (j >> 1) * 8;
+            // not a NaN's, nor that of a token that no row sees (which may be anything)
+            if (word[j] < 0x7F80u && (!edge || (key >= any_lo && key < any_hi)))
+              mytop = max(mytop, static_cast<int>(word[j] >> 7));
+          }
+          mytop = min(__reduce_max_sync(0xffffffffu, mytop), C::TOP);
+          larger = mytop != top;
+        }
+      }
+      // bit 0: a maximum is published; fp16: above it, the largest scale's exponent field
+      if (lane == 0) raised[buf][warp] = BF16 ? raise : 2 * mytop + raise;
       const int perm = (gid >> 1) * 4 + (gid & 1);  // order (2t, 2t+1, 2t+8, 2t+9) of the value side
       float f0 = mref[0], f1 = mref[1];
       if (raise) {
@@ -695,6 +762,10 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
         }
         l_run[0] += v[0] + v[2];
         l_run[1] += v[1] + v[3];
+        if constexpr (!BF16) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] *= power(C::TOP - mytop);
+        }
         float* d = P + (blk * ROWS + 2 * tig) * PP + perm;
         d[0] = v[0];
         d[2] = v[2];
@@ -702,15 +773,17 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
         d[PP + 2] = v[3];
       }
       // ---------------- new maxima, if any warp published some ----------------
-      const bool rescale = compute_barrier_or(raise);
+      const bool rescale = compute_barrier_or(raise || larger);
       // A warp's P refers to its own published maximum, or to the old one: in
       // the value loop row gid's factor brings it to the new one.
       float vold = 0.f, vnew = 0.f;
+      int newtop = top;
       if (rescale) {
         float m0 = mref[0], m1 = mref[1];
 #pragma unroll
         for (int w = 0; w < 8; ++w) {
-          if (raised[buf][w]) {
+          if (!BF16) newtop = max(newtop, raised[buf][w] >> 1);
+          if (raised[buf][w] & 1) {
             const float2 x = *reinterpret_cast<const float2*>(M + w * ROWS + 2 * tig);
             m0 = fmaxf(m0, x.x);
             m1 = fmaxf(m1, x.y);
@@ -720,7 +793,11 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
         if (raise) mine = *reinterpret_cast<const float2*>(M + warp * ROWS + 2 * tig);
         l_run[0] *= ex2(mine.x - finite_or_zero(m0));
         l_run[1] *= ex2(mine.y - finite_or_zero(m1));
-        const float a0 = ex2(mref[0] - finite_or_zero(m0)), a1 = ex2(mref[1] - finite_or_zero(m1));
+        float a0 = ex2(mref[0] - finite_or_zero(m0)), a1 = ex2(mref[1] - finite_or_zero(m1));
+        if constexpr (!BF16) {
+          a0 *= power(top - newtop);
+          a1 *= power(top - newtop);
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           acc[j][0] *= a0;
@@ -735,6 +812,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
         vnew = finite_or_zero((gid & 1) ? n1 : n0);
         mref[0] = m0;
         mref[1] = m1;
+        top = newtop;
       }
 
       // ---------------- values ----------------
@@ -743,7 +821,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
       for (int e = 0; e < 4; ++e) wz[e] = 0.f;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        wait_full();
+        if (BF16) wait_full();  // fp16: before the barrier
         const uint32_t stage = ring + slot * C::STAGE_BYTES;
         const uint32_t codes = stage + dg * KV4_CODE_BYTES + (tig * 8 + (gid ^ (2 * tig))) * 16;
         const uint32_t metas = stage + NG * KV4_CODE_BYTES + dg * KV4_META_BYTES + tig * 8;
@@ -765,8 +843,9 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
             const bool off2 = edge && pr.z == 0.f, off3 = edge && pr.w == 0.f;
             if (rescale) {
               const int w = (half * SB + sblk) & 7;
-              const float from = raised[buf][w] ? M[w * ROWS + gid] : vold;
-              const float f = ex2(finite_or_zero(from) - vnew);
+              const float from = (raised[buf][w] & 1) ? M[w * ROWS + gid] : vold;
+              float f = ex2(finite_or_zero(from) - vnew);
+              if (!BF16) f *= power((raised[buf][w] >> 1) - newtop);
               pr.x *= f;
               pr.y *= f;
               pr.z *= f;
@@ -811,6 +890,12 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
     }
 
     // ---------------- epilogue of the piece ----------------
+    if constexpr (!BF16) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][e] *= power(top - C::TOP);
+    }
     // every warp has the rows' maximum; the sums of the eight warps' l
     compute_barrier();  // all value-side reads of P and M are done
     float* xM = sM;             // [ROWS] maxima
