@@ -101,6 +101,7 @@ struct AttendShape {
   int row_tiles, ctas, join_blocks;
   bool wide;  // tiles of more blocks (kv4_warp_blocks)
   long long units;
+  long long part_ctas;  // room for the parts of this many CTAs: no call within the same lengths has more
   // Dense path (0 requests: not taken): rows of K and V, requests at a time.
   int dense_rows, dense_batch;
 };
@@ -128,7 +129,7 @@ bool dense_path(int B, int Hq, int Hkv, int N, int D, int sms) {
 }
 
 // Units of 8 query rows, and the CTAs of the launch: two per SM, fewer where there
-// are fewer tiles.
+// are fewer tiles. max_len 0: not known (a size call before the table is).
 AttendShape attend_shape(int B, int Hq, int Hkv, int N, int D, int max_len, int window, int sms) {
   AttendShape s{};
   s.B = B;
@@ -142,10 +143,13 @@ AttendShape attend_shape(int B, int Hq, int Hkv, int N, int D, int max_len, int 
   long long span = max_len;
   if (window > 0) span = std::min<long long>(span, static_cast<long long>(window) + 8 / s.G + 1);
   s.units = static_cast<long long>(B) * s.row_tiles * Hkv;
-  auto tiles = [&](bool wide) {
+  auto tiles_of = [&](bool wide, long long keys) {
     const int tile_tokens = 8 * 16 * kv4_warp_blocks(D, wide);
-    return s.units * ((span + 15 + tile_tokens - 1) / tile_tokens + 1);
+    return s.units * ((keys + 15 + tile_tokens - 1) / tile_tokens + 1);
   };
+  auto tiles = [&](bool wide) { return tiles_of(wide, span); };
+  // Short tiles and no window give the most CTAs, and more keys never fewer.
+  s.part_ctas = max_len > 0 ? std::min<long long>(2LL * sms, tiles_of(false, max_len)) : 2LL * sms;
   // Short tiles where each gets a CTA of its own: one token over a window of 512,
   // 16/8 heads, 4 requests at head_dim 256 12.6 us against 13.7, at 128 11.6 and
   // 12.8, at 64 10.4 and 11.4. Else long ones, fewer barriers: 8 requests at 256
@@ -156,7 +160,7 @@ AttendShape attend_shape(int B, int Hq, int Hkv, int N, int D, int max_len, int 
   s.ctas = static_cast<int>(std::min<long long>(2LL * sms, tiles(s.wide)));
   // the join: at most two CTAs per SM, all of them where few units are cut into many parts
   s.join_blocks = 1;
-  if (dense_path(B, Hq, Hkv, N, D, sms)) {
+  if (max_len > 0 && dense_path(B, Hq, Hkv, N, D, sms)) {
     long long held = max_len;
     if (window > 0) held = std::min<long long>(held, static_cast<long long>(window) + N + 15);
     s.dense_rows = static_cast<int>((std::max<long long>(held, 1) + 15) / 16 * 16);
@@ -169,9 +173,15 @@ AttendShape attend_shape(int B, int Hq, int Hkv, int N, int D, int max_len, int 
 
 // Dense path: K and V [dense_batch][Hkv][dense_rows][D] 16-bit. Else parts
 // [2 * ctas][8][D] fp32, their maxima and sums [2 * ctas][8].
+long long dense_bytes(const AttendShape& s) { return 4LL * s.Hkv * s.dense_rows * s.D; }  // of one request
+long long part_bytes(const AttendShape& s, long long ctas) { return 2 * ctas * 8 * (s.D * 4LL + 8) + 256; }
+// Both ways' room, and never less for more keys: a caller's bound may lie above
+// the table's capacity, which the launch then takes for it.
 long long attend_workspace(const AttendShape& s) {
-  if (s.dense_batch) return 4LL * s.dense_batch * s.Hkv * s.dense_rows * s.D + 256;
-  return 2LL * s.ctas * 8 * (static_cast<long long>(s.D) * 4 + 8) + 256;
+  long long need = part_bytes(s, s.part_ctas);
+  if (s.dense_batch)
+    need = std::max(need, s.dense_batch < s.B ? std::max(dense_bytes(s), kDenseBytes) : s.B * dense_bytes(s));
+  return need;
 }
 
 template <class C>
@@ -475,10 +485,14 @@ extern "C" int gqafa_kv4_attend(const void* q, const long long* q_strides, const
   if ((rc = bind_device(st))) return rc;
   const int sms = sm_count();
   if (sms <= 0) return fail(GQAFA_ERR_CUDA, "cannot read the device's multiprocessor count");
-  const AttendShape s = attend_shape(batch, heads_q, heads_kv, seqlen_q, head_dim, max_kv_len, win, sms);
+  AttendShape s = attend_shape(batch, heads_q, heads_kv, seqlen_q, head_dim, max_kv_len, win, sms);
+  // A workspace that was sized for other arguments (max_kv_len 0, a window that a
+  // call without causal does not use) may hold fewer requests at a time, or none:
+  // then the units take the call.
+  if (s.dense_batch) s.dense_batch = static_cast<int>(std::min<long long>(s.dense_batch, workspace_bytes / dense_bytes(s)));
   if (!s.dense_batch && s.units * (capacity / 64 + 2) > INT_MAX)
     return fail(GQAFA_ERR_INVALID, "B * H_Q * N times the block table's capacity out of range");
-  const long long need = attend_workspace(s);
+  const long long need = s.dense_batch ? s.dense_batch * dense_bytes(s) : part_bytes(s, s.ctas);
   if (workspace == nullptr || workspace_bytes < need)
     return fail(GQAFA_ERR_INVALID, "workspace of %lld bytes needed, got %lld", need, workspace_bytes);
   if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0)

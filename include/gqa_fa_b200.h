@@ -255,8 +255,13 @@ GQAFA_API int gqafa_kv4_read(const void* pages, long long num_pages, const int* 
  * kv_lens that the host knows (0: the block table's capacity); it sizes the
  * launch and the workspace. Where a request is longer all the same, no access
  * leaves the buffers, but its rows may be wrong, and then status 18 is recorded.
- * workspace: gqafa_kv4_attend_workspace_size bytes, 256-byte aligned, any
- * contents, not shared by calls that overlap on the GPU. */
+ * workspace: gqafa_kv4_attend_workspace_size bytes (called with the same sizes,
+ * and the same max_kv_len and window or larger ones; 0 stands for any length, a
+ * window counts only with causal), 256-byte aligned, any contents, not shared by
+ * calls that overlap on the GPU. Many query rows also want room for the keys and
+ * values of a request in 16 bits: the size call includes it for a max_kv_len
+ * above 0 (so pass cols * page_size there rather than 0, and window 0 without
+ * causal); in a workspace without it they take the slower way of few rows. */
 GQAFA_API long long gqafa_kv4_attend_workspace_size(int batch, int heads_q, int heads_kv, int seqlen_q, int head_dim,
                                                     int max_kv_len, int window);
 GQAFA_API int gqafa_kv4_attend(const void* q, const long long* q_strides, const void* pages, long long num_pages,

@@ -1,0 +1,77 @@
+"""gqafa_kv4_attend called as a C program calls it, with a workspace of the size that
+gqafa_kv4_attend_workspace_size gives for the documented arguments."""
+import pytest
+import torch
+
+import gemma_triton_flash_attn as gfa
+import kv4_ref
+from gemma_triton_flash_attn import _lib
+from test_kv4_gpu import DEV, filled, i32, rand
+
+pytestmark = pytest.mark.gpu
+
+
+def size_of(q, cache, max_kv_len, window):
+    B, Hq, N, D = q.shape
+    return _lib.load().gqafa_kv4_attend_workspace_size(B, Hq, cache.num_kv_heads, N, D, max_kv_len, window)
+
+
+def attend(q, cache, table, lens, max_kv_len, causal, window, workspace_bytes):
+    """Return code, O: the workspace is filled with NaNs and followed by bytes that must stay."""
+    B, Hq, N, D = q.shape
+    ws = torch.full((workspace_bytes + 4096,), 0xFF, dtype=torch.uint8, device=DEV)
+    o = torch.full_like(q, 7.0)
+    rc = _lib.load().gqafa_kv4_attend(
+        q.data_ptr(), _lib.strides_arg(q.stride()), cache.pages.data_ptr(), cache.num_pages, table.data_ptr(),
+        table.stride(0), table.shape[1], lens.data_ptr(), None, o.data_ptr(), _lib.strides_arg(o.stride()), None, B, Hq,
+        cache.num_kv_heads, N, D, cache.page_size, max_kv_len, D ** -0.5, int(causal), window, 1, ws.data_ptr(),
+        workspace_bytes, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert (ws[workspace_bytes:] == 0xFF).all()
+    return rc, o
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("B,Hq,Hkv,N,L", [(2, 8, 4, 1, 5000), (1, 32, 4, 1, 9400), (2, 64, 4, 140, 700),
+                                          (1, 64, 4, 140, 4700)])  # units of 8 rows, and dense
+@pytest.mark.parametrize("what", ["exact", "zero", "above", "window"])
+def test_workspaces_of_the_documented_size_are_enough(B, Hq, Hkv, N, L, what, D):
+    cache, table, held = filled(B, Hkv, D, L, 64, torch.bfloat16, 4)
+    q = rand((B, Hq, N, D), 2, torch.bfloat16).to(DEV)
+    lens, capacity = [L, L // 3][:B], table.shape[1] * 64
+    causal, window, max_kv_len = True, 0, capacity
+    size = size_of(q, cache, capacity, 0)
+    if what == "zero":  # the table's capacity
+        max_kv_len, size = 0, size_of(q, cache, 0, 0)
+    if what == "above":  # a bound that the table's capacity undercuts
+        bounds = [capacity + 1, capacity + 200, 2 * capacity, 8 * capacity, 1 << 20]
+        sizes = [size_of(q, cache, n, 0) for n in bounds]
+        assert sizes == sorted(sizes)
+        max_kv_len, size = bounds[1], sizes[1]
+    if what == "window":  # which counts only with causal
+        causal, window, size = False, 100, size_of(q, cache, capacity, 100)
+    assert size > 0
+    rc, o = attend(q, cache, table, i32(lens), max_kv_len, causal, window, size)
+    assert rc == _lib.GQAFA_OK, _lib.load().gqafa_last_error()
+    want, _, bound = kv4_ref.attention(q, *held, lens, [N] * B, causal, 0, D ** -0.5)
+    assert ((o.double() - want).abs() <= bound).all()
+    if what in ("exact", "above"):
+        same = gfa.attention_flash_gqa_kv4(q, cache, table, i32(lens), causal=causal)
+        assert torch.equal(o, same)
+    assert _lib.device_status(torch.cuda.current_device(), reset=True) == 0
+
+
+@pytest.mark.parametrize("N", [1, 140])
+def test_a_workspace_that_is_too_small_is_refused(N):
+    cache, table, _ = filled(1, 4, 128, 5000, 64, torch.bfloat16, 4)
+    q = rand((1, 64, N, 128), 2, torch.bfloat16).to(DEV)
+    for size in (0, 256, 4096):
+        rc, o = attend(q, cache, table, i32([5000]), 0, True, 0, size)
+        assert rc == _lib.GQAFA_ERR_INVALID and b"workspace" in _lib.load().gqafa_last_error()
+        assert (o == 7).all()
+
+
+def test_size_call_refuses_what_the_launch_refuses():
+    size = _lib.load().gqafa_kv4_attend_workspace_size
+    assert size(1, 8, 3, 1, 128, 100, 0) == -1 and size(1, 8, 4, 1, 96, 100, 0) == -1
+    assert size(1, 8, 4, 1, 128, -1, 0) == -1 and size(1, 8, 4, 1, 128, 100, -1) == -1
