@@ -731,7 +731,9 @@ __global__ void __launch_bounds__(256, 1)
       if constexpr (C::ROLE == ROLE_FWD) {
         if (p.lse != nullptr && orow < (C::RAGGED ? p.N : N)) {
           const float LN2 = 0.6931471805599453f;
-          p.lse[rowbase_q + orow] = (l_run > 0.f) ? (m_run + __log2f(l_run)) * LN2 : -INFINITY;
+          // ragged: a row that sees a NaN has a NaN for its sum, not none
+          const bool none = C::RAGGED ? l_run == 0.f : !(l_run > 0.f);
+          p.lse[rowbase_q + orow] = none ? -INFINITY : (m_run + __log2f(l_run)) * LN2;
         }
       }
     } else if (C::RAGGED && n_items == 0 && r0 + srow < p.N) {

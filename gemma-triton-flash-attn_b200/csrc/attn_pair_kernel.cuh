@@ -616,7 +616,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::THREADS, 1)
         }
         if (p.lse != nullptr && part == 0 && orow < (C::RAGGED ? p.N : N)) {
           const float LN2 = 0.6931471805599453f;
-          p.lse[rowbase_q + orow] = (l_tot > 0.f) ? (m_run + __log2f(l_tot)) * LN2 : -INFINITY;
+          // ragged: a row that sees a NaN has a NaN for its sum, not none
+          const bool none = C::RAGGED ? l_tot == 0.f : !(l_tot > 0.f);
+          p.lse[rowbase_q + orow] = none ? -INFINITY : (m_run + __log2f(l_tot)) * LN2;
         }
       } else if (C::RAGGED && n_items == 0 && r0 + row < p.N) {
         const long long obase = static_cast<long long>(b) * p.out_sb + static_cast<long long>(h) * p.out_sh +
