@@ -171,9 +171,13 @@ AttendShape attend_shape(int B, int Hq, int Hkv, int N, int D, int max_len, int 
   return s;
 }
 
-// Dense path: K and V [dense_batch][Hkv][dense_rows][D] 16-bit. Else parts
+// Dense path: K and V [dense_batch][Hkv][dense_rows][D] 16-bit, then the bits of
+// groups that are not finite [dense_batch][Hkv][nan_pitch]. Else parts
 // [2 * ctas][8][D] fp32, their maxima and sums [2 * ctas][8].
-long long dense_bytes(const AttendShape& s) { return 4LL * s.Hkv * s.dense_rows * s.D; }  // of one request
+int nan_pitch(const AttendShape& s) { return (s.dense_rows / KV4_TOKENS * (s.D / KV4_GROUP) + 7) / 8 * 8; }
+long long dense_bytes(const AttendShape& s) {  // of one request
+  return s.Hkv * (4LL * s.dense_rows * s.D + 2LL * nan_pitch(s));
+}
 long long part_bytes(const AttendShape& s, long long ctas) { return 2 * ctas * 8 * (s.D * 4LL + 8) + 256; }
 // Both ways' room, and never less for more keys: a caller's bound may lie above
 // the table's capacity, which the launch then takes for it.
@@ -253,6 +257,17 @@ int launch_read(Kv4ReadParams p, int head_dim, bool bf16, cudaStream_t st) {
   }
 #undef GQAFA_LAUNCH
   return launch_status("read");
+}
+
+int launch_spread(const Kv4SpreadParams& p, int head_dim, int batch, cudaStream_t st) {
+  const unsigned blocks = static_cast<unsigned>(batch) * p.Hkv;
+  switch (head_dim) {
+    case 64: kv4_spread_nan_kernel<64><<<blocks, 512, 0, st>>>(p); break;
+    case 128: kv4_spread_nan_kernel<128><<<blocks, 512, 0, st>>>(p); break;
+    case 256: kv4_spread_nan_kernel<256><<<blocks, 512, 0, st>>>(p); break;
+    default: kv4_spread_nan_kernel<512><<<blocks, 512, 0, st>>>(p);
+  }
+  return launch_status("4-bit cache NaN");
 }
 
 int check_attend(int batch, int heads_q, int heads_kv, int seqlen_q, int head_dim, int page_size, int dtype) {
@@ -506,7 +521,6 @@ extern "C" int gqafa_kv4_attend(const void* q, const long long* q_strides, const
     rd.table_stride = table_stride;
     rd.page_shift = log2_of(page_size);
     rd.num_pages = static_cast<int>(num_pages);
-    rd.ragged = 1;
     rd.q_rows = seqlen_q;
     rd.window = win;
     rd.status = status_ptr();
@@ -522,6 +536,8 @@ extern "C" int gqafa_kv4_attend(const void* q, const long long* q_strides, const
       rd.q_lens = q_lens ? q_lens + b : nullptr;
       rd.out[0] = k;
       rd.out[1] = v;
+      rd.nans = v + static_cast<long long>(nb) * heads_kv * s.dense_rows * head_dim;
+      rd.nan_pitch = nan_pitch(s);
       if ((rc = launch_read<true, KV4_READ_UNITS>(rd, head_dim, bf16, st))) return rc;
       RaggedForward f{};
       f.q = static_cast<const uint16_t*>(q) + b * qs[0];
@@ -545,6 +561,23 @@ extern "C" int gqafa_kv4_attend(const void* q, const long long* q_strides, const
       f.scale = softmax_scale;
       f.bf16 = bf16;
       if ((rc = ragged_forward(f, st))) return rc;
+      Kv4SpreadParams sp{};
+      sp.nans = rd.nans;
+      sp.nan_pitch = rd.nan_pitch;
+      sp.o = static_cast<uint16_t*>(f.o);
+      sp.o_sb = os[0];
+      sp.o_sh = os[1];
+      sp.o_sn = os[2];
+      sp.kv_lens = rd.kv_lens;
+      sp.q_lens = rd.q_lens;
+      sp.Hkv = heads_kv;
+      sp.G = s.G;
+      sp.N = seqlen_q;
+      sp.n = s.dense_rows;
+      sp.capacity = f.kv_cap;
+      sp.causal = f.causal;
+      sp.window = win;
+      if ((rc = launch_spread(sp, head_dim, nb, st))) return rc;
     }
     return GQAFA_OK;
   }

@@ -352,8 +352,12 @@ struct Kv4ReadParams {
   int* status;
   // For the ragged forward: the keys it reads (ragged_lens), and zeros only up
   // to the end of its last key block.
-  int ragged, q_rows, window;
+  int q_rows, window;
   const int* q_lens;
+  // tokens of each (block, group) whose values are not finite, a bit each:
+  // [B * Hkv][nan_pitch], item (block from `start` on) * NG + group
+  uint16_t* nans;
+  int nan_pitch;
 };
 
 constexpr int KV4_READ_UNITS = 4;  // groups of a block a warp reads, many of them
@@ -385,8 +389,8 @@ __device__ __forceinline__ uint4 kv4_values(uint32_t codes, uint32_t meta) {
 // L2 drops first took 72 us there instead of 75.
 //
 // For the ragged forward, whose MMAs also multiply masked keys' values by P = 0,
-// a token with a NaN among its values goes out with NaN keys and zero values:
-// rows that see it become NaN, the others stay clean.
+// a value group that is NaN goes out as zeros, and a bit of `nans` tells
+// kv4_spread_nan_kernel to mark the rows that see it.
 template <int D, bool BF16, bool RAGGED, int UNITS>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
   constexpr int NG = D / KV4_GROUP;
@@ -412,7 +416,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
   const long long end = static_cast<long long>(start) + n;
   uint4 codes[UNITS];
   uint2 metas[UNITS];
-  uint32_t bad[UNITS];  // tokens with a NaN among their values
+  uint32_t bad[UNITS];  // tokens whose values in this group are not finite
 #pragma unroll
   for (int k = 0; k < UNITS; ++k) {
     const int g = (item0 + k) % NG;
@@ -436,12 +440,12 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
       metas[k].x = __ldg(reinterpret_cast<const uint32_t*>(m + (lane >> 2) * 4));
     else
       metas[k] = __ldg(reinterpret_cast<const uint2*>(m + (lane >> 3) * 8));
-    if constexpr (RAGGED) {
-      const uint8_t* vals = src + (kind == 0 ? (static_cast<long long>(p.Hkv) << blocks_shift) * kv4_block_bytes(D) : 0);
-      const uint16_t* w = reinterpret_cast<const uint16_t*>(vals + NG * KV4_CODE_BYTES);
-      for (int e = lane; e < NG * KV4_TOKENS; e += 32) {
-        const int at = e & 15, r = (at >> 2) * 2 + (at & 1) + ((at >> 1) & 1) * 8;  // inverse of kv4_value_meta
-        if ((__ldg(w + e) & 0xFFF0u) == KV4_META_NAN) bad[k] |= 1u << r;
+    if (RAGGED && kind == 1) {
+      const uint32_t word[4] = {metas[k].x & 0xFFFFu, metas[k].x >> 16, metas[k].y & 0xFFFFu, metas[k].y >> 16};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = (lane >> 3) * 2 + (j & 1) + (j >> 1) * 8;  // inverse of kv4_value_meta
+        if ((word[j] & 0x7F80u) == 0x7F80u && pos0 + r < len) bad[k] |= 1u << r;
       }
       bad[k] = __reduce_or_sync(0xffffffffu, bad[k]);
     }
@@ -451,13 +455,12 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
     const int g = (item0 + k) % NG;
     const long long pos0 = (static_cast<long long>(start) / 16 + (item0 + k) / NG) * 16;
     if (pos0 >= end) return;
+    if (RAGGED && kind == 1 && lane == 0)
+      p.nans[static_cast<long long>(bh) * p.nan_pitch + item0 + k] = static_cast<uint16_t>(bad[k]);
     uint16_t* out = p.out[kind] + (static_cast<long long>(b) * p.Hkv + h) * p.n * D + g * KV4_GROUP;
     auto value = [&](int r, uint32_t c, uint32_t m) {
       if (pos0 + r >= len) return make_uint4(0, 0, 0, 0);
-      if (RAGGED && ((bad[k] >> r) & 1u)) {
-        const uint32_t x = kind == 0 ? 0x7FFF7FFFu : 0u;
-        return make_uint4(x, x, x, x);
-      }
+      if (RAGGED && ((bad[k] >> r) & 1u)) return make_uint4(0, 0, 0, 0);
       return kv4_values<BF16>(c, m);
     };
     auto store = [&](int r, int j, uint32_t c, uint32_t m) {
@@ -494,6 +497,60 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
       store(2 * t + 1, j, codes[k].y, m.x >> 16);
       store(2 * t + 8, j, codes[k].z, m.y & 0xFFFFu);
       store(2 * t + 9, j, codes[k].w, m.y >> 16);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ NaNs
+struct Kv4SpreadParams {
+  const uint16_t* nans;  // as in Kv4ReadParams
+  int nan_pitch;
+  uint16_t* o;
+  long long o_sb, o_sh, o_sn;
+  const int *kv_lens, *q_lens;
+  int Hkv, G, N, n, capacity, causal, window;  // n: rows of keys that were written out
+};
+
+// After the ragged forward: the dims of a value group that is not finite become
+// NaN in the rows that see its token, as P * NaN would make them. One CTA per
+// request and KV head; without such a group it reads the bits (16 KB for 16384
+// keys at head_dim 512) and leaves: a launch more, 48 tokens of 2 requests behind
+// 7K keys at head_dim 512 take 177.6 us instead of 172.0, 100 tokens of 8 at 64
+// 149.7 instead of 148.1.
+template <int D>
+__global__ void __launch_bounds__(512) kv4_spread_nan_kernel(const Kv4SpreadParams p) {
+  constexpr int NG = D / KV4_GROUP;
+  const int b = blockIdx.x / p.Hkv, h = blockIdx.x - b * p.Hkv;
+  const RaggedLens len = ragged_lens(p.kv_lens, p.q_lens, b, p.capacity, p.N, p.window);
+  const int Nk = min(len.Nk, p.n), off = Nk - len.N;
+  const uint16_t* nans = p.nans + static_cast<long long>(blockIdx.x) * p.nan_pitch;
+  const int items = (Nk + 15) / 16 * NG;
+  uint32_t any = 0;
+  for (int i = threadIdx.x * 8; i < items; i += 512 * 8) {
+    if (i + 8 <= items) {
+      const uint4 w = *reinterpret_cast<const uint4*>(nans + i);
+      any |= w.x | w.y | w.z | w.w;
+    } else {
+      for (int j = i; j < items; ++j) any |= nans[j];
+    }
+  }
+  if (!__syncthreads_or(any != 0)) return;
+  for (int at = threadIdx.x; at < len.N * NG; at += 512) {
+    const int n = at / NG, g = at - n * NG;
+    const int hi = p.causal ? min(Nk, n + off + 1) : Nk;
+    const int lo = (p.causal && p.window > 0) ? max(0, n + off - p.window + 1) : 0;
+    bool hit = false;
+    for (int blk = lo >> 4; !hit && blk * 16 < hi; ++blk) {
+      uint32_t bits = nans[blk * NG + g];
+      if (blk * 16 < lo) bits &= 0xFFFFu << (lo - blk * 16);
+      if (blk * 16 + 16 > hi) bits &= 0xFFFFu >> (blk * 16 + 16 - hi);
+      hit = bits != 0;
+    }
+    if (!hit) continue;
+    for (int i = 0; i < p.G; ++i) {
+      uint4* row = reinterpret_cast<uint4*>(p.o + b * p.o_sb + (h * p.G + i) * p.o_sh + n * p.o_sn + g * KV4_GROUP);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) row[j] = make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);
     }
   }
 }

@@ -189,7 +189,9 @@ def attention_flash_gqa_kv4(q, cache: KV4Cache, block_table, kv_lens, causal=Fal
     row r sits at kv_lens[b] - q_lens[b] + r. With ``causal`` a row sees the keys
     up to its own position, with ``slide_size > 0`` the last slide_size of
     them; without ``causal`` every row sees all keys. Rows from q_lens[b] on,
-    and rows that see no key, are zeros.
+    and rows that see no key, are zeros. Rows that see a key with a group that is
+    not finite are NaN, and so is their LSE; a value group that is not finite makes
+    its 64 dims NaN in the rows that see its token.
 
     Returns O shaped and typed like q (and, with return_lse, the fp32 natural-log
     LSE (B, H_Q, N), -inf where no key is seen). max_kv_len: an upper bound of

@@ -250,7 +250,9 @@ GQAFA_API int gqafa_kv4_read(const void* pages, long long num_pages, const int* 
  * the last of those positions: row r sits at kv_lens[b] - q_lens[b] + r. With
  * causal != 0 a row sees the keys up to its own position, and with window > 0
  * the last `window` of them; without causal every row sees all keys. Rows from
- * q_lens[b] on, and rows that see no key, get zeros (lse -inf). lse may be
+ * q_lens[b] on, and rows that see no key, get zeros (lse -inf). Rows that see a
+ * key with a group that is not finite get NaNs (lse too); a value group that is
+ * not finite makes its 64 dims NaN in the rows that see its token. lse may be
  * NULL, else fp32 [batch, heads_q, seqlen_q]. max_kv_len is an upper bound of
  * kv_lens that the host knows (0: the block table's capacity); it sizes the
  * launch and the workspace. Where a request is longer all the same, no access

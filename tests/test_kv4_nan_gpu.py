@@ -65,3 +65,45 @@ def test_a_key_that_is_not_finite_leaves_no_finite_weights(D, dtype, Hq, Hkv, N,
     assert hit.any()
     assert torch.isnan(o[hit]).all() and torch.isnan(lse[hit]).all()
     assert torch.equal(o[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_lse[~hit])
+
+
+@pytest.mark.parametrize("D,dtype", [(64, torch.bfloat16), (128, torch.float16), (256, torch.bfloat16),
+                                     (512, torch.bfloat16), (512, torch.float16)], ids=ids)
+@pytest.mark.parametrize("Hq,Hkv,N", PATHS)
+@pytest.mark.parametrize("causal,window", CASES)
+def test_a_value_group_that_is_not_finite_spoils_its_dims_only(D, dtype, Hq, Hkv, N, causal, window):
+    """P * NaN in the 64 dims of the group, in the rows that see the token; all else as if it were finite."""
+    B, L, lens, q_lens = 2, 500, [500, 261], [N, N - 2]
+    G, NG = Hq // Hkv, D // 64
+    k, v = rand((B, Hkv, L, D), 1, dtype), rand((B, Hkv, L, D), 2, dtype)
+    q = rand((B, Hq, N, D), 3, dtype).to(DEV)
+    clean, clean_lse = run(k, v, q, lens, q_lens, causal, window)
+    # the first token, one in the middle, a page's last, one that a single row sees, one behind the last
+    marks = [(0, 0, 0, 0), (0, 1, lens[0] - N // 2 - 1, NG - 1), (1, 0, 239, NG // 2), (1, 1, lens[1] - 1, 0),
+             (1, 1, 262, 0)]
+    hit = torch.zeros_like(clean, dtype=torch.bool)
+    for b, h, at, g in marks:
+        v[b, h, at, 64 * g + at % 64] = (math.nan, math.inf, -math.inf)[at % 3]
+        rows = sees(b, lens, q_lens, N, causal, window, at)
+        hit[b, h * G:(h + 1) * G, :, 64 * g:64 * g + 64] |= rows[None, :, None]
+    assert hit.any() and not hit.all()
+    o, lse = run(k, v, q, lens, q_lens, causal, window)
+    assert torch.equal(torch.isnan(o), hit)
+    assert torch.equal(lse, clean_lse)
+    if dtype == torch.bfloat16:
+        assert torch.equal(o[~hit], clean[~hit])
+    else:  # a group's scale that no longer counts may move the power of two that the weights carry
+        assert (o[~hit] - clean[~hit]).abs().max() <= 2 ** -10 * clean.abs().max()
+
+
+@pytest.mark.parametrize("Hq,Hkv,N", PATHS)
+def test_a_row_sees_the_same_nans_in_a_chunk_and_alone(Hq, Hkv, N):
+    B, L, D, dtype = 1, 400, 256, torch.bfloat16
+    k, v = rand((B, Hkv, L, D), 1, dtype), rand((B, Hkv, L, D), 2, dtype)
+    for at in range(3, L, 29):
+        v[0, at % Hkv, at, at % D] = math.nan
+    q = rand((B, Hq, N, D), 3, dtype).to(DEV)
+    o, _ = run(k, v, q, [L], [N], True, 25)
+    for row in (0, 1, N - 1):
+        one, _ = run(k, v, q[:, :, row:row + 1], [L - N + 1 + row], [1], True, 25)
+        assert torch.equal(torch.isnan(one), torch.isnan(o[:, :, row:row + 1]))
