@@ -8,7 +8,10 @@
 // operand as two signed bytes, round(q * 32512 / max|q|) = 256 hi + lo, off by
 // at most 2^-16 of its row's largest value. A group's part of a score is then
 // s * (256 q_hi . c + q_lo . c - z * sum(q)) with an exact integer in the
-// brackets; scales are applied in fp32. (16-bit operands took 28 ALU
+// brackets; scales are applied in fp32. A row whose largest value is more than 32
+// times its mean gets a third byte (2^-24 of the largest value) in a pass of its
+// own over the block: its other dims would lose their bits to that one (a channel
+// of 10000 that the keys do not use put 9 % on the output). (16-bit operands took 28 ALU
 // instructions per 16 tokens x 64 dims to make instead of 12, and the ALU is
 // the busiest pipe; fp8 MMAs of this shape are not native on sm_100.)
 //
@@ -137,12 +140,15 @@ struct Kv4Cfg {
   static constexpr int Q_PITCH = D * 2 + 16;  // bytes; +16: fragment loads hit all banks
   static constexpr int Q_BYTES = ROWS * Q_PITCH;
   static constexpr int SUMQ_BYTES = NG * ROWS * 4;
+  static constexpr int Q3_PITCH = D + 16;     // third bytes of the query
+  static constexpr int Q3_BYTES = ROWS * Q3_PITCH;
   static constexpr int P_PITCH = 20;          // floats of a row's 16 probabilities
   static constexpr int P_BYTES = TB * ROWS * P_PITCH * 4;  // one of two buffers
   static constexpr int M_BYTES = 8 * ROWS * 4;             // one of two buffers
-  static constexpr int MISC_BYTES = 2 * P_BYTES + 2 * M_BYTES + Q_BYTES + SUMQ_BYTES + ROWS * 16 + 256;
+  static constexpr int MISC_BYTES = 2 * P_BYTES + 2 * M_BYTES + Q_BYTES + Q3_BYTES + 2 * SUMQ_BYTES + ROWS * 20 + 256;
   static constexpr int CTAS_PER_SM = 2;
-  static constexpr int NST_FIT = (115000 - MISC_BYTES) / STAGE_BYTES;
+  // half of an SM's 228 KB, less 1 KB that a CTA takes and its static variables
+  static constexpr int NST_FIT = (115400 - MISC_BYTES) / STAGE_BYTES;
   static constexpr int NST = NST_FIT < 12 ? NST_FIT : 12;
   static constexpr int SMEM_BYTES = NST * STAGE_BYTES + MISC_BYTES;
   static constexpr int THREADS = 288;
@@ -365,6 +371,40 @@ __device__ __noinline__ void kv4_wait_slow(uint32_t bar, uint32_t parity, volati
   mbar_wait(bar, parity, abort_flag, status, ST_TIMEOUT_RING_FULL, limit);
 }
 
+// Adds what the query's third bytes give to a block's scores, times w0 and w1 for
+// the lane's two rows.
+template <int NG>
+__device__ __forceinline__ void kv4_third_bytes(float (&v)[4], uint32_t codes, uint32_t metas,
+                                                const uint8_t* query, const int* sums, float w0, float w1) {
+#pragma unroll 1
+  for (int g = 0; g < NG; ++g) {
+    const uint4 w = lds128(codes + g * KV4_CODE_BYTES);
+    const uint32_t m = lds32(metas + g * KV4_META_BYTES);
+    const uint4 q = lds128(smem_u32(query) + g * 64);
+    const int2 sq = *reinterpret_cast<const int2*>(sums + g * 8);
+    constexpr uint32_t M = 0x0F0F0F0Fu;
+    int t[4];
+    imma16832(t, w.x & M, w.z & M, (w.x >> 4) & M, (w.z >> 4) & M, q.x, q.y, 0, 0, 0, 0);
+    imma16832(t, w.y & M, w.w & M, (w.y >> 4) & M, (w.w >> 4) & M, q.z, q.w, t[0], t[1], t[2], t[3]);
+    const float s0 = meta_scale(m << 16), s1 = meta_scale(m);
+    const int z0 = m & 15, z1 = (m >> 16) & 15;
+    v[0] = fmaf(s0, static_cast<float>(t[0] - z0 * sq.x) * w0, v[0]);
+    v[1] = fmaf(s0, static_cast<float>(t[1] - z0 * sq.y) * w1, v[1]);
+    v[2] = fmaf(s1, static_cast<float>(t[2] - z1 * sq.x) * w0, v[2]);
+    v[3] = fmaf(s1, static_cast<float>(t[3] - z1 * sq.y) * w1, v[3]);
+  }
+}
+// Out of line where a warp has several blocks of a tile, each a copy of code that
+// few queries run: 46.5 us against 48.8 at head_dim 128, fp16; with one block
+// (head_dim 512) 109.5 against 107.7.
+template <int NG>
+__device__ __noinline__ float4 kv4_third_bytes_call(uint32_t codes, uint32_t metas, const uint8_t* query,
+                                                    const int* sums, float w0, float w1) {
+  float v[4] = {};
+  kv4_third_bytes<NG>(v, codes, metas, query, sums, w0, w1);
+  return make_float4(v[0], v[1], v[2], v[3]);
+}
+
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 
 template <class C>
@@ -377,11 +417,14 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
   float* sP = reinterpret_cast<float*>(smem + NST * C::STAGE_BYTES);  // [2][TB][ROWS][PP]
   float* sM = sP + 2 * C::P_BYTES / 4;                                 // [2][8 warps][ROWS]
   uint8_t* sQ = reinterpret_cast<uint8_t*>(sM + 2 * 8 * ROWS);         // [ROWS] rows of Q_PITCH bytes
-  int* sSum = reinterpret_cast<int*>(sQ + C::Q_BYTES);                 // [NG][ROWS] sum of the integer query
-  int2* sMask = reinterpret_cast<int2*>(sSum + C::SUMQ_BYTES / 4);     // [ROWS]: first key, number of keys
+  uint8_t* sQ3 = sQ + C::Q_BYTES;                                      // [ROWS] rows of Q3_PITCH bytes
+  int* sSum = reinterpret_cast<int*>(sQ3 + C::Q3_BYTES);               // [NG][ROWS] sum of the integer query
+  int* sSum3 = sSum + C::SUMQ_BYTES / 4;                               // [NG][ROWS] sum of the third bytes
+  int2* sMask = reinterpret_cast<int2*>(sSum3 + C::SUMQ_BYTES / 4);    // [ROWS]: first key, number of keys
   float* sScale = reinterpret_cast<float*>(sMask + ROWS);              // [ROWS]: log2 units per unit of MMA result
   int* sMost = reinterpret_cast<int*>(sScale + ROWS);                  // [ROWS]: largest |q|, as bits
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sMost + ROWS);
+  int* sAbs = sMost + ROWS;                                            // [ROWS]: sum of the integer query's magnitudes
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sAbs + ROWS);
   __shared__ int scratch[40];
   __shared__ __align__(16) int raised[2][8];  // warps that published a maximum for a tile
   __shared__ int abort_word;
@@ -495,6 +538,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
   const Kv4Tops tops = p.tops;
   const uint32_t ring = smem_u32(sRing);
   const uint32_t qbase = smem_u32(sQ + gid * C::Q_PITCH + tig * 32);
+  // Does row i take third bytes? 32512 * D / sAbs is its largest value over its mean.
+  auto wide_row = [&](int i) { return sMost[i] > 0 && sMost[i] < 0x7F800000 && sAbs[i] < 1016 * D; };
   int slot = 0, buf = 0;  // next ring stage, P buffer
   uint32_t phase = 0;
   auto wait_at = [&](int s, uint32_t ph) {
@@ -517,7 +562,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
 
   pieces([&](const Kv4Unit& u, int h, int t0, int t1) {
     // ---- queries of the unit, their sums per group, the rows' key ranges
-    if (threadIdx.x < ROWS) sMost[threadIdx.x] = 0;  // last read before the previous piece's last barrier
+    if (threadIdx.x < 2 * ROWS) sMost[threadIdx.x] = 0;  // and sAbs: last read before the previous piece's last barrier
     compute_barrier();  // the previous piece's readers are done
     const int r0 = u.rt * ROWS, rows = p.G * u.qlen, off = u.len - u.qlen;
     constexpr int CH = D / 8, RSTEP = 256 / CH, RN = (ROWS + RSTEP - 1) / RSTEP;
@@ -558,16 +603,23 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
       const float up = fminf(32512.f / most, 1e38f);  // 1e38 for a row of zeros: its integers are 0
       float x[8];
       load8(raw[k], x);
-      int v[8], sum = 0;
+      int v[8], third[8], sum = 0, sum3 = 0, abs = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         v[e] = __float2int_rn(x[e] * up);
+        third[e] = min(__float2int_rn(fmaf(x[e], up, -static_cast<float>(v[e])) * 256.f), 127);
         sum += v[e];
+        sum3 += third[e];
+        abs += v[e] < 0 ? -v[e] : v[e];
       }
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      for (int o = 1; o < 8; o <<= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        sum3 += __shfl_xor_sync(0xffffffffu, sum3, o);
+        abs += __shfl_xor_sync(0xffffffffu, abs, o);
+      }
       if (i < ROWS) {
-        uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
+        uint32_t hi[2] = {0, 0}, lo[2] = {0, 0}, lo3[2] = {0, 0};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           // byte order of a word's nibbles: even ones dims 0, 4, 1, 5, odd ones 2, 6, 3, 7
@@ -575,9 +627,15 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
           const int vh = (v[e] + 128) >> 8;
           hi[reg] |= (static_cast<uint32_t>(vh) & 0xFFu) << (8 * byte);
           lo[reg] |= (static_cast<uint32_t>(v[e] - (vh << 8)) & 0xFFu) << (8 * byte);
+          lo3[reg] |= (static_cast<uint32_t>(third[e]) & 0xFFu) << (8 * byte);
         }
+        *reinterpret_cast<uint2*>(sQ3 + i * C::Q3_PITCH + qc * 8) = make_uint2(lo3[0], lo3[1]);
         *reinterpret_cast<uint4*>(sQ + i * C::Q_PITCH + qc * 16) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
-        if ((qc & 7) == 0) sSum[(qc >> 3) * ROWS + i] = sum;
+        if ((qc & 7) == 0) {
+          sSum[(qc >> 3) * ROWS + i] = sum;
+          sSum3[(qc >> 3) * ROWS + i] = sum3;
+          if (bits < 0x7F800000) atomicAdd(&sAbs[i], abs);
+        }
         // a row with an infinity or a NaN has no finite scores
         if (qc == 0) sScale[i] = bits >= 0x7F800000 ? NAN : p.scale_log2 * (most / 32512.f);
       }
@@ -593,6 +651,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
       sMask[threadIdx.x] = make_int2(lo, max(0, hi - lo));
     }
     compute_barrier();
+    const bool wide = __any_sync(0xffffffffu, wide_row(lane & 7));
     // keys that every row of the unit sees: [all_lo, all_hi) (what its padding rows see is not used)
     const int nlast = (min(r0 + ROWS, rows) - 1) / p.G;
     const int any_hi = p.causal ? min(u.len, off + nlast + 1) : u.len;  // and keys that some row sees
@@ -656,6 +715,20 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
             v[1] = fmaf(s0, static_cast<float>(th[1] * 256 + (tl[1] - z0 * sq.y)), v[1]);
             v[2] = fmaf(s1, static_cast<float>(th[2] * 256 + (tl[2] - z1 * sq.x)), v[2]);
             v[3] = fmaf(s1, static_cast<float>(th[3] * 256 + (tl[3] - z1 * sq.y)), v[3]);
+          }
+          if (wide) {
+            const float w0 = wide_row(2 * tig) ? 0x1p-8f : 0.f, w1 = wide_row(2 * tig + 1) ? 0x1p-8f : 0.f;
+            const uint8_t* third = sQ3 + gid * C::Q3_PITCH + tig * 16;
+            const int* sums = sSum3 + 2 * tig;
+            if constexpr (KB == 1) {
+              kv4_third_bytes<NG>(s[kb], codes, metas, third, sums, w0, w1);
+            } else {
+              const float4 t = kv4_third_bytes_call<NG>(codes, metas, third, sums, w0, w1);
+              s[kb][0] += t.x;
+              s[kb][1] += t.y;
+              s[kb][2] += t.z;
+              s[kb][3] += t.w;
+            }
           }
         }
         release();

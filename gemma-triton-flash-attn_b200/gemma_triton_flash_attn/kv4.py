@@ -193,6 +193,11 @@ def attention_flash_gqa_kv4(q, cache: KV4Cache, block_table, kv_lens, causal=Fal
     not finite are NaN, and so is their LSE; a value group that is not finite makes
     its 64 dims NaN in the rows that see its token.
 
+    Scores, softmax and sums are held in 32 bits. Few rows: the query enters the
+    scores to 2^-16 of its row's largest value (2^-24 where that is more than 32
+    times the mean), and weight times scale the sums in 16 bits; many rows: the
+    weights in 16 bits. Keys or values beyond 2^96 may overflow the sums.
+
     Returns O shaped and typed like q (and, with return_lse, the fp32 natural-log
     LSE (B, H_Q, N), -inf where no key is seen). max_kv_len: an upper bound of
     kv_lens known to the host, which sizes the launch and the workspace (default:

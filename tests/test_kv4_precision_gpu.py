@@ -159,3 +159,49 @@ def test_fp16_values_over_the_whole_range_under_growing_scores(D):
     for step in (3.3 / 2500, 3.46 / 1500, 3.6 / 1000, 0.02):  # 5 in log2 units is 3.4657 in score
         k = (torch.arange(L) * step).clamp(max=40.0)[None, None, :, None] * unit
         compare(q, k.half(), v.half())
+
+
+# ------------------------------------------------------------------ queries
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("large", [4, 64, 8192])
+def test_one_large_channel_of_the_query_costs_the_others_nothing(D, large, dtype):
+    """A channel that the keys do not use is 1, 16 and 2048 times the next largest one: multiples of 1/32
+    next to 127/32 * large / 4 are exact in 24 bits."""
+    for L, N, Hq in ((17, 1, 8), (1000, 3, 6)):
+        q = exact_query((2, Hq, N, D), 1, dtype)
+        q[0, :, :, 5] = 127 / 32 * large / 4
+        q[1, ::2, :, D - 3] = -127 / 32 * large / 4
+        k, v = rand((2, 2, L, D), 2, dtype), rand((2, 2, L, D), 3, dtype)
+        k[..., 5], k[..., D - 3] = 0, 0
+        compare(q, k, v, [L, L // 2 + 3])
+
+
+def test_a_row_does_not_depend_on_the_rows_beside_it():
+    """Rows with a large channel, zeros and NaNs among the eight rows of a unit."""
+    L, D, dtype = 900, 128, torch.bfloat16
+    k, v = rand((1, 1, L, D), 1, dtype), rand((1, 1, L, D), 2, dtype)
+    cache, table = cache_of(k, v)
+    q = rand((1, 8, 1, D), 3, dtype).to(DEV)
+    want = gfa.attention_flash_gqa_kv4(q, cache, table, i32([L]), causal=True)
+    other = q.clone()
+    other[0, 1, 0, 7], other[0, 2], other[0, 5, 0, 0], other[0, 6, 0, 1] = 1e5, 0, math.nan, math.inf
+    got = gfa.attention_flash_gqa_kv4(other, cache, table, i32([L]), causal=True)
+    for h in (0, 3, 4, 7):
+        assert torch.equal(got[0, h], want[0, h])
+    assert torch.isfinite(got[0, 1:3]).all() and torch.isnan(got[0, 5:7]).all()
+
+
+@pytest.mark.parametrize("D,Hq,N,L", [(64, 4, 1, 3000), (512, 16, 1, 9000), (128, 32, 150, 600)])
+def test_bf16_keys_and_values_up_to_2_to_the_95(D, Hq, N, L):
+    """Queries times 2^-90 and keys times 2^90 give the same scores."""
+    dtype = torch.bfloat16
+    k, v = rand((1, 2, L, D), 1, dtype), rand((1, 2, L, D), 2, dtype)
+    q = rand((1, Hq, N, D), 3, dtype).to(DEV)
+    got = []
+    for pq, pk, pv in ((0, 0, 0), (-90, 90, 0), (0, 0, 92), (20, -20, -90)):
+        cache, table = cache_of(k * 2.0 ** pk, v * 2.0 ** pv)
+        o = gfa.attention_flash_gqa_kv4(q * 2.0 ** pq, cache, table, i32([L]), causal=True)
+        got.append(o.double() * 2.0 ** -pv)
+    for o in got[1:]:
+        assert torch.equal(o, got[0])
