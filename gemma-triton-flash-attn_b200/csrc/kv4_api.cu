@@ -106,9 +106,16 @@ struct AttendShape {
   int dense_rows, dense_batch;
 };
 
-// Bytes of K and V in 16 bits that the dense path holds at a time; it goes over
-// the batch in groups of requests beyond that (one at least).
-constexpr long long kDenseBytes = 2LL << 30;
+// Bytes that the dense path holds at a time, 2 GiB of K and V in 16 bits and the
+// bits that go with them (a 2048th); it goes over the batch in groups of requests
+// beyond that (one at least).
+constexpr long long kDenseBytes = (2LL << 30) + (1LL << 20);
+
+// Dense path: K and V [batch][Hkv][rows][D] 16-bit, then the bits of groups that
+// are not finite [batch][Hkv][kv4_nan_pitch].
+long long dense_bytes(int Hkv, long long rows, int D) {  // of one request
+  return Hkv * (4 * rows * D + 2 * kv4_nan_pitch(rows, D));
+}
 
 // Many query rows per KV head are bound by the products, not by the cache: then
 // the keys and values are written out in 16 bits once (exactly) and the tcgen05
@@ -160,31 +167,31 @@ AttendShape attend_shape(int B, int Hq, int Hkv, int N, int D, int max_len, int 
   s.ctas = static_cast<int>(std::min<long long>(2LL * sms, tiles(s.wide)));
   // the join: at most two CTAs per SM, all of them where few units are cut into many parts
   s.join_blocks = 1;
-  if (max_len > 0 && dense_path(B, Hq, Hkv, N, D, sms)) {
-    long long held = max_len;
-    if (window > 0) held = std::min<long long>(held, static_cast<long long>(window) + N + 15);
-    s.dense_rows = static_cast<int>((std::max<long long>(held, 1) + 15) / 16 * 16);
-    s.dense_batch = static_cast<int>(
-        std::min<long long>(B, std::max<long long>(1, kDenseBytes / (4LL * Hkv * s.dense_rows * D))));
+  long long held = max_len;
+  if (window > 0) held = std::min<long long>(held, static_cast<long long>(window) + N + 15);
+  const long long rows16 = (held + 15) / 16 * 16;
+  if (max_len > 0) {
+    const int batch =
+        static_cast<int>(std::min<long long>(B, std::max<long long>(1, kDenseBytes / dense_bytes(Hkv, rows16, D))));
+    if (dense_path(B, Hq, Hkv, N, D, sms)) {
+      s.dense_rows = static_cast<int>(rows16);
+      s.dense_batch = batch;
+    }
   }
   while (s.join_blocks < 8 * D / 128 && s.join_blocks * s.units <= sms) s.join_blocks *= 2;
   return s;
 }
 
-// Dense path: K and V [dense_batch][Hkv][dense_rows][D] 16-bit, then the bits of
-// groups that are not finite [dense_batch][Hkv][nan_pitch]. Else parts
-// [2 * ctas][8][D] fp32, their maxima and sums [2 * ctas][8].
-int nan_pitch(const AttendShape& s) { return (s.dense_rows / KV4_TOKENS * (s.D / KV4_GROUP) + 7) / 8 * 8; }
-long long dense_bytes(const AttendShape& s) {  // of one request
-  return s.Hkv * (4LL * s.dense_rows * s.D + 2LL * nan_pitch(s));
-}
+// Parts [2 * ctas][8][D] fp32, their maxima and sums [2 * ctas][8].
 long long part_bytes(const AttendShape& s, long long ctas) { return 2 * ctas * 8 * (s.D * 4LL + 8) + 256; }
 // Both ways' room, and never less for more keys: a caller's bound may lie above
 // the table's capacity, which the launch then takes for it.
 long long attend_workspace(const AttendShape& s) {
   long long need = part_bytes(s, s.part_ctas);
-  if (s.dense_batch)
-    need = std::max(need, s.dense_batch < s.B ? std::max(dense_bytes(s), kDenseBytes) : s.B * dense_bytes(s));
+  if (s.dense_batch) {
+    const long long one = dense_bytes(s.Hkv, s.dense_rows, s.D);
+    need = std::max(need, s.dense_batch < s.B ? std::max(one, kDenseBytes) : s.B * one);
+  }
   return need;
 }
 
@@ -504,10 +511,11 @@ extern "C" int gqafa_kv4_attend(const void* q, const long long* q_strides, const
   // A workspace that was sized for other arguments (max_kv_len 0, a window that a
   // call without causal does not use) may hold fewer requests at a time, or none:
   // then the units take the call.
-  if (s.dense_batch) s.dense_batch = static_cast<int>(std::min<long long>(s.dense_batch, workspace_bytes / dense_bytes(s)));
+  const long long one = dense_bytes(heads_kv, s.dense_rows, head_dim);
+  if (s.dense_batch) s.dense_batch = static_cast<int>(std::min<long long>(s.dense_batch, workspace_bytes / one));
   if (!s.dense_batch && s.units * (capacity / 64 + 2) > INT_MAX)
     return fail(GQAFA_ERR_INVALID, "B * H_Q * N times the block table's capacity out of range");
-  const long long need = s.dense_batch ? s.dense_batch * dense_bytes(s) : part_bytes(s, s.ctas);
+  const long long need = s.dense_batch ? s.dense_batch * one : part_bytes(s, s.ctas);
   if (workspace == nullptr || workspace_bytes < need)
     return fail(GQAFA_ERR_INVALID, "workspace of %lld bytes needed, got %lld", need, workspace_bytes);
   if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
@@ -536,8 +544,6 @@ extern "C" int gqafa_kv4_attend(const void* q, const long long* q_strides, const
       rd.q_lens = q_lens ? q_lens + b : nullptr;
       rd.out[0] = k;
       rd.out[1] = v;
-      rd.nans = v + static_cast<long long>(nb) * heads_kv * s.dense_rows * head_dim;
-      rd.nan_pitch = nan_pitch(s);
       if ((rc = launch_read<true, KV4_READ_UNITS>(rd, head_dim, bf16, st))) return rc;
       RaggedForward f{};
       f.q = static_cast<const uint16_t*>(q) + b * qs[0];
@@ -562,8 +568,7 @@ extern "C" int gqafa_kv4_attend(const void* q, const long long* q_strides, const
       f.bf16 = bf16;
       if ((rc = ragged_forward(f, st))) return rc;
       Kv4SpreadParams sp{};
-      sp.nans = rd.nans;
-      sp.nan_pitch = rd.nan_pitch;
+      sp.nans = v + static_cast<long long>(nb) * heads_kv * s.dense_rows * head_dim;
       sp.o = static_cast<uint16_t*>(f.o);
       sp.o_sb = os[0];
       sp.o_sh = os[1];

@@ -354,11 +354,15 @@ struct Kv4ReadParams {
   // to the end of its last key block.
   int q_rows, window;
   const int* q_lens;
-  // tokens of each (block, group) whose values are not finite, a bit each:
-  // [B * Hkv][nan_pitch], item (block from `start` on) * NG + group
-  uint16_t* nans;
-  int nan_pitch;
 };
+
+// Behind the values that are written out for the ragged forward: a bit for each
+// token of a (block, group) whose values are not finite, [B * Hkv][kv4_nan_pitch],
+// item (block from the first one on) * NG + group. rows: as many as are written
+// out, a multiple of 16.
+__host__ __device__ constexpr long long kv4_nan_pitch(long long rows, int head_dim) {
+  return (rows / KV4_TOKENS * (head_dim / KV4_GROUP) + 7) / 8 * 8;
+}
 
 constexpr int KV4_READ_UNITS = 4;  // groups of a block a warp reads, many of them
 
@@ -389,7 +393,7 @@ __device__ __forceinline__ uint4 kv4_values(uint32_t codes, uint32_t meta) {
 // L2 drops first took 72 us there instead of 75.
 //
 // For the ragged forward, whose MMAs also multiply masked keys' values by P = 0,
-// a value group that is NaN goes out as zeros, and a bit of `nans` tells
+// a value group that is NaN goes out as zeros, and a bit behind them tells
 // kv4_spread_nan_kernel to mark the rows that see it.
 template <int D, bool BF16, bool RAGGED, int UNITS>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
@@ -440,7 +444,11 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
       metas[k].x = __ldg(reinterpret_cast<const uint32_t*>(m + (lane >> 2) * 4));
     else
       metas[k] = __ldg(reinterpret_cast<const uint2*>(m + (lane >> 3) * 8));
-    if (RAGGED && kind == 1) {
+  }
+  if (RAGGED && kind == 1 && (static_cast<long long>(start) / 16 + item0 / NG) * 16 < end) {
+#pragma unroll
+    for (int k = 0; k < UNITS; ++k) {
+      const long long pos0 = (static_cast<long long>(start) / 16 + (item0 + k) / NG) * 16;
       const uint32_t word[4] = {metas[k].x & 0xFFFFu, metas[k].x >> 16, metas[k].y & 0xFFFFu, metas[k].y >> 16};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -455,8 +463,12 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
     const int g = (item0 + k) % NG;
     const long long pos0 = (static_cast<long long>(start) / 16 + (item0 + k) / NG) * 16;
     if (pos0 >= end) return;
-    if (RAGGED && kind == 1 && lane == 0)
-      p.nans[static_cast<long long>(bh) * p.nan_pitch + item0 + k] = static_cast<uint16_t>(bad[k]);
+    if (RAGGED && kind == 1 && k == 0 && lane == 0) {
+      static_assert(UNITS == 4 || !RAGGED, "four words of 16 bits; the pitch leaves room for those behind the last item");
+      *reinterpret_cast<uint2*>(p.out[1] + static_cast<long long>(p.B) * p.Hkv * p.n * D + bh * kv4_nan_pitch(p.n, D) +
+                                item0) = make_uint2(bad[0] | bad[UNITS > 1 ? 1 : 0] << 16,
+                                                    bad[UNITS > 2 ? 2 : 0] | bad[UNITS > 3 ? 3 : 0] << 16);
+    }
     uint16_t* out = p.out[kind] + (static_cast<long long>(b) * p.Hkv + h) * p.n * D + g * KV4_GROUP;
     auto value = [&](int r, uint32_t c, uint32_t m) {
       if (pos0 + r >= len) return make_uint4(0, 0, 0, 0);
@@ -503,8 +515,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
 
 // ------------------------------------------------------------------ NaNs
 struct Kv4SpreadParams {
-  const uint16_t* nans;  // as in Kv4ReadParams
-  int nan_pitch;
+  const uint16_t* nans;  // see kv4_nan_pitch
   uint16_t* o;
   long long o_sb, o_sh, o_sn;
   const int *kv_lens, *q_lens;
@@ -523,7 +534,7 @@ __global__ void __launch_bounds__(512) kv4_spread_nan_kernel(const Kv4SpreadPara
   const int b = blockIdx.x / p.Hkv, h = blockIdx.x - b * p.Hkv;
   const RaggedLens len = ragged_lens(p.kv_lens, p.q_lens, b, p.capacity, p.N, p.window);
   const int Nk = min(len.Nk, p.n), off = Nk - len.N;
-  const uint16_t* nans = p.nans + static_cast<long long>(blockIdx.x) * p.nan_pitch;
+  const uint16_t* nans = p.nans + blockIdx.x * kv4_nan_pitch(p.n, D);
   const int items = (Nk + 15) / 16 * NG;
   uint32_t any = 0;
   for (int i = threadIdx.x * 8; i < items; i += 512 * 8) {
