@@ -124,15 +124,20 @@ long long dense_bytes(int Hkv, long long rows, int D) {  // of one request
 // the MMAs above take 8 rows of all heads of a group and split the keys. Both
 // times grow with the keys: per key a unit of 8 rows costs the whole GPU 82, 46,
 // 29, 21 ps at head_dim 512, 256, 128, 64, a wave of 128-row tiles 20.6, 18.7,
-// 16.4, 18.0 ns. Measured on both sides of the rule, 2 requests of 7K keys, 32/4
+// 16.4, 18.0 ns; a group of `batch` requests is one launch, of one wave at least.
+// Measured on both sides of the rule, 2 requests of 7K keys, 32/4
 // heads, head_dim 512: 24 tokens 141 us in units and 171 us dense, 48 tokens 240
 // and 172 us; 8 requests, 16/4 heads, head_dim 64: 48 tokens 120 and 147 us, 100
-// tokens 231 and 148 us.
-bool dense_path(int B, int Hq, int Hkv, int N, int D, int sms) {
+// tokens 231 and 148 us; 64 requests of 4000 keys in a table for 131072, one a
+// group, 8/8 heads, head_dim 512: 64 tokens 1980 us and 12.9 ms (there the empty part
+// of the table costs the dense way more than the rule says: 256 tokens are dense,
+// 12.9 ms, where units would take about 8).
+bool dense_path(int B, int batch, int Hq, int Hkv, int N, int D, int sms) {
   const long long units = static_cast<long long>(B) * Hkv * ((static_cast<long long>(Hq / Hkv) * N + 7) / 8);
-  const long long tiles = static_cast<long long>(B) * Hq * ((N + 127) / 128) * (D == 512 ? 2 : 1);
+  const long long tiles = static_cast<long long>(batch) * Hq * ((N + 127) / 128) * (D == 512 ? 2 : 1);
+  const long long waves = static_cast<long long>((B + batch - 1) / batch) * ((tiles + sms - 1) / sms);
   const int ratio = D == 512 ? 250 : (D == 256 ? 400 : (D == 128 ? 560 : 860));
-  return units > ratio * ((tiles + sms - 1) / sms);
+  return units > ratio * waves;
 }
 
 // Units of 8 query rows, and the CTAs of the launch: two per SM, fewer where there
@@ -173,7 +178,7 @@ AttendShape attend_shape(int B, int Hq, int Hkv, int N, int D, int max_len, int 
   if (max_len > 0) {
     const int batch =
         static_cast<int>(std::min<long long>(B, std::max<long long>(1, kDenseBytes / dense_bytes(Hkv, rows16, D))));
-    if (dense_path(B, Hq, Hkv, N, D, sms)) {
+    if (dense_path(B, batch, Hq, Hkv, N, D, sms)) {
       s.dense_rows = static_cast<int>(rows16);
       s.dense_batch = batch;
     }

@@ -75,3 +75,19 @@ def test_size_call_refuses_what_the_launch_refuses():
     size = _lib.load().gqafa_kv4_attend_workspace_size
     assert size(1, 8, 3, 1, 128, 100, 0) == -1 and size(1, 8, 4, 1, 96, 100, 0) == -1
     assert size(1, 8, 4, 1, 128, -1, 0) == -1 and size(1, 8, 4, 1, 128, 100, -1) == -1
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,N,dense", [(6, 8, 8, 64, False), (6, 32, 4, 200, True)])
+def test_requests_that_are_written_out_one_at_a_time_count_a_launch_each(B, Hq, Hkv, N, dense):
+    """A table for 131072 tokens, head_dim 512: one request or two fill the 2 GiB, so six requests are several
+    launches of a wave each, which a few rows are not worth."""
+    D, capacity, lens = 512, 131072, [600, 240, 64, 0, 257, 333]
+    cache, table, held = filled(B, Hkv, D, 600, 64, torch.bfloat16, 31)
+    wide = torch.full((B, capacity // 64), -1, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    q = rand((B, Hq, N, D), 8, torch.bfloat16).to(DEV)
+    assert (size_of(q, cache, capacity, 0) >= 2 ** 30) == dense
+    assert (size_of(q, cache, 1024, 0) >= 2 ** 24) == (N >= 64)  # a short table: all in one launch
+    o = gfa.attention_flash_gqa_kv4(q, cache, wide, i32(lens), causal=True)
+    want, _, bound = kv4_ref.attention(q, *held, lens, [N] * B, True, 0, D ** -0.5)
+    assert ((o.double() - want).abs() <= bound).all()
