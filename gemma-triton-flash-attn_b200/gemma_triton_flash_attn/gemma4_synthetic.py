@@ -99,6 +99,8 @@ class DecoderKV4Cache:
 
     def __init__(self, cfg: Gemma4SyntheticConfig, max_batch: int, max_len: int, num_pages: int | None = None,
                  page_size: int = 64, dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        if max_batch <= 0 or max_len <= 0:
+            raise ValueError(f"sizes must be positive (max_batch={max_batch} max_len={max_len})")
         columns = -(-max_len // page_size)
         num_pages = max_batch * columns if num_pages is None else num_pages
         self.max_len, self.page_size = columns * page_size, page_size
@@ -224,13 +226,35 @@ class Gemma4SyntheticDecoder(nn.Module):
         x = self.norm(x)
         return x @ self.embed.weight.t()
 
+    def _check_step(self, input_ids, new_lens, cache):
+        rows = cache.kv_lens.shape[0]
+        if input_ids.dim() != 2:
+            raise ValueError(f"input_ids must be 2-D (B, N), got shape {tuple(input_ids.shape)}")
+        if input_ids.shape[0] != rows:
+            raise ValueError(f"input_ids has {input_ids.shape[0]} rows, the cache {rows}")
+        if input_ids.shape[1] == 0:
+            raise ValueError("input_ids holds no token")
+        if tuple(new_lens.shape) != (rows,):
+            raise ValueError(f"new_lens must have shape ({rows},), got {tuple(new_lens.shape)}")
+        if len(cache.layers) != len(self.layers):
+            raise ValueError(f"the cache has {len(cache.layers)} layers, the decoder {len(self.layers)}")
+        for i, (layer, pages) in enumerate(zip(self.layers, cache.layers)):
+            a = layer.attn
+            if (a.num_kv_heads, a.head_dim) != (pages.num_kv_heads, pages.head_dim):
+                raise ValueError(f"layer {i} has {a.num_kv_heads} KV heads of {a.head_dim}, the cache's "
+                                 f"{pages.num_kv_heads} of {pages.head_dim}")
+            dtype = a.k_proj.weight.dtype
+            if dtype != pages.dtype and not torch.is_autocast_enabled():
+                raise TypeError(f"layer {i} has dtype {dtype}, the cache's {pages.dtype}")
+
     @torch.no_grad()
     def step(self, input_ids, new_lens, cache: DecoderKV4Cache):
         """One serving step: input_ids (B, N) holds new_lens[b] (int32 CUDA, 0..N, negative: finished) new
         tokens of each of the cache's rows, padded to N. Returns the logits (B, N, vocab) (of padding and
-        refused requests: of no meaning) and the step's plan."""
-        n = input_ids.shape[1]
-        plan = cache.plan(new_lens, n)
+        refused requests: of no meaning) and the step's plan. Arguments that do not fit the cache are refused
+        before its tables and lengths move on."""
+        self._check_step(input_ids, new_lens, cache)
+        plan = cache.plan(new_lens, input_ids.shape[1])
         x = self.embed(input_ids) * (self.cfg.hidden_size ** 0.5)
         ropes = {}
         for layer, pages in zip(self.layers, cache.layers):
