@@ -362,6 +362,11 @@ extern "C" int gqafa_kv4_append(const void* k, const long long* k_strides, const
   int rc;
   if ((rc = check_cache(heads_kv, head_dim, page_size, dtype))) return rc;
   if (batch <= 0 || seqlen <= 0) return fail(GQAFA_ERR_INVALID, "sizes must be positive (B=%d N=%d)", batch, seqlen);
+  const long long units = static_cast<long long>(seqlen) * (head_dim / KV4_GROUP);  // (token, group) pairs
+  // the last CTA's pairs run up to 127 past the last one, in 32 bits
+  if (heads_kv > 65535 || batch > 65535 || units > INT_MAX - 127)
+    return fail(GQAFA_ERR_INVALID, "B (%d), heads_kv (%d) and tokens (%d) out of range (65535, 65535, and 2^31 - 128 "
+                "groups of 64 values)", batch, heads_kv, seqlen);
   if ((rc = check_pages(pages, num_pages, page_size))) return rc;
   if ((rc = check_ints("slot_map", slot_map))) return rc;
   if (slot_stride < 0) return fail(GQAFA_ERR_INVALID, "slot_map: negative row stride");
@@ -388,10 +393,6 @@ extern "C" int gqafa_kv4_append(const void* k, const long long* k_strides, const
   p.num_slots = static_cast<int>(num_pages * page_size);
   p.status = status_ptr();
   if (!p.status) return fail(GQAFA_ERR_CUDA, "cannot resolve the device status word");
-  const long long units = static_cast<long long>(seqlen) * (head_dim / KV4_GROUP);  // (token, group) pairs
-  if (heads_kv > 65535 || batch > 65535 || units > INT_MAX)
-    return fail(GQAFA_ERR_INVALID, "B (%d), heads_kv (%d) and tokens (%d) out of range (65535, 65535, 2^28)", batch,
-                heads_kv, seqlen);
   const int sms = sm_count();
   if (sms <= 0) return fail(GQAFA_ERR_CUDA, "cannot read the device's multiprocessor count");
   // Few groups: four lanes each, the shorter way through (at head_dim 256, 8 heads:
