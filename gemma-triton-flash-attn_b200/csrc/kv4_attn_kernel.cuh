@@ -600,7 +600,9 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
       const int i = qi + k * RSTEP;
       const int bits = sMost[min(i, ROWS - 1)];
       const float most = __int_as_float(bits);
-      const float up = fminf(32512.f / most, 1e38f);  // 1e38 for a row of zeros: its integers are 0
+      // an integer's worth, and integers per unit: 1e-38 at least, whose reciprocal
+      // is still a number (a row of zeros: its integers are 0)
+      const float worth = fmaxf(most / 32512.f, 1e-38f), up = fminf(32512.f / most, 1e38f);
       float x[8];
       load8(raw[k], x);
       int v[8], third[8], sum = 0, sum3 = 0, abs = 0;
@@ -637,7 +639,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) kv4_attn_kernel(co
           if (bits < 0x7F800000) atomicAdd(&sAbs[i], abs);
         }
         // a row with an infinity or a NaN has no finite scores
-        if (qc == 0) sScale[i] = bits >= 0x7F800000 ? NAN : p.scale_log2 * (most / 32512.f);
+        if (qc == 0) sScale[i] = bits >= 0x7F800000 ? NAN : p.scale_log2 * worth;
       }
     }
     if (threadIdx.x < ROWS) {

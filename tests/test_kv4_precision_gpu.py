@@ -205,3 +205,25 @@ def test_bf16_keys_and_values_up_to_2_to_the_95(D, Hq, N, L):
         got.append(o.double() * 2.0 ** -pv)
     for o in got[1:]:
         assert torch.equal(o, got[0])
+
+
+def test_queries_too_small_for_a_reciprocal():
+    """32512 / max|q| passes fp32's range below 2^-113: the query's integers are then fewer, not wrong."""
+    L, D, dtype = 500, 128, torch.bfloat16
+    k, v = rand((1, 1, L, D), 1, dtype), rand((1, 1, L, D), 2, dtype)
+    q = rand((1, 8, 1, D), 3, dtype).to(DEV)
+    got = []
+    for pq, pk, factor in ((0, 0, 1.0), (-115, 90, 2.0 ** 25)):
+        cache, table = cache_of(k * 2.0 ** pk, v)
+        got.append(gfa.attention_flash_gqa_kv4(q * 2.0 ** pq, cache, table, i32([L]), causal=True,
+                                               softmax_scale=factor * D ** -0.5).double())
+    # steps of 1e-38 on queries of 2^-115: a score off by at most D^-0.5 * 2^24 * 1e-38 * sum |k| < 1e-2
+    assert (got[1] - got[0]).abs().max() <= 2 * 1e-2 * v.double().abs().max()
+    assert got[0].abs().max() > 0.1
+
+
+def test_an_all_zero_query_weighs_every_key_alike():
+    L, D = 333, 256
+    for dtype in (torch.bfloat16, torch.float16):
+        k, v = rand((1, 2, L, D), 1, dtype), rand((1, 2, L, D), 2, dtype)
+        compare(torch.zeros(1, 4, 2, D, dtype=dtype, device=DEV), k, v)
