@@ -167,11 +167,13 @@ AttendShape attend_shape(int B, int Hq, int Hkv, int N, int D, int max_len, int 
   // 12.8, at 64 10.4 and 11.4. Else long ones, fewer barriers: 8 requests at 256
   // 15.2 us against 16.8, at 128 13.7 and 14.8; 16 requests of 8K to 16K keys, 32/4
   // heads, at 256 65.3 and 69.7, at 128 43.5 and 49.6, at 64 32.8 and 34.3. At 512
-  // one block a warp is the best of both: with two, 114.8 us against 105.8.
+  // one block a warp is the best of both: with two, 114.8 us against 105.8. (All
+  // before the query's third byte, which added about 2 %.) Few units lose CTAs at
+  // the change, but no time: one request of 32/4 heads at 128, 9216 keys in 296 CTAs
+  // 12.7 us, 9472 in 80 12.3; 16/2 heads, 18800 keys 13.5, 19000 12.2; at 256 9216
+  // keys 13.7, 9472 14.2.
   s.wide = D != 512 && tiles(false) > 2LL * sms;
   s.ctas = static_cast<int>(std::min<long long>(2LL * sms, tiles(s.wide)));
-  // the join: at most two CTAs per SM, all of them where few units are cut into many parts
-  s.join_blocks = 1;
   long long held = max_len;
   if (window > 0) held = std::min<long long>(held, static_cast<long long>(window) + N + 15);
   const long long rows16 = (held + 15) / 16 * 16;
@@ -183,6 +185,8 @@ AttendShape attend_shape(int B, int Hq, int Hkv, int N, int D, int max_len, int 
       s.dense_batch = batch;
     }
   }
+  // the join: at most two CTAs per SM, all of them where few units are cut into many parts
+  s.join_blocks = 1;
   while (s.join_blocks < 8 * D / 128 && s.join_blocks * s.units <= sms) s.join_blocks *= 2;
   return s;
 }

@@ -35,7 +35,8 @@
 // before a tile's barrier, a word per thread; a larger one is published as a
 // raised maximum is. That costs 109 us against 104 at head_dim 512, 16 requests of
 // 8K to 16K keys, 46.5 against 42.6 at 128 (each warp looking after its own groups
-// in the value loop, with a power for each: 113 and 49.5).
+// in the value loop, with a power for each: 113 and 49.5). Groups whose scales are
+// below 2^-10 of the head's largest have that much less room.
 // bf16 needs none of it.
 //
 // Shape. A decode step has G = H_Q / H_KV query rows per KV head, far below
@@ -57,14 +58,15 @@
 // The ninth warp costs registers (96 a thread, two CTAs per SM, instead of 128),
 // but warp 0 issuing the copies between its own tiles delays the other seven:
 // 130 us against 106 at head_dim 512, 16 requests of 8K to 16K keys, 54 against
-// 38 at head_dim 128. A producer warpgroup that gives its registers away (104 for the
-// others) made the first 1 % faster and the second 5 % slower.
+// 38 at head_dim 128 (both before the third byte and fp16's power of two). A producer
+// warpgroup that gives its registers away (104 for the others) made the first 1 %
+// faster and the second 5 % slower.
 //
-// Measured: 16 requests of 8K to 16K keys, 32/4 heads, head_dim 512: 106 us for 430
-// MB of codes, 4.0 TB/s; 131072 keys of one request, 16/2 heads: 44.5 us, 3.2 TB/s.
-// Bound by neither alone: 58 % of the issue slots, 56 % of the ALU; without the
-// products the first takes 83 us. 20 rows at head_dim 128 (three units): 38 us,
-// bound by instructions.
+// Measured: 16 requests of 8K to 16K keys, 32/4 heads, head_dim 512: 107.8 us for 430
+// MB of codes, 4.0 TB/s (fp16 111); 131072 keys of one request, 16/2 heads: 46.0 us,
+// 3.1 TB/s. Bound by neither alone: 57 % of the issue slots, 56 % of the ALU
+// (profiles/kv4_decode_d512.md); without the products the first took 83 us. 20 rows
+// at head_dim 128 (three units): 40.4 us, fp16 43.6, bound by instructions.
 //
 // Split. The tiles of all (request, row tile, KV head) units form one list,
 // cut into equal contiguous shares, one per CTA: ragged lengths and a single

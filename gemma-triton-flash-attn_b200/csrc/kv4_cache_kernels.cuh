@@ -385,12 +385,13 @@ __device__ __forceinline__ uint4 kv4_values(uint32_t codes, uint32_t meta) {
 // group, as stored; all loads in flight together) and writes 16 tokens x 64
 // values of each: 128 contiguous bytes per token. blockIdx.x: request, head and
 // 8 * UNITS (block, group) pairs; blockIdx.y: keys / values. Rows behind a
-// request's last token become zeros. Bound by the writes, 79 % of the bytes:
-// 16384 tokens of 8 heads at head_dim 256 take 36 us, 4.7 TB/s; a plain fill of as
-// many bytes as are written takes 38. (Key stores of 16 bytes, half a sector each:
-// 42 us. Two or eight groups a warp instead of four: 7 and 3 % more over five
-// ragged caches of up to 16384 tokens, 8 heads at head_dim 128.) Stores that the
-// L2 drops first took 72 us there instead of 75.
+// request's last token become zeros. Mostly writes, 79 % of the bytes: 16384 tokens
+// of 8 heads at head_dim 256 take 34.8 us, 4.9 TB/s read and written, five ragged
+// caches of up to 16384 tokens at head_dim 128 5.3 TB/s, of the copy's 6.6. (Key
+// stores of 16 bytes, half a sector each: 42 us. Two or eight groups a warp instead
+// of four: 7 and 3 % more over the ragged caches.) Stores that the L2 drops first
+// took 72 us there instead of 75. Not gone into: `p.out[kind]` makes every thread
+// copy the parameters to local memory first.
 //
 // For the ragged forward, whose MMAs also multiply masked keys' values by P = 0,
 // a value group that is NaN goes out as zeros, and a bit behind them tells

@@ -171,7 +171,7 @@ def kv4_append(cache: KV4Cache, k, v, slot_map) -> None:
 def kv4_read(cache: KV4Cache, block_table, kv_lens, max_len: int, starts=None):
     """Cached keys and values as dense (B, H_KV, max_len, D) tensors.
 
-    Row i of request b is position starts[b] + i (starts None: 0), zeros from
+    Row i of request b is position starts[b] + i (starts None or negative: 0), zeros from
     kv_lens[b] on. The values are exactly those that the attention uses, so a
     prompt that attends to them through ``attention_flash_gqa`` sees what its
     later decode steps will see."""

@@ -204,7 +204,8 @@ GQAFA_API int gqafa_bwd_stage_rows(int stage, const void* q, const long long* q_
  * Lengths, tables and slots are read on the device, so a captured graph can be
  * replayed with new ones. Entries that are out of range never leave the given
  * arrays: a slot outside the cache is skipped, a page outside the pool is
- * replaced by page 0, a length beyond the block table is clamped to it; the
+ * replaced by page 0 (read as zeros by gqafa_kv4_read and by attention of many
+ * rows), a length beyond the block table is clamped to it; the
  * first such entry is recorded in the status word (gqafa_device_status: 16
  * page, 17 slot, 18 length), and the results of that request are undefined.
  * Nothing is allocated and nothing synchronises.
@@ -239,8 +240,8 @@ GQAFA_API int gqafa_kv4_append(const void* k, const long long* k_strides, const 
                                int heads_kv, int seqlen, int head_dim, int page_size, int dtype, void* stream);
 
 /* Cached keys and values as contiguous [batch, heads_kv, seqlen, head_dim]
- * tensors (32-byte aligned): row i of request b is position starts[b] + i (starts NULL: 0), zeros
- * from kv_lens[b] on. */
+ * tensors (32-byte aligned): row i of request b is position starts[b] + i
+ * (starts NULL or negative: 0), zeros from kv_lens[b] on. */
 GQAFA_API int gqafa_kv4_read(const void* pages, long long num_pages, const int* block_table, long long table_stride,
                              int cols, const int* kv_lens, const int* starts, void* k, void* v, int batch,
                              int heads_kv, int seqlen, int head_dim, int page_size, int dtype, void* stream);
