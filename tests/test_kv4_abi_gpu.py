@@ -91,3 +91,26 @@ def test_requests_that_are_written_out_one_at_a_time_count_a_launch_each(B, Hq, 
     o = gfa.attention_flash_gqa_kv4(q, cache, wide, i32(lens), causal=True)
     want, _, bound = kv4_ref.attention(q, *held, lens, [N] * B, True, 0, D ** -0.5)
     assert ((o.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("D", [128, 512])
+@pytest.mark.parametrize("fits", [1, 2, 3])
+def test_a_workspace_for_fewer_requests_at_a_time_gives_the_same_bits(fits, D):
+    """Groups of one and two requests of three, with a NaN in a value group of each."""
+    B, Hq, Hkv, N, L = 3, 32, 4, 200, 600
+    cache, table, _ = filled(B, Hkv, D, L, 64, torch.bfloat16, 4)
+    bad = rand((B, Hkv, 1, D), 5, torch.bfloat16).to(DEV)
+    bad[0, 1, 0, 5], bad[1, 2, 0, D - 1], bad[2, 0, 0, 64] = float("nan"), float("inf"), -float("inf")
+    page = table[:, 400 // 64].tolist()
+    gfa.kv4_append(cache, bad, bad.nan_to_num(0, 0, 0), i32([[p * 64 + 400 % 64] for p in page]))  # keys first
+    gfa.kv4_append(cache, bad.nan_to_num(0, 0, 0), bad, i32([[p * 64 + 400 % 64] for p in page]))
+    q, lens = rand((B, Hq, N, D), 2, torch.bfloat16).to(DEV), i32([L, 450, 590])
+    want = gfa.attention_flash_gqa_kv4(q, cache, table, lens, causal=True)
+    assert torch.isnan(want).any() and torch.isfinite(want).any()
+    capacity = table.shape[1] * 64
+    whole = size_of(q, cache, capacity, 0)
+    one = Hkv * capacity * (4 * D + D / 512)  # K, V and a bit for each token and group
+    assert whole == 3 * one
+    rc, o = attend(q, cache, table, lens, capacity, True, 0, int(one) * fits)
+    assert rc == _lib.GQAFA_OK
+    assert torch.equal(o.nan_to_num(1e9), want.nan_to_num(1e9)) and torch.equal(torch.isnan(o), torch.isnan(want))

@@ -107,3 +107,16 @@ def test_a_row_sees_the_same_nans_in_a_chunk_and_alone(Hq, Hkv, N):
     for row in (0, 1, N - 1):
         one, _ = run(k, v, q[:, :, row:row + 1], [L - N + 1 + row], [1], True, 25)
         assert torch.equal(torch.isnan(one), torch.isnan(o[:, :, row:row + 1]))
+
+
+def test_nans_go_to_the_rows_of_a_strided_output():
+    """Queries (and outputs) as a projection leaves them, (B, N, H, D) in memory."""
+    B, Hq, Hkv, N, L, D, dtype = 2, 32, 4, 160, 300, 128, torch.bfloat16
+    k, v = rand((B, Hkv, L, D), 1, dtype), rand((B, Hkv, L, D), 2, dtype)
+    v[0, 2, 200, 70], v[1, 3, 250, 1] = math.nan, math.inf
+    base = rand((B, N, Hq, D), 3, dtype).to(DEV)
+    for causal, window in CASES:
+        want, _ = run(k, v, base.transpose(1, 2).contiguous(), [L, 299], [N, 100], causal, window)
+        o, _ = run(k, v, base.transpose(1, 2), [L, 299], [N, 100], causal, window)
+        assert o.stride() == base.transpose(1, 2).stride() and torch.isnan(o).any()
+        assert torch.equal(torch.isnan(o), torch.isnan(want)) and torch.equal(o.nan_to_num(0), want.nan_to_num(0))

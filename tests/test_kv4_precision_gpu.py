@@ -227,3 +227,29 @@ def test_an_all_zero_query_weighs_every_key_alike():
     for dtype in (torch.bfloat16, torch.float16):
         k, v = rand((1, 2, L, D), 1, dtype), rand((1, 2, L, D), 2, dtype)
         compare(torch.zeros(1, 4, 2, D, dtype=dtype, device=DEV), k, v)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("value", [0.0, 1.0, -0.37])
+def test_constant_values_come_back(D, value, dtype):
+    """The offset of the codes cancels: zeros are exactly zeros, whatever the weights."""
+    L = 3001
+    k, v = rand((1, 2, L, D), 1, dtype, 2.0), torch.full((1, 2, L, D), value, dtype=dtype)
+    q = exact_query((1, 8, 3, D), 3, dtype)
+    o, want, _ = compare(q, k, v)
+    if value == 0:
+        assert (o == 0).all()
+    assert (want - want.flatten()[0]).abs().max() < 1e-12
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=ids)
+def test_groups_of_very_different_size_in_one_head(dtype):
+    """One dim group a thousand times the other, either way round, and rows of one token."""
+    L, D = 2000, 128
+    k, q = rand((2, 1, L, D), 1, dtype), exact_query((2, 8, 1, D), 2, dtype)
+    v = 1 + 0.5 * rand((2, 1, L, D), 3, torch.float32)
+    v[0, ..., :64] *= 2.0 ** -10
+    v[1, ..., 64:] *= 2.0 ** 9
+    compare(q, k, v.to(dtype), [L, 1])
+    compare(q, k, v.to(dtype), [1, L])
