@@ -520,9 +520,14 @@ extern "C" int gqafa_kv4_attend(const void* q, const long long* q_strides, const
   AttendShape s = attend_shape(batch, heads_q, heads_kv, seqlen_q, head_dim, max_kv_len, win, sms);
   // A workspace that was sized for other arguments (max_kv_len 0, a window that a
   // call without causal does not use) may hold fewer requests at a time, or none:
-  // then the units take the call.
+  // then the units take the call, and also where groups so small do not pay.
   const long long one = dense_bytes(heads_kv, s.dense_rows, head_dim);
-  if (s.dense_batch) s.dense_batch = static_cast<int>(std::min<long long>(s.dense_batch, workspace_bytes / one));
+  if (s.dense_batch && workspace_bytes / one < s.dense_batch) {
+    s.dense_batch = static_cast<int>(std::max<long long>(0, workspace_bytes / one));
+    if (s.dense_batch && workspace_bytes >= part_bytes(s, s.ctas) &&
+        !dense_path(batch, s.dense_batch, heads_q, heads_kv, seqlen_q, head_dim, sms))
+      s.dense_batch = 0;
+  }
   if (!s.dense_batch && s.units * (capacity / 64 + 2) > INT_MAX)
     return fail(GQAFA_ERR_INVALID, "B * H_Q * N times the block table's capacity out of range");
   const long long need = s.dense_batch ? s.dense_batch * one : part_bytes(s, s.ctas);

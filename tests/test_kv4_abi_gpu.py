@@ -114,3 +114,30 @@ def test_a_workspace_for_fewer_requests_at_a_time_gives_the_same_bits(fits, D):
     rc, o = attend(q, cache, table, lens, capacity, True, 0, int(one) * fits)
     assert rc == _lib.GQAFA_OK
     assert torch.equal(o.nan_to_num(1e9), want.nan_to_num(1e9)) and torch.equal(torch.isnan(o), torch.isnan(want))
+
+
+def test_groups_that_are_too_small_to_pay_are_not_made():
+    """24 requests whose keys and values fit the workspace one at a time: units of 8 rows, as the same call with
+    max_kv_len 0 in the size call; and no workspace, or a negative size, is refused."""
+    B, Hq, Hkv, N, D, L = 24, 8, 4, 48, 128, 300
+    cache, table, held = filled(B, Hkv, D, L, 64, torch.bfloat16, 4)
+    q, lens = rand((B, Hq, N, D), 2, torch.bfloat16).to(DEV), i32([L] * B)
+    capacity = table.shape[1] * 64
+    units = size_of(q, cache, 0, 0)
+    one = Hkv * capacity * (4 * D + D // 512)
+    assert size_of(q, cache, capacity, 0) > units > one
+    rc, o = attend(q, cache, table, lens, capacity, True, 0, units)
+    rc0, o0 = attend(q, cache, table, lens, 0, True, 0, units)
+    assert rc == rc0 == _lib.GQAFA_OK and torch.equal(o, o0)
+    dense = gfa.attention_flash_gqa_kv4(q, cache, table, lens, causal=True)
+    want, _, bound = kv4_ref.attention(q, *held, [L] * B, [N] * B, True, 0, D ** -0.5)
+    for got in (o, dense):
+        assert ((got.double() - want).abs() <= bound).all()
+    for bad in (0, -1, -2 ** 40):
+        lib = _lib.load()
+        rc = lib.gqafa_kv4_attend(
+            q.data_ptr(), _lib.strides_arg(q.stride()), cache.pages.data_ptr(), cache.num_pages, table.data_ptr(),
+            table.stride(0), table.shape[1], lens.data_ptr(), None, o.data_ptr(), _lib.strides_arg(o.stride()), None, B,
+            Hq, Hkv, N, D, cache.page_size, capacity, D ** -0.5, 1, 0, 1, dense.data_ptr(), bad,
+            torch.cuda.current_stream().cuda_stream)
+        assert rc == _lib.GQAFA_ERR_INVALID and b"workspace" in lib.gqafa_last_error()
